@@ -11,6 +11,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libbndm_hip.so")
+TOKENS_LIB_PATH = os.path.join(_HERE, "libbndm_tokens.so")
 
 MAX_LEVELS = 8
 
@@ -38,7 +39,17 @@ class UNetProfile(C.Structure):
                 ("dom_launches", C.c_int), ("dom_flops", C.c_double), ("dom_bytes", C.c_double)]
 
 
+class AttentionShape(C.Structure):
+    _fields_ = [
+        ("B", C.c_int64), ("Nq", C.c_int64), ("Nk", C.c_int64),
+        ("H", C.c_int), ("Hk", C.c_int), ("D", C.c_int), ("Dv", C.c_int),
+        ("q_strides", C.c_int64 * 3), ("k_strides", C.c_int64 * 3), ("v_strides", C.c_int64 * 3),
+        ("causal", C.c_int), ("dtype", C.c_int), ("lam_f32", C.c_int), ("scale", C.c_float),
+    ]
+
+
 _vp, _i, _f, _sz = C.c_void_p, C.c_int, C.c_float, C.c_size_t
+_l, _d = C.c_int64, C.c_double
 
 # name -> (restype, argtypes); mirrors include/bndm_hip.h one to one
 SIGNATURES = {
@@ -67,7 +78,22 @@ SIGNATURES = {
     "bndm_unet_profile": (_i, [_vp, _vp, _vp, _vp, _i, _i, C.POINTER(UNetProfile), _vp]),
 }
 
+# the same of include/bndm_tokens.h
+TOKENS_SIGNATURES = {
+    "bndm_tokens_abi_version": (_i, []),
+    "bndm_tokens_last_error": (C.c_char_p, []),
+    "bndm_tokens_linear": (_i, [_vp, _l, _vp, _vp, _vp, _l, _vp, _vp, _l, _l, _l, _i, _i, _vp]),
+    "bndm_tokens_linear_backward_workspace_bytes": (_sz, [_l, _l, _l, _i, _i]),
+    "bndm_tokens_linear_backward": (_i, [_vp, _l, _vp, _vp, _l, _vp, _vp, _vp, _vp, _l, _l, _l, _i, _i, _vp, _sz, _vp]),
+    "bndm_tokens_rotary": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _l, _l, _i, _vp, _i, _d, _i, _i, _i, _vp]),
+    "bndm_tokens_attention_workspace_bytes": (_sz, [C.POINTER(AttentionShape)]),
+    "bndm_tokens_attention": (_i, [C.POINTER(AttentionShape), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "bndm_tokens_attention_backward_workspace_bytes": (_sz, [C.POINTER(AttentionShape)]),
+    "bndm_tokens_attention_backward": (_i, [C.POINTER(AttentionShape)] + [_vp] * 16 + [_sz, _vp]),
+}
+
 _lib = None
+_tokens = None
 
 
 class BndmError(RuntimeError):
@@ -93,12 +119,40 @@ def load():
     return lib
 
 
+def load_tokens():
+    """dlopen the library of the operators over tokens (once).  Raises if it has not been built."""
+    global _tokens
+    if _tokens is not None:
+        return _tokens
+    if not os.path.exists(TOKENS_LIB_PATH):
+        raise BndmError(
+            f"{TOKENS_LIB_PATH} not found: the HIP extension is required (no CPU fallback). "
+            "Build it with `make -C bndm_amd/csrc` or __graft_entry__.build().")
+    lib = C.CDLL(TOKENS_LIB_PATH)
+    for name, (res, args) in TOKENS_SIGNATURES.items():
+        fn = getattr(lib, name)
+        fn.restype, fn.argtypes = res, args
+    if lib.bndm_tokens_abi_version() != 1:
+        raise BndmError("libbndm_tokens.so ABI version mismatch")
+    _tokens = lib
+    return lib
+
+
+def _raise(rc: int, what: str, error: bytes):
+    msg = error.decode("utf-8", "replace")
+    if rc == -1:
+        raise NotImplementedError(f"{what}: {msg}")
+    raise BndmError(f"{what} failed (code {rc}): {msg}")
+
+
 def check(rc: int, what: str):
     if rc != 0:
-        msg = load().bndm_last_error().decode("utf-8", "replace")
-        if rc == -1:
-            raise NotImplementedError(f"{what}: {msg}")
-        raise BndmError(f"{what} failed (code {rc}): {msg}")
+        _raise(rc, what, load().bndm_last_error())
+
+
+def check_tokens(rc: int, what: str):
+    if rc != 0:
+        _raise(rc, what, load_tokens().bndm_tokens_last_error())
 
 
 def current_stream_ptr():
