@@ -82,7 +82,8 @@ SIGNATURES = {
 TOKENS_SIGNATURES = {
     "bndm_tokens_abi_version": (_i, []),
     "bndm_tokens_last_error": (C.c_char_p, []),
-    "bndm_tokens_linear": (_i, [_vp, _l, _vp, _vp, _vp, _l, _vp, _vp, _l, _l, _l, _i, _i, _vp]),
+    "bndm_tokens_linear_workspace_bytes": (_sz, [_l, _l, _l]),
+    "bndm_tokens_linear": (_i, [_vp, _l, _vp, _vp, _vp, _l, _vp, _vp, _l, _l, _l, _i, _i, _vp, _sz, _vp]),
     "bndm_tokens_linear_backward_workspace_bytes": (_sz, [_l, _l, _l, _i, _i]),
     "bndm_tokens_linear_backward": (_i, [_vp, _l, _vp, _vp, _l, _vp, _vp, _vp, _vp, _l, _l, _l, _i, _i, _vp, _sz, _vp]),
     "bndm_tokens_rotary": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _l, _l, _i, _vp, _i, _d, _i, _i, _i, _vp]),

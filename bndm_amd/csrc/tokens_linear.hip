@@ -5,30 +5,49 @@
 //   dW        dW[n][k] = sum_m dz[m][n] x[m][k]       both hold it across their rows
 //
 // One kernel takes all three: an operand whose rows run along the summed index is read from LDS as rows, one whose rows run across it
-// by transposing LDS reads, so no operand is copied into another layout first.
+// by transposing LDS reads, so no operand is copied into another layout first.  Few rows go to a kernel of their own, which reads the
+// weights straight into registers.
 #include "tokens_common.hpp"
 
 namespace bndm {
 namespace {
 
 // ---------------------------------------------------------------------------------------------- activation
-// Phi(z): erfcf's error is relative, which 1 + erf(z) loses for negative z
+// Phi(-|z|) = exp(-z^2 / 2) t P(t) / 2 with t = 1 / (1 + 0.3 |z| / sqrt 2): P was fitted to exp(x^2) erfc(x) over x >= 0, least largest
+// relative error 2.0e-8 in exact arithmetic, 4.9e-7 in 32 bits, in the far tail too, where 1 + erf(z) has nothing left.
+struct Gauss { float below, density; };          // Phi(z), exp(-z^2 / 2) / sqrt(2 pi)
+__device__ __forceinline__ Gauss gauss(float z) {
+    const float t = __builtin_amdgcn_rcpf(1.0f + 0.21213203435596426f * fabsf(z));
+    const float e = __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);
+    float p = -0.12952277064323425f;
+    p = __builtin_fmaf(p, t, 0.4855625629425049f);
+    p = __builtin_fmaf(p, t, -0.5122767686843872f);
+    p = __builtin_fmaf(p, t, 0.5477185845375061f);
+    p = __builtin_fmaf(p, t, -0.09464973956346512f);
+    p = __builtin_fmaf(p, t, 0.2149256467819214f);
+    p = __builtin_fmaf(p, t, 0.14833927154541016f);
+    p = __builtin_fmaf(p, t, 0.17071521282196045f);
+    p = __builtin_fmaf(p, t, 0.1691880077123642f);
+    const float tail = 0.5f * p * t * e;
+    return {z < 0.f ? tail : 1.0f - tail, 0.39894228040143268f * e};
+}
+__device__ __forceinline__ float logistic(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * z)); }
+
 __device__ __forceinline__ float act_value(int act, float z) {
-    if (act == BNDM_ACT_SILU) return z / (1.0f + __expf(-z));
-    if (act == BNDM_ACT_GELU) return 0.5f * z * erfcf(-0.70710678118654752f * z);
+    if (act == BNDM_ACT_SILU) return z * logistic(z);
+    if (act == BNDM_ACT_GELU) return z * gauss(z).below;
     return z;
 }
 __device__ __forceinline__ float act_slope(int act, float z) {
     if (act == BNDM_ACT_SILU) {
-        const float s = 1.0f / (1.0f + __expf(-z));
+        const float s = logistic(z);
         return s * (1.0f + z * (1.0f - s));
     }
-    return 0.5f * erfcf(-0.70710678118654752f * z) + 0.39894228040143268f * z * __expf(-0.5f * z * z);
+    const Gauss g = gauss(z);
+    return __builtin_fmaf(z, g.density, g.below);
 }
 
-// ---------------------------------------------------------------------------------------------- the product
-// C[m][n] = sum_k A(m, k) B(n, k).  TA false: A(m, k) = a[m * lda + k]; true: a[k * lda + m]; TB likewise.
-// The B operand's index runs down the registers of a result tile, so a lane holds 4 consecutive n of one row m.
+// ---------------------------------------------------------------------------------------------- what is done with a result
 struct Epilogue {
     const void *bias;
     const void *residual;
@@ -37,246 +56,546 @@ struct Epilogue {
     int act;
 };
 
-constexpr int BM = 128, BN = 128, BK = 64;
-constexpr int NT = 256;
-
-template <typename T> __device__ __forceinline__ void store_row4(const Epilogue &e, T *c, int64_t ldc, int64_t m, int64_t n, int64_t M, int64_t N,
-                                                                 f32x4 v, bool wide) {
-    if (m >= M || n >= N) return;
-    const int left = (int)min((int64_t)4, N - n);
-    float bias[4] = {0.f, 0.f, 0.f, 0.f}, res[4] = {0.f, 0.f, 0.f, 0.f};
-    if (wide) {                                            // n % 4 == 0, N % 4 == 0, rows of 8-byte pieces
-        if (e.bias) {
-            const s16x4 b = *reinterpret_cast<const s16x4 *>((const T *)e.bias + n);
+// N_ consecutive results of row m from column n on; WIDE: all of them are inside, and everything is in pieces of 16 bytes
+template <typename T> __device__ __forceinline__ void load8_of(float (&to)[8], const T *from) {
+    const s16x8 v = *reinterpret_cast<const s16x8 *>(from);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { const short s = b[i]; bias[i] = widen<T>(s); }
-        }
-        if (e.residual) {
-            const s16x4 r = *reinterpret_cast<const s16x4 *>((const T *)e.residual + m * e.ldr + n);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { const short s = r[i]; res[i] = widen<T>(s); }
-        }
+    for (int i = 0; i < 8; ++i) { const short s = v[i]; to[i] = widen<T>(s); }
+}
+template <typename T> __device__ __forceinline__ void finish8(const Epilogue &e, T *c, int64_t m, int64_t n, int64_t N, float (&v)[8], bool wide) {
+    const int left = (int)min((int64_t)8, N - n);
+    float bias[8] = {}, res[8] = {};
+    if (wide) {
+        if (e.bias) load8_of<T>(bias, (const T *)e.bias + n);
+        if (e.residual) load8_of<T>(res, (const T *)e.residual + m * e.ldr + n);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 8; ++i)
             if (i < left) {
                 if (e.bias) bias[i] = (float)((const T *)e.bias)[n + i];
                 if (e.residual) res[i] = (float)((const T *)e.residual)[m * e.ldr + n + i];
             }
     }
-    float y[4];
+    float y[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[i] += bias[i];
-        y[i] = act_value(e.act, v[i]) + res[i];
+    for (int i = 0; i < 8; ++i) v[i] += bias[i];
+    if (e.act == BNDM_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = act_value(BNDM_ACT_SILU, v[i]) + res[i];
+    } else if (e.act == BNDM_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = act_value(BNDM_ACT_GELU, v[i]) + res[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = v[i] + res[i];
     }
     if (wide) {
-        if (e.z) *reinterpret_cast<s16x4 *>((T *)e.z + m * N + n) = pack4<T>(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<s16x4 *>(c + m * ldc + n) = pack4<T>(y[0], y[1], y[2], y[3]);
+        if (e.z) *reinterpret_cast<s16x8 *>((T *)e.z + m * N + n) = pack8<T>(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
+        *reinterpret_cast<s16x8 *>(c + m * N + n) = pack8<T>(y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 8; ++i)
             if (i < left) {
                 if (e.z) ((T *)e.z)[m * N + n + i] = (T)v[i];
-                c[m * ldc + n + i] = (T)y[i];
+                c[m * N + n + i] = (T)y[i];
             }
     }
 }
 
-// one operand's tile of 128 rows x 64 of the summed index, 16 KB, in 16-byte chunks whose places are swizzled
-//   rows along the summed index: [128][8 chunks];  across it: [64][16 chunks]
-template <typename T, bool TR, bool WIDE>
-__device__ __forceinline__ void stage(char *lds, const T *p, int64_t ld, int64_t row0, int64_t rows, int64_t k0, int64_t K, int tid) {
-    constexpr int C = TR ? 16 : 8;
-    const int64_t outer0 = TR ? k0 : row0, inner0 = TR ? row0 : k0;
-    const int64_t outers = (TR ? K : rows) - outer0, inners = (TR ? rows : K) - inner0;   // what is there, from here on
-    const T *base = p + outer0 * ld + inner0;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    if constexpr (WIDE) {
+// ---------------------------------------------------------------------------------------------- the product
+// C[m][n] = sum_k A(m, k) B(n, k).  TA false: A(m, k) = a[m * lda + k]; true: a[k * lda + m]; TB likewise.
+// B's index runs down the registers of a result tile, in an order that gives a lane 16 consecutive n of one row m.
+constexpr int BK = 64;
+
+struct Product {
+    const void *a, *b;
+    void *c;                       // [M][N]
+    float *part;                   // splits > 1: [splits][M][N] sums of the parts of K
+    int64_t lda, ldb, M, N, K;
+    int64_t split_k;               // summed index of a part, a multiple of BK
+    int tiles_m, tiles_n, tiles, splits, wide_out;
+};
+
+// ROWS of one operand x 64 of the summed index in LDS, 16-byte chunks in swizzled places: rows along the summed index: [ROWS][8 chunks];
+// across it: [64][ROWS / 8 chunks].  Copied by THREADS threads.
+template <typename T, bool TR, int ROWS, int THREADS> struct Operand {
+    static constexpr int C = TR ? ROWS / 8 : 8;
+    static constexpr int N = ROWS * 8 / THREADS;              // chunks of a thread
+    static constexpr int STEP = THREADS / C;                  // rows between them; a multiple of the swizzle's period
+    static_assert(STEP % (TR ? 16 : 32) == 0, "one swizzle for all chunks of a thread");
+
+    const char *base;              // where the tile of this step begins
+    int64_t step_bytes;
+    int row, c;                    // of the thread's first chunk
+    int ld;
+    int64_t rows_in, inner_in;     // what is there from the first tile on: rows, elements of a row
+
+    __device__ __forceinline__ static int place(int row) {
+        if constexpr (TR) return swizzle<16>(row);
+        else return ((row & 2) << 1) | (((row >> 2) & 3) ^ ((row >> 3) & 2));
+    }
+    __device__ __forceinline__ void begin(const void *p, int64_t ld_, int64_t first, int64_t extent, int64_t k0, int64_t k1, int tid) {
+        ld = (int)ld_;
+        base = (const char *)p + (TR ? k0 * ld_ + first : first * ld_ + k0) * 2;
+        step_bytes = TR ? BK * ld_ * 2 : BK * 2;
+        rows_in = TR ? k1 - k0 : extent - first;
+        inner_in = TR ? extent - first : k1 - k0;
+        row = tid / C;
+        c = (tid % C) ^ place(row);
+    }
+    __device__ __forceinline__ void next() {
+        base += step_bytes;
+        if constexpr (TR) rows_in -= BK;
+        else inner_in -= BK;
+    }
+    __device__ __forceinline__ bool has(int i) const { return row + i * STEP < rows_in && c * 8 < inner_in; }
+
+    // every chunk is inside or outside as a whole: straight into LDS
+    __device__ __forceinline__ void copy(char *lds, int w) const {
         const __amdgpu_buffer_rsrc_t rs = uniform_rsrc(base, kAnywhere);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = i * NT + tid, row = at / C, c = (at % C) ^ swizzle<C>(row);
-            // (the inner extent is a multiple of 8 here, so a chunk is in or out as a whole)
-            const bool in = row < outers && c * 8 < inners;
-            const uint32_t off = in ? (uint32_t)(row * (int)ld + c * 8) * 2u : kNowhere;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(lds + (i * NT + w * 64) * 16), 16, off, 0, 0, 0);
+        for (int i = 0; i < N; ++i) {
+            const uint32_t off = has(i) ? (uint32_t)((row + i * STEP) * ld + c * 8) * 2u : kNowhere;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(lds + (i * THREADS + w * 64) * 16), 16, off, 0, 0, 0);
         }
-    } else {
-#pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-            const int at = i * NT + tid, row = at / C, c = (at % C) ^ swizzle<C>(row);
-            s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (row < outers) {
+    }
+    // any alignment, any size: through registers
+    __device__ __forceinline__ void load(s16x8 (&v)[N]) const {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (c * 8 + e < inners) v[e] = reinterpret_cast<const short *>(base)[row * ld + c * 8 + e];
+        for (int i = 0; i < N; ++i) {
+            const short *p = (const short *)base + (int64_t)(row + i * STEP) * ld + c * 8;
+            v[i] = (s16x8){0, 0, 0, 0, 0, 0, 0, 0};
+            if (row + i * STEP < rows_in) {
+                if (c * 8 + 8 <= inner_in) __builtin_memcpy(&v[i], p, 16);
+                else
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (c * 8 + e < inner_in) v[i][e] = p[e];
             }
-            *reinterpret_cast<s16x8 *>(lds + at * 16) = v;
         }
     }
-}
-
-// lane's 8 values of row `row` (of 32, + row0) and k = 16 s + 8 (l / 32) .. + 7
-template <bool TR> __device__ __forceinline__ s16x8 fragment(const char *lds, int row0, int s, int l) {
-    const int h = l >> 5;
-    if constexpr (!TR) {
-        const int row = row0 + (l & 31), c = 2 * s + h;
-        return *reinterpret_cast<const s16x8 *>(lds + row * 128 + ((c ^ swizzle<8>(row)) << 4));
-    } else {
-        const int i = l & 15, col = row0 + (l & 16) + 4 * (i & 3);
-        const int k = 16 * s + 8 * h + (i >> 2);
-        const s16x4 lo = lds_read_tr(lds + k * 256 + (((col >> 3) ^ swizzle<16>(k)) << 4) + (col & 4) * 2);
-        const s16x4 hi = lds_read_tr(lds + (k + 4) * 256 + (((col >> 3) ^ swizzle<16>(k + 4)) << 4) + (col & 4) * 2);
-        return join(lo, hi);
+    __device__ __forceinline__ static void put(char *lds, const s16x8 (&v)[N], int tid) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) *reinterpret_cast<s16x8 *>(lds + (i * THREADS + tid) * 16) = v[i];
     }
-}
+};
 
-template <typename T, bool TA, bool TB, bool WIDE>
-__global__ __launch_bounds__(NT) void gemm_kernel(const T *a, int64_t lda, const T *b, int64_t ldb, T *c, int64_t ldc, int64_t M, int64_t N,
-                                                  int64_t K, Epilogue ep, int wide_out) {
-    __shared__ __attribute__((aligned(16))) char smem[2][2 * BM * BK * 2];
+// A lane's 8 values for rows first .. + 32 BLOCKS and k = 16 s + 8 (l / 32) .. + 7.  `order`: lane i of a block's 32 has row i, or, for
+// the operand that runs down the registers, the row that makes registers 0 .. 15 of lane half h rows 16 h + 0 .. 15.
+template <typename T, bool TR, int ROWS, int BLOCKS, bool DOWN> struct Reader {
+    static constexpr int BASES = TR ? 2 * (BLOCKS < 4 ? BLOCKS : 4) : 4;
+    int at[BASES];
+
+    __device__ __forceinline__ void begin(int first, int l) {
+        const int h = l >> 5, i = l & 31;
+        if constexpr (!TR) {
+            const int row = DOWN ? 16 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3) : i;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) at[s] = (first + row) * 128 + (((2 * s + h) ^ Operand<T, false, 64, 256>::place(row)) << 4);
+        } else {
+            const int q = l & 3, g = (l >> 4) & 1, col = DOWN ? 16 * (q & 1) + 4 * (2 * g + (q >> 1)) : 16 * g + 4 * q;
+            const int k = 8 * h + ((l & 15) >> 2);
+#pragma unroll
+            for (int b = 0; b < BASES / 2; ++b)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    at[2 * b + u] = (k + 4 * u) * (ROWS * 2) + ((((first + 32 * b + col) >> 3) ^ swizzle<16>(k + 4 * u)) << 4) + (col & 4) * 2;
+        }
+    }
+    __device__ __forceinline__ s16x8 read(const char *lds, int block, int s) const {
+        if constexpr (!TR) return *reinterpret_cast<const s16x8 *>(lds + at[s] + block * 4096);
+        else {
+            static_assert(BLOCKS <= 4, "");
+            const s16x4 lo = lds_read_tr(lds + at[2 * block] + s * 16 * ROWS * 2), hi = lds_read_tr(lds + at[2 * block + 1] + s * 16 * ROWS * 2);
+            return join(lo, hi);
+        }
+    }
+};
+
+template <typename T, bool TA, bool TB, bool WIDE, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void gemm_kernel(Product p, Epilogue ep) {
+    constexpr int THREADS = 64 * (BM / WM) * (BN / WN), FM = WM / 32, FN = WN / 32;
+    constexpr int A_BYTES = BM * BK * 2, STAGE = (BM + BN) * BK * 2;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, l = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const unsigned tiles_n = (unsigned)((N + BN - 1) / BN);
-    const int64_t m0 = (int64_t)(blockIdx.x / tiles_n) * BM, n0 = (int64_t)(blockIdx.x % tiles_n) * BN;
-    const int wm = (w >> 1) * 64, wn = (w & 1) * 64;
 
-    f32x16 acc[2][2];
+    // Workgroups go to the 8 XCDs in turn: each gets a run of tiles, in groups of 8 tiles of rows, so that what runs at one time
+    // behind one L2 shares its operands.
+    const int per = (p.tiles + 7) / 8;
+    const int split = blockIdx.x / (per * 8), id = blockIdx.x - split * per * 8;
+    const int tile = (id & 7) * per + (id >> 3);
+    if (tile >= p.tiles) return;
+    const int group = tile / (8 * p.tiles_n), in_group = tile - group * 8 * p.tiles_n;
+    const int high = min(8, p.tiles_m - group * 8);
+    const int64_t m0 = (int64_t)(group * 8 + in_group % high) * BM, n0 = (int64_t)(in_group / high) * BN;
+    const int wm = (w / (BN / WN)) * WM, wn = (w % (BN / WN)) * WN;
+
+    f32x16 acc[FM][FN];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < FN; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-    const int steps = (int)((K + BK - 1) / BK);
+    const int64_t k0 = split * p.split_k, k1 = min(p.K, k0 + p.split_k);
+    const int steps = (int)((k1 - k0 + BK - 1) / BK);
+    typedef Operand<T, TA, BM, THREADS> OA;
+    typedef Operand<T, TB, BN, THREADS> OB;
+    OA oa;
+    OB ob;
+    oa.begin(p.a, p.lda, m0, p.M, k0, k1, tid);
+    ob.begin(p.b, p.ldb, n0, p.N, k0, k1, tid);
+    Reader<T, TA, BM, FM, false> ra;
+    Reader<T, TB, BN, FN, true> rb;
+    ra.begin(wm, l);
+    rb.begin(wn, l);
+    s16x8 va[WIDE ? 1 : OA::N], vb[WIDE ? 1 : OB::N];
     if (steps) {
-        stage<T, TA, WIDE>(smem[0], a, lda, m0, M, 0, K, tid);
-        stage<T, TB, WIDE>(smem[0] + BM * BK * 2, b, ldb, n0, N, 0, K, tid);
+        if constexpr (WIDE) {
+            oa.copy(smem, w);
+            ob.copy(smem + A_BYTES, w);
+        } else {
+            oa.load(va);
+            ob.load(vb);
+            OA::put(smem, va, tid);
+            OB::put(smem + A_BYTES, vb, tid);
+        }
     }
     for (int s = 0; s < steps; ++s) {
         wait_lds_dma();
         __syncthreads();                                   // tile s is there, and tile s - 1 has been read by every wave
-        if (s + 1 < steps) {
-            stage<T, TA, WIDE>(smem[(s + 1) & 1], a, lda, m0, M, (int64_t)(s + 1) * BK, K, tid);
-            stage<T, TB, WIDE>(smem[(s + 1) & 1] + BM * BK * 2, b, ldb, n0, N, (int64_t)(s + 1) * BK, K, tid);
+        char *other = smem + ((s + 1) & 1) * STAGE;
+        const bool more = s + 1 < steps;
+        if (more) {
+            oa.next();
+            ob.next();
+            if constexpr (WIDE) {
+                oa.copy(other, w);
+                ob.copy(other + A_BYTES, w);
+            } else {
+                oa.load(va);
+                ob.load(vb);
+            }
         }
-        const char *ta = smem[s & 1], *tb = ta + BM * BK * 2;
+        const char *ta = smem + (s & 1) * STAGE, *tb = ta + A_BYTES;
 #pragma unroll
         for (int kk = 0; kk < BK / 16; ++kk) {
-            s16x8 fa[2], fb[2];
+            s16x8 fa[FM], fb[FN];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                fa[i] = fragment<TA>(ta, wm + 32 * i, kk, l);
-                fb[i] = fragment<TB>(tb, wn + 32 * i, kk, l);
-            }
+            for (int i = 0; i < FM; ++i) fa[i] = ra.read(ta, i, kk);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int j = 0; j < FN; ++j) fb[j] = rb.read(tb, j, kk);
 #pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = mfma32<T>(fb[j], fa[i], acc[i][j]);
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = mfma32<T>(fb[j], fa[i], acc[i][j]);
         }
+        if constexpr (!WIDE)
+            if (more) {
+                OA::put(other, va, tid);
+                OB::put(other + A_BYTES, vb, tid);
+            }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < FN; ++j) {
+            const int64_t m = m0 + wm + 32 * i + (l & 31), n = n0 + wn + 32 * j + 16 * (l >> 5);
+            if (m >= p.M) continue;
+            if (p.part) {
+                float *to = p.part + ((int64_t)split * p.M + m) * p.N + n;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const f32x4 v = {acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]};
-                store_row4<T>(ep, c, ldc, m0 + wm + 32 * i + (l & 31), n0 + wn + 32 * j + 8 * r + 4 * (l >> 5), M, N, v, wide_out);
+                for (int r = 0; r < 16; ++r)
+                    if (n + r < p.N) to[r] = acc[i][j][r];
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; r += 8) {
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = acc[i][j][r + e];
+                    if (n + r < p.N) finish8<T>(ep, (T *)p.c, m, n + r, p.N, v, p.wide_out);
+                }
             }
+        }
 }
 
+// adds up the parts of K, in order
+template <typename T> __global__ __launch_bounds__(256) void join_kernel(Product p, Epilogue ep) {
+    const int64_t chunks = (p.N + 7) / 8;
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= p.M * chunks) return;
+    const int64_t m = id / chunks, n = (id - m * chunks) * 8;
+    float v[8] = {};
+    for (int s = 0; s < p.splits; ++s) {
+        const float *from = p.part + ((int64_t)s * p.M + m) * p.N + n;
+        if (p.wide_out) {
+            const f32x4 a = *reinterpret_cast<const f32x4 *>(from), b = *reinterpret_cast<const f32x4 *>(from + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += a[e], v[4 + e] += b[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (n + e < p.N) v[e] += from[e];
+        }
+    }
+    finish8<T>(ep, (T *)p.c, m, n, p.N, v, p.wide_out);
+}
+
+// ---------------------------------------------------------------------------------------------- few rows
+// A workgroup takes 16 columns and 16 MT rows; its 4 waves split the summed index, read both operands straight into registers
+// (16 bytes of a row each, whatever its alignment) and join their sums in LDS.  What bounds it is the weights' way from memory.
+template <typename T, int MT> __global__ __launch_bounds__(256) void rows_kernel(Product p, Epilogue ep) {
+    __shared__ float sums[4][16][16 * MT + 1];
+    const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
+    const int64_t n0 = (int64_t)(blockIdx.x / p.tiles_m) * 16, m0 = (int64_t)(blockIdx.x % p.tiles_m) * 16 * MT;
+    const short *wp = (const short *)p.b + min(n0 + (l & 15), p.N - 1) * p.ldb;
+    const short *xp[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) xp[t] = (const short *)p.a + min(m0 + 16 * t + (l & 15), p.M - 1) * p.lda;
+    f32x4 acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    auto load = [&](const short *row, int64_t k) {
+        s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (k + 8 <= p.K) __builtin_memcpy(&v, row + k, 16);
+        else if (k < p.K)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (k + e < p.K) v[e] = row[k + e];
+        return v;
+    };
+    // 128 of the summed index a turn, 4 steps for each wave at once
+    for (int64_t k = (int64_t)w * 128; k < p.K; k += 512) {
+        s16x8 wf[4], xf[4][MT];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int64_t at = k + 32 * s + 8 * (l >> 4);
+            wf[s] = load(wp, at);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) xf[s][t] = load(xp[t], at);
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[t] = mfma16<T>(wf[s], xf[s][t], acc[t]);
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sums[w][4 * (l >> 4) + r][16 * t + (l & 15)] = acc[t][r];
+    __syncthreads();
+    for (int i = tid; i < 16 * MT * 2; i += 256) {
+        const int64_t m = m0 + i / 2, n = n0 + (i & 1) * 8;
+        if (m >= p.M || n >= p.N) continue;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int col = (i & 1) * 8 + e;
+            v[e] = (sums[0][col][i / 2] + sums[1][col][i / 2]) + (sums[2][col][i / 2] + sums[3][col][i / 2]);
+        }
+        finish8<T>(ep, (T *)p.c, m, n, p.N, v, p.wide_out);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- which kernel
+struct Choice {
+    int kind;                      // 0: few rows, 1: tiles of 128 x 128, 2: tiles of 256 x 256
+    int splits, mt;
+    int64_t split_k;
+};
+
+// What a step of 64 along the summed index takes a workgroup, and how many run on the 256 CUs at once; splitting it costs the parts' way
+// to memory and back and a launch.
+Choice choose(int64_t M, int64_t N, int64_t K, bool rows_ok, bool wide) {
+    Choice best = {1, 1, 1, K};
+    if (rows_ok && M <= 64) {
+        best.kind = 0;
+        best.mt = ceil_div64(N, 16) * ceil_div64(M, 16) <= 1024 ? 1 : M <= 16 ? 1 : M <= 32 ? 2 : 4;
+        return best;
+    }
+    double least = 1e300;
+    for (int kind = 1; kind <= (wide ? 2 : 1); ++kind) {
+        const int64_t t = kind == 2 ? 256 : 128;
+        const int64_t tiles = ceil_div64(M, t) * ceil_div64(N, t), steps = ceil_div64(K, BK);
+        const int at_once = kind == 2 ? 256 : 512;
+        const double step_us = kind == 2 ? 1.2 : 0.9;
+        for (int s = 1; s <= 16; s *= 2) {
+            if (s > 1 && (steps / s < 8 || tiles * s > 2 * at_once)) break;
+            double us = (double)ceil_div64(tiles * s, at_once) * ((double)ceil_div64(steps, s) * step_us + 3.0);
+            if (s > 1) us += 4.0 + (double)M * N * 8.0 * s / 4.0e6;
+            if (us < least) least = us, best = {kind, s, 1, ceil_div64(steps, s) * BK};
+        }
+    }
+    best.splits = (int)ceil_div64(K > 0 ? K : 1, best.split_k > 0 ? best.split_k : 1);
+    if (best.splits < 1) best.splits = 1;
+    return best;
+}
+size_t parts_bytes(const Choice &c, int64_t M, int64_t N) { return c.splits > 1 ? (size_t)c.splits * M * N * 4 : 0; }
+
+template <typename T, bool TA, bool TB, bool WIDE, int BM, int BN, int WM, int WN>
+int launch_tiles(Product &p, const Epilogue &ep, hipStream_t stream) {
+    constexpr int LDS = 2 * (BM + BN) * BK * 2;
+    const int64_t tiles = ceil_div64(p.M, BM) * ceil_div64(p.N, BN);
+    TOKENS_REQUIRE(tiles * p.splits < (1 << 22), "linear: more tiles than a launch takes");
+    p.tiles_m = (int)ceil_div64(p.M, BM), p.tiles_n = (int)ceil_div64(p.N, BN), p.tiles = (int)tiles;
+    if constexpr (LDS > 65536) {
+        const hipError_t e = hipFuncSetAttribute((const void *)gemm_kernel<T, TA, TB, WIDE, BM, BN, WM, WN>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        if (e != hipSuccess) {
+            (void)hipGetLastError();
+            tokens_error("linear: %d bytes of LDS: %s", LDS, hipGetErrorString(e));
+            return (int)e;
+        }
+    }
+    hipLaunchKernelGGL((gemm_kernel<T, TA, TB, WIDE, BM, BN, WM, WN>), dim3((unsigned)((tiles + 7) / 8 * 8 * p.splits)),
+                       dim3(64 * (BM / WM) * (BN / WN)), LDS, stream, p, ep);
+    return tokens_launch_status("linear");
+}
+
+// `parts`: room for the parts of K (workspace), 16-byte aligned
 template <typename T, bool TA, bool TB>
-int gemm(const void *a, int64_t lda, const void *b, int64_t ldb, void *c, int64_t ldc, int64_t M, int64_t N, int64_t K, const Epilogue &ep,
+int gemm(const void *a, int64_t lda, const void *b, int64_t ldb, void *c, int64_t M, int64_t N, int64_t K, const Epilogue &ep, void *parts,
          hipStream_t stream) {
     // 16-byte loads: rows and the index along them in pieces of 8 elements (a piece is inside or outside as a whole)
     const bool wide_in = lda % 8 == 0 && ldb % 8 == 0 && (uint64_t)a % 16 == 0 && (uint64_t)b % 16 == 0 && (TA ? M : K) % 8 == 0 &&
                          (TB ? N : K) % 8 == 0;
-    const bool wide_out = N % 4 == 0 && ldc % 4 == 0 && (uint64_t)c % 8 == 0 && (!ep.bias || (uint64_t)ep.bias % 8 == 0) &&
-                          (!ep.residual || ((uint64_t)ep.residual % 8 == 0 && ep.ldr % 4 == 0)) && (!ep.z || (uint64_t)ep.z % 8 == 0);
-    const int64_t tiles = ceil_div64(N, BN) * ceil_div64(M, BM);
-    TOKENS_REQUIRE(tiles < (1 << 24), "linear: more tiles than a launch takes");
-    const dim3 grid((unsigned)tiles);
-    if (wide_in) hipLaunchKernelGGL((gemm_kernel<T, TA, TB, true>), grid, dim3(NT), 0, stream, (const T *)a, lda, (const T *)b, ldb, (T *)c, ldc, M, N, K, ep, (int)wide_out);
-    else hipLaunchKernelGGL((gemm_kernel<T, TA, TB, false>), grid, dim3(NT), 0, stream, (const T *)a, lda, (const T *)b, ldb, (T *)c, ldc, M, N, K, ep, (int)wide_out);
-    return tokens_launch_status("linear");
+    const bool wide_out = N % 8 == 0 && (uint64_t)c % 16 == 0 && (!ep.bias || (uint64_t)ep.bias % 16 == 0) &&
+                          (!ep.residual || ((uint64_t)ep.residual % 16 == 0 && ep.ldr % 8 == 0)) && (!ep.z || (uint64_t)ep.z % 16 == 0);
+    const Choice ch = choose(M, N, K, !TA && !TB, wide_in);
+    Product p = {a, b, c, ch.splits > 1 ? (float *)parts : nullptr, lda, ldb, M, N, K, ch.split_k, 0, 0, 0, ch.splits, (int)wide_out};
+    if constexpr (!TA && !TB)
+        if (ch.kind == 0) {
+            p.tiles_m = (int)ceil_div64(M, 16 * ch.mt);
+            const int64_t blocks = ceil_div64(N, 16) * p.tiles_m;
+            TOKENS_REQUIRE(blocks < (1 << 24), "linear: more tiles than a launch takes");
+            if (ch.mt == 1) hipLaunchKernelGGL((rows_kernel<T, 1>), dim3((unsigned)blocks), dim3(256), 0, stream, p, ep);
+            else if (ch.mt == 2) hipLaunchKernelGGL((rows_kernel<T, 2>), dim3((unsigned)blocks), dim3(256), 0, stream, p, ep);
+            else hipLaunchKernelGGL((rows_kernel<T, 4>), dim3((unsigned)blocks), dim3(256), 0, stream, p, ep);
+            return tokens_launch_status("linear");
+        }
+    int rc;
+    if (!wide_in) rc = launch_tiles<T, TA, TB, false, 128, 128, 64, 64>(p, ep, stream);
+    else if (ch.kind == 2) rc = launch_tiles<T, TA, TB, true, 256, 256, 128, 64>(p, ep, stream);
+    else rc = launch_tiles<T, TA, TB, true, 128, 128, 64, 64>(p, ep, stream);
+    if (rc || ch.splits == 1) return rc;
+    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)ceil_div64(M * ceil_div64(N, 8), 256)), dim3(256), 0, stream, p, ep);
+    return tokens_launch_status("linear join");
+}
+// the largest that gemm() may take for either way of loading, which depends on addresses
+size_t gemm_bytes(int64_t M, int64_t N, int64_t K, bool rows_ok) {
+    const size_t a = parts_bytes(choose(M, N, K, rows_ok, true), M, N), b = parts_bytes(choose(M, N, K, rows_ok, false), M, N);
+    return ((a > b ? a : b) + 255) / 256 * 256;
 }
 
 // ---------------------------------------------------------------------------------------------- dz = dy act'(z), column sums
-// A workgroup takes 64 columns x a run of rows: 16 column groups of 4 x 16 rows at a time.  Column sums are of the unrounded dz, one
-// row of partial sums for each run, added up in a fixed order by the second kernel.
-constexpr int DZ_COLS = 64;
+// A workgroup takes 256 columns x a run of rows, 8 columns a thread and 8 rows at a time.  Column sums are of the unrounded dz, one row
+// of partial sums for each run, added up in a fixed order by the second kernel.
+constexpr int DZ_COLS = 256;
 
 template <typename T>
 __global__ __launch_bounds__(256) void dz_kernel(const T *dy, int64_t lddy, const T *z, T *dz, float *part, int64_t M, int64_t N, int64_t run,
-                                                 int act) {
-    const int64_t n = (int64_t)blockIdx.x * DZ_COLS + (threadIdx.x & 15) * 4;
+                                                 int act, int wide) {
+    const int64_t n = (int64_t)blockIdx.x * DZ_COLS + (threadIdx.x & 31) * 8;
     const int64_t m1 = min(M, (int64_t)(blockIdx.y + 1) * run);
-    const int left = n < N ? (int)min((int64_t)4, N - n) : 0;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int64_t m = (int64_t)blockIdx.y * run + (threadIdx.x >> 4); m < m1; m += 16) {
+    const int left = n < N ? (int)min((int64_t)8, N - n) : 0;
+    float sum[8] = {};
+    if (left) {
+#pragma unroll 2
+        for (int64_t m = (int64_t)blockIdx.y * run + (threadIdx.x >> 5); m < m1; m += 8) {
+            float g[8] = {}, zz[8] = {};
+            if (wide) {
+                load8_of<T>(g, dy + m * lddy + n);
+                if (act != BNDM_ACT_NONE) load8_of<T>(zz, z + m * N + n);
+            } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i < left) {
-                float g = (float)dy[m * lddy + n + i];
-                if (act != BNDM_ACT_NONE) {
-                    g *= act_slope(act, (float)z[m * N + n + i]);
-                    dz[m * N + n + i] = (T)g;
-                }
-                sum[i] += g;
+                for (int i = 0; i < 8; ++i)
+                    if (i < left) {
+                        g[i] = (float)dy[m * lddy + n + i];
+                        if (act != BNDM_ACT_NONE) zz[i] = (float)z[m * N + n + i];
+                    }
             }
+            if (act == BNDM_ACT_SILU) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) g[i] *= act_slope(BNDM_ACT_SILU, zz[i]);
+            } else if (act == BNDM_ACT_GELU) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) g[i] *= act_slope(BNDM_ACT_GELU, zz[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] += g[i];
+            if (act != BNDM_ACT_NONE) {
+                if (wide) *reinterpret_cast<s16x8 *>(dz + m * N + n) = pack8<T>(g[0], g[1], g[2], g[3], g[4], g[5], g[6], g[7]);
+                else
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (i < left) dz[m * N + n + i] = (T)g[i];
+            }
+        }
     }
     if (!part) return;
-    __shared__ float s[16][DZ_COLS];
+    __shared__ float s[8][DZ_COLS];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[threadIdx.x >> 4][(threadIdx.x & 15) * 4 + i] = sum[i];
+    for (int i = 0; i < 8; ++i) s[threadIdx.x >> 5][(threadIdx.x & 31) * 8 + i] = sum[i];
     __syncthreads();
-    if (threadIdx.x < DZ_COLS) {
-        float t = 0.f;
+    float t = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) t += s[i][threadIdx.x];
-        const int64_t col = (int64_t)blockIdx.x * DZ_COLS + threadIdx.x;
-        if (col < N) part[(int64_t)blockIdx.y * N + col] = t;
+    for (int i = 0; i < 8; ++i) t += s[i][threadIdx.x];
+    const int64_t col = (int64_t)blockIdx.x * DZ_COLS + threadIdx.x;
+    if (col < N) part[(int64_t)blockIdx.y * N + col] = t;
+}
+
+// 32 columns a workgroup, 8 runs at a time
+template <typename T> __global__ __launch_bounds__(256) void column_sums_kernel(const float *part, T *out, int64_t N, int runs) {
+    __shared__ float s[8][32];
+    const int64_t n = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+    float t = 0.f;
+    if (n < N)
+#pragma unroll 4
+        for (int r = threadIdx.x >> 5; r < runs; r += 8) t += part[(int64_t)r * N + n];
+    s[threadIdx.x >> 5][threadIdx.x & 31] = t;
+    __syncthreads();
+    if (threadIdx.x < 32 && n < N) {
+        t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t += s[i][threadIdx.x];
+        out[n] = (T)t;
     }
 }
 
-template <typename T> __global__ __launch_bounds__(256) void column_sums_kernel(const float *part, T *out, int64_t N, int runs) {
-    const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (n >= N) return;
-    float t = 0.f;
-    for (int r = 0; r < runs; ++r) t += part[(int64_t)r * N + n];
-    out[n] = (T)t;
+// rows of a run: 8 at least (a workgroup's rows at a time), about 2048 workgroups in all
+int64_t rows_of_run(int64_t M, int64_t N) {
+    const int64_t runs = ceil_div64(2048, ceil_div64(N, DZ_COLS));
+    return ceil_div64(ceil_div64(M, runs), 8) * 8;
 }
-
-// rows of a run: a workgroup's 256 threads take 16 rows at a time; at most 64 runs
-int64_t rows_of_run(int64_t M) { return ceil_div64(ceil_div64(M, 64), 16) * 16; }
 size_t dz_bytes(int64_t M, int64_t N, int act) { return act == BNDM_ACT_NONE ? 0 : (size_t)(((M * N * 2) + 255) / 256 * 256); }
+size_t sums_bytes(int64_t M, int64_t N, bool want) { return want ? (size_t)((ceil_div64(M, rows_of_run(M, N)) * N * 4 + 255) / 256 * 256) : 0; }
 
 template <typename T>
 int backward(const void *dy, int64_t lddy, const void *z, const void *x, int64_t ldx, const void *w, void *dx, void *dw, void *dbias, int64_t M,
              int64_t N, int64_t K, int act, void *workspace, hipStream_t stream) {
     const void *dz = dy;
     int64_t lddz = lddy;
+    char *parts = (char *)workspace + dz_bytes(M, N, act) + sums_bytes(M, N, dbias != nullptr);
     if (act != BNDM_ACT_NONE || dbias) {
         float *part = dbias ? (float *)((char *)workspace + dz_bytes(M, N, act)) : nullptr;
-        const int64_t run = rows_of_run(M);
+        const int64_t run = rows_of_run(M, N);
         const int runs = (int)ceil_div64(M, run);
+        const int wide = N % 8 == 0 && lddy % 8 == 0 && (uint64_t)dy % 16 == 0 && (uint64_t)z % 16 == 0;
         hipLaunchKernelGGL((dz_kernel<T>), dim3((unsigned)ceil_div64(N, DZ_COLS), (unsigned)runs), dim3(256), 0, stream, (const T *)dy, lddy,
-                           (const T *)z, (T *)workspace, part, M, N, run, act);
+                           (const T *)z, (T *)workspace, part, M, N, run, act, wide);
         if (int rc = tokens_launch_status("linear dz")) return rc;
         if (act != BNDM_ACT_NONE) dz = workspace, lddz = N;
         if (dbias) {
-            hipLaunchKernelGGL((column_sums_kernel<T>), dim3((unsigned)ceil_div64(N, 256)), dim3(256), 0, stream, part, (T *)dbias, N, runs);
+            hipLaunchKernelGGL((column_sums_kernel<T>), dim3((unsigned)ceil_div64(N, 32)), dim3(256), 0, stream, part, (T *)dbias, N, runs);
             if (int rc = tokens_launch_status("linear column sums")) return rc;
         }
     }
     const Epilogue none = {nullptr, nullptr, 0, nullptr, BNDM_ACT_NONE};
     if (dx)
-        if (int rc = gemm<T, false, true>(dz, lddz, w, K, dx, K, M, K, N, none, stream)) return rc;
+        if (int rc = gemm<T, false, true>(dz, lddz, w, K, dx, M, K, N, none, parts, stream)) return rc;
     if (dw)
-        if (int rc = gemm<T, true, true>(dz, lddz, x, ldx, dw, K, N, K, M, none, stream)) return rc;
+        if (int rc = gemm<T, true, true>(dz, lddz, x, ldx, dw, N, K, M, none, parts, stream)) return rc;
     return 0;
 }
 
@@ -284,7 +603,7 @@ int check(const char *what, int64_t M, int64_t N, int64_t K, int act, int dtype)
     TOKENS_REQUIRE(M >= 0 && N >= 0 && K >= 0, "%s: negative size", what);
     TOKENS_REQUIRE(act == BNDM_ACT_NONE || act == BNDM_ACT_SILU || act == BNDM_ACT_GELU, "%s: activation %d", what, act);
     TOKENS_REQUIRE(dtype == BNDM_DTYPE_F16 || dtype == BNDM_DTYPE_BF16, "%s: dtype %d (f16 and bf16 only)", what, dtype);
-    TOKENS_REQUIRE(M <= (1 << 23) && N <= (1 << 23) && K <= (1 << 23), "%s: sizes up to 2^23", what);
+    TOKENS_REQUIRE(M <= (1 << 30) && N <= (1 << 22) && K <= (1 << 22), "%s: up to 2^30 rows, sizes up to 2^22", what);
     return 0;
 }
 
@@ -293,20 +612,30 @@ int check(const char *what, int64_t M, int64_t N, int64_t K, int act, int dtype)
 
 using namespace bndm;
 
+extern "C" size_t bndm_tokens_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    if (M <= 0 || N <= 0 || K < 0) return 0;
+    return gemm_bytes(M, N, K, true);
+}
+
 extern "C" int bndm_tokens_linear(const void *x, int64_t ldx, const void *w, const void *bias, const void *residual, int64_t ldr, void *y,
-                                  void *z, int64_t M, int64_t N, int64_t K, int act, int dtype, void *stream) {
+                                  void *z, int64_t M, int64_t N, int64_t K, int act, int dtype, void *workspace, size_t workspace_bytes,
+                                  void *stream) {
     if (int rc = check("bndm_tokens_linear", M, N, K, act, dtype)) return rc;
     if (M == 0 || N == 0) return 0;
     TOKENS_REQUIRE((x || K == 0) && (w || K == 0) && y, "bndm_tokens_linear: NULL tensor");
-    TOKENS_REQUIRE(ldx >= 0 && ldx <= (1 << 23) && (!residual || ldr >= 0), "bndm_tokens_linear: row stride");
+    TOKENS_REQUIRE(ldx >= 0 && ldx <= (1 << 22) && (!residual || ldr >= 0), "bndm_tokens_linear: row stride");
+    const size_t need = bndm_tokens_linear_workspace_bytes(M, N, K);
+    TOKENS_REQUIRE(need == 0 || (workspace && (uint64_t)workspace % 16 == 0 && workspace_bytes >= need),
+                   "bndm_tokens_linear: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     const Epilogue ep = {bias, residual, ldr, z, act};
-    if (dtype == BNDM_DTYPE_F16) return gemm<f16, false, false>(x, ldx, w, K, y, N, M, N, K, ep, (hipStream_t)stream);
-    return gemm<bf16, false, false>(x, ldx, w, K, y, N, M, N, K, ep, (hipStream_t)stream);
+    if (dtype == BNDM_DTYPE_F16) return gemm<f16, false, false>(x, ldx, w, K, y, M, N, K, ep, workspace, (hipStream_t)stream);
+    return gemm<bf16, false, false>(x, ldx, w, K, y, M, N, K, ep, workspace, (hipStream_t)stream);
 }
 
 extern "C" size_t bndm_tokens_linear_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int act, int want_dbias) {
-    if (M <= 0 || N <= 0 || K < 0) return 0;
-    return dz_bytes(M, N, act) + (want_dbias ? (size_t)ceil_div64(M, rows_of_run(M)) * N * 4 : 0);
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    const size_t a = gemm_bytes(M, K, N, false), b = gemm_bytes(N, K, M, false);
+    return dz_bytes(M, N, act) + sums_bytes(M, N, want_dbias) + (a > b ? a : b);
 }
 
 extern "C" int bndm_tokens_linear_backward(const void *dy, int64_t lddy, const void *z, const void *x, int64_t ldx, const void *w, void *dx,
@@ -315,9 +644,9 @@ extern "C" int bndm_tokens_linear_backward(const void *dy, int64_t lddy, const v
     if (int rc = check("bndm_tokens_linear_backward", M, N, K, act, dtype)) return rc;
     TOKENS_REQUIRE(M > 0 && N > 0 && K > 0, "bndm_tokens_linear_backward: empty layer");
     TOKENS_REQUIRE(dy && (act == BNDM_ACT_NONE || z) && (!dw || x) && (!dx || w), "bndm_tokens_linear_backward: NULL tensor");
-    TOKENS_REQUIRE(ldx >= 0 && ldx <= (1 << 23) && lddy >= 0 && lddy <= (1 << 23), "bndm_tokens_linear_backward: row stride");
+    TOKENS_REQUIRE(ldx >= 0 && ldx <= (1 << 22) && lddy >= 0 && lddy <= (1 << 22), "bndm_tokens_linear_backward: row stride");
     const size_t need = bndm_tokens_linear_backward_workspace_bytes(M, N, K, act, dbias != nullptr);
-    TOKENS_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "bndm_tokens_linear_backward: workspace of %zu bytes, %zu needed",
+    TOKENS_REQUIRE(need == 0 || (workspace && (uint64_t)workspace % 16 == 0 && workspace_bytes >= need), "bndm_tokens_linear_backward: workspace of %zu bytes, %zu needed",
                    workspace_bytes, need);
     if (dtype == BNDM_DTYPE_F16) return backward<f16>(dy, lddy, z, x, ldx, w, dx, dw, dbias, M, N, K, act, workspace, (hipStream_t)stream);
     return backward<bf16>(dy, lddy, z, x, ldx, w, dx, dw, dbias, M, N, K, act, workspace, (hipStream_t)stream);

@@ -74,8 +74,11 @@ def _linear_forward(x, weight, bias, residual, act, dtype, keep):
     z = x.new_empty((m, n)) if keep and act else None
     res, ldr = _rows(residual, n) if residual is not None else (None, 0)
     if m:
-        _launch(_lib.load_tokens().bndm_tokens_linear, "linear", x.device, rows.data_ptr(), ldx, weight.data_ptr(), _ptr(bias), _ptr(res), ldr,
-                y.data_ptr(), _ptr(z), m, n, k, act, dtype)
+        lib = _lib.load_tokens()
+        need = lib.bndm_tokens_linear_workspace_bytes(m, n, k)
+        work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+        _launch(lib.bndm_tokens_linear, "linear", x.device, rows.data_ptr(), ldx, weight.data_ptr(), _ptr(bias), _ptr(res), ldr, y.data_ptr(),
+                _ptr(z), m, n, k, act, dtype, _ptr(work), need)
     return y, z
 
 

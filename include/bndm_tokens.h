@@ -35,10 +35,13 @@ const char *bndm_tokens_last_error(void);
 #define BNDM_ACT_SILU 1
 #define BNDM_ACT_GELU 2  /* z Phi(z) */
 
-int bndm_tokens_linear(const void *x, int64_t ldx, const void *w, const void *bias, const void *residual, int64_t ldr,
-                       void *y, void *z, int64_t M, int64_t N, int64_t K, int act, int dtype, void *stream);
+/* bytes of scratch of the call below (0 where it needs none); scratch starts at 16 bytes */
+size_t bndm_tokens_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
 
-/* bytes of scratch of the call below (0 where it needs none) */
+int bndm_tokens_linear(const void *x, int64_t ldx, const void *w, const void *bias, const void *residual, int64_t ldr,
+                       void *y, void *z, int64_t M, int64_t N, int64_t K, int act, int dtype, void *workspace,
+                       size_t workspace_bytes, void *stream);
+
 size_t bndm_tokens_linear_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int act, int want_dbias);
 
 /* Gradients of the layer from dy [M, N] (rows lddy apart): dz = dy act'(z), dx = dz W, dw = dz^T x, dbias = column sums of dz.

@@ -46,13 +46,18 @@ def refused(lib, rc, word):
 
 
 def test_linear_refusals(lib):
-    good = dict(x=P, ldx=16, w=P, b=0, r=0, ldr=0, y=P, z=0, M=4, N=8, K=16, act=0, dtype=0)
-    for change, word in [(dict(M=-1), "negative"), (dict(act=3), "activation"), (dict(dtype=2), "dtype"), (dict(N=1 << 24), "2^23"),
+    need = lib.bndm_tokens_linear_workspace_bytes(128, 128, 65536)
+    assert need > 0 and lib.bndm_tokens_linear_workspace_bytes(4, 8, 16) == 0          # one tile, a long sum: split
+    big = dict(x=P, ldx=65536, w=P, b=0, r=0, ldr=0, y=P, z=0, M=128, N=128, K=65536, act=0, dtype=0)
+    for work, size in ((P, need - 1), (0, need), (P + 8, need)):
+        refused(lib, lib.bndm_tokens_linear(*big.values(), work, size, None), "workspace")
+    good = dict(x=P, ldx=16, w=P, b=0, r=0, ldr=0, y=P, z=0, M=4, N=8, K=16, act=0, dtype=0, work=0, size=0)
+    for change, word in [(dict(M=-1), "negative"), (dict(act=3), "activation"), (dict(dtype=2), "dtype"), (dict(N=1 << 24), "2^22"),
                          (dict(x=0), "NULL"), (dict(w=0), "NULL"), (dict(y=0), "NULL"), (dict(ldx=-1), "stride"), (dict(r=P, ldr=-1), "stride")]:
         refused(lib, lib.bndm_tokens_linear(*{**good, **change}.values(), None), word)
     assert lib.bndm_tokens_linear(*{**good, "M": 0}.values(), None) == 0
     need = lib.bndm_tokens_linear_backward_workspace_bytes(100, 8, 16, 1, 1)
-    assert need >= 100 * 8 * 2 + 8 * 4 and lib.bndm_tokens_linear_backward_workspace_bytes(100, 8, 16, 0, 0) == 0
+    assert need >= 100 * 8 * 2 + 8 * 4
     good = dict(dy=P, lddy=8, z=P, x=P, ldx=16, w=P, dx=P, dw=P, db=P, M=100, N=8, K=16, act=1, dtype=1, work=P, size=need)
     for change, word in [(dict(M=0), "empty"), (dict(z=0), "NULL"), (dict(dy=0), "NULL"), (dict(x=0), "NULL"), (dict(w=0), "NULL"),
                          (dict(size=need - 1), "workspace"), (dict(work=0), "workspace"), (dict(lddy=-8), "stride"), (dict(act=9), "activation")]:
