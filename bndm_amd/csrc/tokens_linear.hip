@@ -105,7 +105,9 @@ template <typename T> __device__ __forceinline__ void finish8(const Epilogue &e,
 // ---------------------------------------------------------------------------------------------- the product
 // C[m][n] = sum_k A(m, k) B(n, k).  TA false: A(m, k) = a[m * lda + k]; true: a[k * lda + m]; TB likewise.
 // B's index runs down the registers of a result tile, in an order that gives a lane 16 consecutive n of one row m.
-constexpr int BK = 64;
+// The tiles of a step of 32 of the summed index wait in LDS, three steps ahead of the products: one step ahead (64 at a time, 128 KB as
+// well) the products wait for memory instead, 165 us for 137 Gflop where this takes TODO.
+constexpr int BK = 32, STAGES = 4;
 
 struct Product {
     const void *a, *b;
@@ -116,13 +118,13 @@ struct Product {
     int tiles_m, tiles_n, tiles, splits, wide_out;
 };
 
-// ROWS of one operand x 64 of the summed index in LDS, 16-byte chunks in swizzled places: rows along the summed index: [ROWS][8 chunks];
-// across it: [64][ROWS / 8 chunks].  Copied by THREADS threads.
+// ROWS of one operand x 32 of the summed index in LDS, 16-byte chunks in swizzled places: rows along the summed index: [ROWS][4 chunks];
+// across it: [32][ROWS / 8 chunks].  Copied by THREADS threads.
 template <typename T, bool TR, int ROWS, int THREADS> struct Operand {
-    static constexpr int C = TR ? ROWS / 8 : 8;
-    static constexpr int N = ROWS * 8 / THREADS;              // chunks of a thread
+    static constexpr int C = TR ? ROWS / 8 : BK / 8;
+    static constexpr int N = ROWS * (BK / 8) / THREADS;       // chunks of a thread
     static constexpr int STEP = THREADS / C;                  // rows between them; a multiple of the swizzle's period
-    static_assert(STEP % (TR ? 16 : 32) == 0, "one swizzle for all chunks of a thread");
+    static_assert(STEP % 16 == 0, "one swizzle for all chunks of a thread");
 
     const char *base;              // where the tile of this step begins
     int64_t step_bytes;
@@ -130,10 +132,7 @@ template <typename T, bool TR, int ROWS, int THREADS> struct Operand {
     int ld;
     int64_t rows_in, inner_in;     // what is there from the first tile on: rows, elements of a row
 
-    __device__ __forceinline__ static int place(int row) {
-        if constexpr (TR) return swizzle<16>(row);
-        else return ((row & 2) << 1) | (((row >> 2) & 3) ^ ((row >> 3) & 2));
-    }
+    __device__ __forceinline__ static int place(int row) { return TR ? swizzle<16>(row) : swizzle<4>(row); }
     __device__ __forceinline__ void begin(const void *p, int64_t ld_, int64_t first, int64_t extent, int64_t k0, int64_t k1, int tid) {
         ld = (int)ld_;
         base = (const char *)p + (TR ? k0 * ld_ + first : first * ld_ + k0) * 2;
@@ -183,7 +182,7 @@ template <typename T, bool TR, int ROWS, int THREADS> struct Operand {
 // A lane's 8 values for rows first .. + 32 BLOCKS and k = 16 s + 8 (l / 32) .. + 7.  `order`: lane i of a block's 32 has row i, or, for
 // the operand that runs down the registers, the row that makes registers 0 .. 15 of lane half h rows 16 h + 0 .. 15.
 template <typename T, bool TR, int ROWS, int BLOCKS, bool DOWN> struct Reader {
-    static constexpr int BASES = TR ? 2 * (BLOCKS < 4 ? BLOCKS : 4) : 4;
+    static constexpr int BASES = TR ? 2 * BLOCKS : BK / 16;
     int at[BASES];
 
     __device__ __forceinline__ void begin(int first, int l) {
@@ -191,26 +190,56 @@ template <typename T, bool TR, int ROWS, int BLOCKS, bool DOWN> struct Reader {
         if constexpr (!TR) {
             const int row = DOWN ? 16 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3) : i;
 #pragma unroll
-            for (int s = 0; s < 4; ++s) at[s] = (first + row) * 128 + (((2 * s + h) ^ Operand<T, false, 64, 256>::place(row)) << 4);
+            for (int s = 0; s < BASES; ++s) at[s] = (first + row) * (BK * 2) + (((2 * s + h) ^ swizzle<4>(row)) << 4);
         } else {
             const int q = l & 3, g = (l >> 4) & 1, col = DOWN ? 16 * (q & 1) + 4 * (2 * g + (q >> 1)) : 16 * g + 4 * q;
             const int k = 8 * h + ((l & 15) >> 2);
 #pragma unroll
-            for (int b = 0; b < BASES / 2; ++b)
+            for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
                     at[2 * b + u] = (k + 4 * u) * (ROWS * 2) + ((((first + 32 * b + col) >> 3) ^ swizzle<16>(k + 4 * u)) << 4) + (col & 4) * 2;
         }
     }
     __device__ __forceinline__ s16x8 read(const char *lds, int block, int s) const {
-        if constexpr (!TR) return *reinterpret_cast<const s16x8 *>(lds + at[s] + block * 4096);
+        if constexpr (!TR) return *reinterpret_cast<const s16x8 *>(lds + at[s] + block * 32 * BK * 2);
         else {
-            static_assert(BLOCKS <= 4, "");
             const s16x4 lo = lds_read_tr(lds + at[2 * block] + s * 16 * ROWS * 2), hi = lds_read_tr(lds + at[2 * block + 1] + s * 16 * ROWS * 2);
             return join(lo, hi);
         }
     }
 };
+
+// One step: copies of a later one are sent off, then the products of this one.  The two pointers are __restrict__, and the function
+// inlined, so that the compiler knows that the copies do not write what is read here: it would wait for them before the first read.
+template <typename T, bool TA, bool TB, bool WIDE, int BM, int BN, int FM, int FN, int THREADS, typename OA, typename OB, typename RA, typename RB, typename VA, typename VB>
+__device__ __forceinline__ void step(char *__restrict__ ahead, const char *__restrict__ now, OA &oa, OB &ob, const RA &ra, const RB &rb, VA &va,
+                                     VB &vb, f32x16 (&acc)[FM][FN], int w) {
+    constexpr int A_BYTES = BM * BK * 2;
+    if constexpr (WIDE) {
+            oa.copy(ahead, w);
+            ob.copy(ahead + A_BYTES, w);
+            oa.next();
+            ob.next();
+        } else {
+            oa.next();
+            ob.next();
+            oa.load(va);
+            ob.load(vb);
+        }
+#pragma unroll
+        for (int kk = 0; kk < BK / 16; ++kk) {
+            s16x8 fa[FM], fb[FN];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) fa[i] = ra.read(now, i, kk);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) fb[j] = rb.read(now + A_BYTES, j, kk);
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = mfma32<T>(fb[j], fa[i], acc[i][j]);
+        }
+}
 
 template <typename T, bool TA, bool TB, bool WIDE, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void gemm_kernel(Product p, Epilogue ep) {
@@ -252,52 +281,35 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void gemm_kernel(Produc
     ra.begin(wm, l);
     rb.begin(wn, l);
     s16x8 va[WIDE ? 1 : OA::N], vb[WIDE ? 1 : OB::N];
-    if (steps) {
-        if constexpr (WIDE) {
-            oa.copy(smem, w);
-            ob.copy(smem + A_BYTES, w);
-        } else {
-            oa.load(va);
-            ob.load(vb);
-            OA::put(smem, va, tid);
-            OB::put(smem + A_BYTES, vb, tid);
-        }
-    }
-    for (int s = 0; s < steps; ++s) {
-        wait_lds_dma();
-        __syncthreads();                                   // tile s is there, and tile s - 1 has been read by every wave
-        char *other = smem + ((s + 1) & 1) * STAGE;
-        const bool more = s + 1 < steps;
-        if (more) {
+    // (steps past the end are copied as well, as zeros without a read: the count of what is under way stays the same)
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; ++s) {
+            oa.copy(smem + s * STAGE, w);
+            ob.copy(smem + s * STAGE + A_BYTES, w);
             oa.next();
             ob.next();
-            if constexpr (WIDE) {
-                oa.copy(other, w);
-                ob.copy(other + A_BYTES, w);
-            } else {
-                oa.load(va);
-                ob.load(vb);
-            }
         }
-        const char *ta = smem + (s & 1) * STAGE, *tb = ta + A_BYTES;
-#pragma unroll
-        for (int kk = 0; kk < BK / 16; ++kk) {
-            s16x8 fa[FM], fb[FN];
-#pragma unroll
-            for (int i = 0; i < FM; ++i) fa[i] = ra.read(ta, i, kk);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) fb[j] = rb.read(tb, j, kk);
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = mfma32<T>(fb[j], fa[i], acc[i][j]);
-        }
-        if constexpr (!WIDE)
-            if (more) {
-                OA::put(other, va, tid);
-                OB::put(other + A_BYTES, vb, tid);
-            }
+    } else {
+        oa.load(va);
+        ob.load(vb);
+        OA::put(smem, va, tid);
+        OB::put(smem + A_BYTES, vb, tid);
     }
+    int slot = 0;
+    for (int s = 0; s < steps; ++s) {
+        // tile s is there (two later ones may be under way), and tile s - 1 has been read by every wave
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(WIDE ? (STAGES - 2) * (OA::N + OB::N) : 0) : "memory");
+        const int slot_now = slot;
+        char *ahead = smem + ((slot + (WIDE ? STAGES - 1 : 1)) & (STAGES - 1)) * STAGE;
+        slot = (slot + 1) & (STAGES - 1);
+        step<T, TA, TB, WIDE, BM, BN, FM, FN, THREADS>(ahead, smem + slot_now * STAGE, oa, ob, ra, rb, va, vb, acc, w);
+        if constexpr (!WIDE) {
+            OA::put(ahead, va, tid);
+            OB::put(ahead + A_BYTES, vb, tid);
+        }
+    }
+    wait_lds_dma();                                        // no copy outlives the workgroup
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -418,14 +430,14 @@ Choice choose(int64_t M, int64_t N, int64_t K, bool rows_ok, bool wide) {
     double least = 1e300;
     for (int kind = 1; kind <= (wide ? 2 : 1); ++kind) {
         const int64_t t = kind == 2 ? 256 : 128;
-        const int64_t tiles = ceil_div64(M, t) * ceil_div64(N, t), steps = ceil_div64(K, BK);
+        const int64_t tiles = ceil_div64(M, t) * ceil_div64(N, t), steps = ceil_div64(K, 64);
         const int at_once = kind == 2 ? 256 : 512;
         const double step_us = kind == 2 ? 1.2 : 0.9;
         for (int s = 1; s <= 16; s *= 2) {
             if (s > 1 && (steps / s < 8 || tiles * s > 2 * at_once)) break;
             double us = (double)ceil_div64(tiles * s, at_once) * ((double)ceil_div64(steps, s) * step_us + 3.0);
             if (s > 1) us += 4.0 + (double)M * N * 8.0 * s / 4.0e6;
-            if (us < least) least = us, best = {kind, s, 1, ceil_div64(steps, s) * BK};
+            if (us < least) least = us, best = {kind, s, 1, ceil_div64(steps, s) * 64};
         }
     }
     best.splits = (int)ceil_div64(K > 0 ? K : 1, best.split_k > 0 ? best.split_k : 1);
@@ -436,7 +448,7 @@ size_t parts_bytes(const Choice &c, int64_t M, int64_t N) { return c.splits > 1 
 
 template <typename T, bool TA, bool TB, bool WIDE, int BM, int BN, int WM, int WN>
 int launch_tiles(Product &p, const Epilogue &ep, hipStream_t stream) {
-    constexpr int LDS = 2 * (BM + BN) * BK * 2;
+    constexpr int LDS = STAGES * (BM + BN) * BK * 2;
     const int64_t tiles = ceil_div64(p.M, BM) * ceil_div64(p.N, BN);
     TOKENS_REQUIRE(tiles * p.splits < (1 << 22), "linear: more tiles than a launch takes");
     p.tiles_m = (int)ceil_div64(p.M, BM), p.tiles_n = (int)ceil_div64(p.N, BN), p.tiles = (int)tiles;
