@@ -104,10 +104,10 @@ template <typename T> __device__ __forceinline__ void finish8(const Epilogue &e,
 
 // ---------------------------------------------------------------------------------------------- the product
 // C[m][n] = sum_k A(m, k) B(n, k).  TA false: A(m, k) = a[m * lda + k]; true: a[k * lda + m]; TB likewise.
-// B's index runs down the registers of a result tile, in an order that gives a lane 16 consecutive n of one row m.
+// B's index runs down the registers of a result tile: a lane holds runs of 4 consecutive n of one row m.
 // The tiles of a step of 32 of the summed index wait in LDS, three steps ahead of the products: one step ahead (64 at a time, 128 KB as
 // well) the products wait for memory instead, 165 us for 137 Gflop where this takes TODO.
-constexpr int BK = 32, STAGES = 4;
+constexpr int BK = 32;
 
 struct Product {
     const void *a, *b;
@@ -123,8 +123,8 @@ struct Product {
 template <typename T, bool TR, int ROWS, int THREADS> struct Operand {
     static constexpr int C = TR ? ROWS / 8 : BK / 8;
     static constexpr int N = ROWS * (BK / 8) / THREADS;       // chunks of a thread
-    static constexpr int STEP = THREADS / C;                  // rows between them; a multiple of the swizzle's period
-    static_assert(STEP % 16 == 0, "one swizzle for all chunks of a thread");
+    static constexpr int STEP = THREADS / C;                  // rows between them
+    static_assert(STEP % 16 == 0 || (TR && STEP == 8), "the swizzle's period is 16 rows, and 8 rows on it differs by 2");
 
     const char *base;              // where the tile of this step begins
     int64_t step_bytes;
@@ -147,14 +147,15 @@ template <typename T, bool TR, int ROWS, int THREADS> struct Operand {
         if constexpr (TR) rows_in -= BK;
         else inner_in -= BK;
     }
-    __device__ __forceinline__ bool has(int i) const { return row + i * STEP < rows_in && c * 8 < inner_in; }
+    __device__ __forceinline__ int chunk(int i) const { return STEP == 8 ? c ^ ((i & 1) << 1) : c; }
+    __device__ __forceinline__ bool has(int i) const { return row + i * STEP < rows_in && chunk(i) * 8 < inner_in; }
 
     // every chunk is inside or outside as a whole: straight into LDS
     __device__ __forceinline__ void copy(char *lds, int w) const {
         const __amdgpu_buffer_rsrc_t rs = uniform_rsrc(base, kAnywhere);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const uint32_t off = has(i) ? (uint32_t)((row + i * STEP) * ld + c * 8) * 2u : kNowhere;
+            const uint32_t off = has(i) ? (uint32_t)((row + i * STEP) * ld + chunk(i) * 8) * 2u : kNowhere;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(lds + (i * THREADS + w * 64) * 16), 16, off, 0, 0, 0);
         }
     }
@@ -162,14 +163,15 @@ template <typename T, bool TR, int ROWS, int THREADS> struct Operand {
     __device__ __forceinline__ void load(s16x8 (&v)[N]) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const short *p = (const short *)base + (int64_t)(row + i * STEP) * ld + c * 8;
+            const int at = chunk(i) * 8;
+            const short *p = (const short *)base + (int64_t)(row + i * STEP) * ld + at;
             v[i] = (s16x8){0, 0, 0, 0, 0, 0, 0, 0};
             if (row + i * STEP < rows_in) {
-                if (c * 8 + 8 <= inner_in) __builtin_memcpy(&v[i], p, 16);
+                if (at + 8 <= inner_in) __builtin_memcpy(&v[i], p, 16);
                 else
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        if (c * 8 + e < inner_in) v[i][e] = p[e];
+                        if (at + e < inner_in) v[i][e] = p[e];
             }
         }
     }
@@ -179,21 +181,18 @@ template <typename T, bool TR, int ROWS, int THREADS> struct Operand {
     }
 };
 
-// A lane's 8 values for rows first .. + 32 BLOCKS and k = 16 s + 8 (l / 32) .. + 7.  `order`: lane i of a block's 32 has row i, or, for
-// the operand that runs down the registers, the row that makes registers 0 .. 15 of lane half h rows 16 h + 0 .. 15.
-template <typename T, bool TR, int ROWS, int BLOCKS, bool DOWN> struct Reader {
+// A lane's 8 values of row first + 32 block + l % 32 and k = 16 s + 8 (l / 32) .. + 7.
+template <typename T, bool TR, int ROWS, int BLOCKS> struct Reader {
     static constexpr int BASES = TR ? 2 * BLOCKS : BK / 16;
     int at[BASES];
 
     __device__ __forceinline__ void begin(int first, int l) {
         const int h = l >> 5, i = l & 31;
         if constexpr (!TR) {
-            const int row = DOWN ? 16 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3) : i;
 #pragma unroll
-            for (int s = 0; s < BASES; ++s) at[s] = (first + row) * (BK * 2) + (((2 * s + h) ^ swizzle<4>(row)) << 4);
+            for (int s = 0; s < BASES; ++s) at[s] = (first + i) * (BK * 2) + (((2 * s + h) ^ swizzle<4>(i)) << 4);
         } else {
-            const int q = l & 3, g = (l >> 4) & 1, col = DOWN ? 16 * (q & 1) + 4 * (2 * g + (q >> 1)) : 16 * g + 4 * q;
-            const int k = 8 * h + ((l & 15) >> 2);
+            const int col = (l & 16) + 4 * (l & 3), k = 8 * h + ((l & 15) >> 2);
 #pragma unroll
             for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
@@ -241,8 +240,8 @@ __device__ __forceinline__ void step(char *__restrict__ ahead, const char *__res
         }
 }
 
-template <typename T, bool TA, bool TB, bool WIDE, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void gemm_kernel(Product p, Epilogue ep) {
+template <typename T, bool TA, bool TB, bool WIDE, int BM, int BN, int WM, int WN, int STAGES>
+__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void gemm_kernel(Product p, Epilogue ep) {
     constexpr int THREADS = 64 * (BM / WM) * (BN / WN), FM = WM / 32, FN = WN / 32;
     constexpr int A_BYTES = BM * BK * 2, STAGE = (BM + BN) * BK * 2;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -251,10 +250,9 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void gemm_kernel(Produc
 
     // Workgroups go to the 8 XCDs in turn: each gets a run of tiles, in groups of 8 tiles of rows, so that what runs at one time
     // behind one L2 shares its operands.
-    const int per = (p.tiles + 7) / 8;
-    const int split = blockIdx.x / (per * 8), id = blockIdx.x - split * per * 8;
-    const int tile = (id & 7) * per + (id >> 3);
-    if (tile >= p.tiles) return;
+    const int per = (p.tiles * p.splits + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (id >= p.tiles * p.splits) return;
+    const int split = id / p.tiles, tile = id - split * p.tiles;
     const int group = tile / (8 * p.tiles_n), in_group = tile - group * 8 * p.tiles_n;
     const int high = min(8, p.tiles_m - group * 8);
     const int64_t m0 = (int64_t)(group * 8 + in_group % high) * BM, n0 = (int64_t)(in_group / high) * BN;
@@ -276,8 +274,8 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void gemm_kernel(Produc
     OB ob;
     oa.begin(p.a, p.lda, m0, p.M, k0, k1, tid);
     ob.begin(p.b, p.ldb, n0, p.N, k0, k1, tid);
-    Reader<T, TA, BM, FM, false> ra;
-    Reader<T, TB, BN, FN, true> rb;
+    Reader<T, TA, BM, FM> ra;
+    Reader<T, TB, BN, FN> rb;
     ra.begin(wm, l);
     rb.begin(wn, l);
     s16x8 va[WIDE ? 1 : OA::N], vb[WIDE ? 1 : OB::N];
@@ -301,36 +299,53 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void gemm_kernel(Produc
         // tile s is there (two later ones may be under way), and tile s - 1 has been read by every wave
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(WIDE ? (STAGES - 2) * (OA::N + OB::N) : 0) : "memory");
         const int slot_now = slot;
-        char *ahead = smem + ((slot + (WIDE ? STAGES - 1 : 1)) & (STAGES - 1)) * STAGE;
-        slot = (slot + 1) & (STAGES - 1);
+        const int to = slot + (WIDE ? STAGES - 1 : 1);
+        char *ahead = smem + (to >= STAGES ? to - STAGES : to) * STAGE;
+        slot = slot + 1 == STAGES ? 0 : slot + 1;
         step<T, TA, TB, WIDE, BM, BN, FM, FN, THREADS>(ahead, smem + slot_now * STAGE, oa, ob, ra, rb, va, vb, acc, w);
         if constexpr (!WIDE) {
             OA::put(ahead, va, tid);
             OB::put(ahead + A_BYTES, vb, tid);
         }
     }
-    wait_lds_dma();                                        // no copy outlives the workgroup
+    wait_lds_dma();                                        // no copy is under way any more
+    __syncthreads();
+    // Results go through LDS, 32 rows x WN columns of a wave at a time, so that eight lanes write 128 bytes of a row: written from where
+    // the products leave them, 8 bytes here and there, 134 MB took 70 us (1.9 TB/s).
+    static_assert(WN == 64 && 8 * 1024 * (THREADS / 64) <= STAGES * STAGE, "a wave's 8 KB");
+    char *own = smem + w * 8192;
 #pragma unroll
-    for (int i = 0; i < FM; ++i)
+    for (int i = 0; i < FM; ++i) {
 #pragma unroll
-        for (int j = 0; j < FN; ++j) {
-            const int64_t m = m0 + wm + 32 * i + (l & 31), n = n0 + wn + 32 * j + 16 * (l >> 5);
-            if (m >= p.M) continue;
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const f32x4 v = {acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]};
+                const int row = l & 31, chunk = 8 * j + (r >> 1) + (l >> 5);
+                *reinterpret_cast<f32x4 *>(own + row * 256 + ((chunk ^ (row & 15)) << 4)) = v;
+            }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int row = 8 * t + (l >> 3), chunk = 2 * (l & 7);
+            const f32x4 lo = *reinterpret_cast<const f32x4 *>(own + row * 256 + ((chunk ^ (row & 15)) << 4));
+            const f32x4 hi = *reinterpret_cast<const f32x4 *>(own + row * 256 + (((chunk + 1) ^ (row & 15)) << 4));
+            float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            const int64_t m = m0 + wm + 32 * i + row, n = n0 + wn + 8 * (l & 7);
+            if (m >= p.M || n >= p.N) continue;
             if (p.part) {
                 float *to = p.part + ((int64_t)split * p.M + m) * p.N + n;
+                if (p.wide_out) {
+                    *reinterpret_cast<f32x4 *>(to) = lo;
+                    *reinterpret_cast<f32x4 *>(to + 4) = hi;
+                } else
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (n + r < p.N) to[r] = acc[i][j][r];
-            } else {
-#pragma unroll
-                for (int r = 0; r < 16; r += 8) {
-                    float v[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = acc[i][j][r + e];
-                    if (n + r < p.N) finish8<T>(ep, (T *)p.c, m, n + r, p.N, v, p.wide_out);
-                }
-            }
+                    for (int e = 0; e < 8; ++e)
+                        if (n + e < p.N) to[e] = v[e];
+            } else finish8<T>(ep, (T *)p.c, m, n, p.N, v, p.wide_out);
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
 }
 
 // adds up the parts of K, in order
@@ -429,8 +444,8 @@ Choice choose(int64_t M, int64_t N, int64_t K, bool rows_ok, bool wide) {
     }
     double least = 1e300;
     for (int kind = 1; kind <= (wide ? 2 : 1); ++kind) {
-        const int64_t t = kind == 2 ? 256 : 128;
-        const int64_t tiles = ceil_div64(M, t) * ceil_div64(N, t), steps = ceil_div64(K, 64);
+        const int64_t t = kind == 2 ? 256 : 128, tn = t;
+        const int64_t tiles = ceil_div64(M, t) * ceil_div64(N, tn), steps = ceil_div64(K, 64);
         const int at_once = kind == 2 ? 256 : 512;
         const double step_us = kind == 2 ? 1.2 : 0.9;
         for (int s = 1; s <= 16; s *= 2) {
@@ -446,21 +461,21 @@ Choice choose(int64_t M, int64_t N, int64_t K, bool rows_ok, bool wide) {
 }
 size_t parts_bytes(const Choice &c, int64_t M, int64_t N) { return c.splits > 1 ? (size_t)c.splits * M * N * 4 : 0; }
 
-template <typename T, bool TA, bool TB, bool WIDE, int BM, int BN, int WM, int WN>
+template <typename T, bool TA, bool TB, bool WIDE, int BM, int BN, int WM, int WN, int STAGES>
 int launch_tiles(Product &p, const Epilogue &ep, hipStream_t stream) {
     constexpr int LDS = STAGES * (BM + BN) * BK * 2;
     const int64_t tiles = ceil_div64(p.M, BM) * ceil_div64(p.N, BN);
     TOKENS_REQUIRE(tiles * p.splits < (1 << 22), "linear: more tiles than a launch takes");
     p.tiles_m = (int)ceil_div64(p.M, BM), p.tiles_n = (int)ceil_div64(p.N, BN), p.tiles = (int)tiles;
     if constexpr (LDS > 65536) {
-        const hipError_t e = hipFuncSetAttribute((const void *)gemm_kernel<T, TA, TB, WIDE, BM, BN, WM, WN>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        const hipError_t e = hipFuncSetAttribute((const void *)gemm_kernel<T, TA, TB, WIDE, BM, BN, WM, WN, STAGES>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
         if (e != hipSuccess) {
             (void)hipGetLastError();
             tokens_error("linear: %d bytes of LDS: %s", LDS, hipGetErrorString(e));
             return (int)e;
         }
     }
-    hipLaunchKernelGGL((gemm_kernel<T, TA, TB, WIDE, BM, BN, WM, WN>), dim3((unsigned)((tiles + 7) / 8 * 8 * p.splits)),
+    hipLaunchKernelGGL((gemm_kernel<T, TA, TB, WIDE, BM, BN, WM, WN, STAGES>), dim3((unsigned)((tiles * p.splits + 7) / 8 * 8)),
                        dim3(64 * (BM / WM) * (BN / WN)), LDS, stream, p, ep);
     return tokens_launch_status("linear");
 }
@@ -487,9 +502,9 @@ int gemm(const void *a, int64_t lda, const void *b, int64_t ldb, void *c, int64_
             return tokens_launch_status("linear");
         }
     int rc;
-    if (!wide_in) rc = launch_tiles<T, TA, TB, false, 128, 128, 64, 64>(p, ep, stream);
-    else if (ch.kind == 2) rc = launch_tiles<T, TA, TB, true, 256, 256, 128, 64>(p, ep, stream);
-    else rc = launch_tiles<T, TA, TB, true, 128, 128, 64, 64>(p, ep, stream);
+    if (!wide_in) rc = launch_tiles<T, TA, TB, false, 128, 128, 64, 64, 4>(p, ep, stream);
+    else if (ch.kind == 2) rc = launch_tiles<T, TA, TB, true, 256, 256, 128, 64, 4>(p, ep, stream);
+    else rc = launch_tiles<T, TA, TB, true, 128, 128, 64, 64, 4>(p, ep, stream);
     if (rc || ch.splits == 1) return rc;
     hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)ceil_div64(M * ceil_div64(N, 8), 256)), dim3(256), 0, stream, p, ep);
     return tokens_launch_status("linear join");
