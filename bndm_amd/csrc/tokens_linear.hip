@@ -56,27 +56,31 @@ struct Epilogue {
     int act;
 };
 
-// N_ consecutive results of row m from column n on; WIDE: all of them are inside, and everything is in pieces of 16 bytes
-template <typename T> __device__ __forceinline__ void load8_of(float (&to)[8], const T *from) {
-    const s16x8 v = *reinterpret_cast<const s16x8 *>(from);
+// 8 values of a row, whatever its alignment; the first `left` of them where the row ends before
+template <typename T> __device__ __forceinline__ void load8_of(float (&to)[8], const T *from, int left) {
+    s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (left == 8) __builtin_memcpy(&v, from, 16);
+    else
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = reinterpret_cast<const short *>(from)[min(i, left - 1)];
 #pragma unroll
     for (int i = 0; i < 8; ++i) { const short s = v[i]; to[i] = widen<T>(s); }
 }
-template <typename T> __device__ __forceinline__ void finish8(const Epilogue &e, T *c, int64_t m, int64_t n, int64_t N, float (&v)[8], bool wide) {
-    const int left = (int)min((int64_t)8, N - n);
-    float bias[8] = {}, res[8] = {};
-    if (wide) {
-        if (e.bias) load8_of<T>(bias, (const T *)e.bias + n);
-        if (e.residual) load8_of<T>(res, (const T *)e.residual + m * e.ldr + n);
-    } else {
+template <typename T> __device__ __forceinline__ void store8_of(T *to, const float (&v)[8], int left) {
+    const s16x8 p = pack8<T>(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
+    if (left == 8) __builtin_memcpy(to, &p, 16);
+    else
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < left) {
-                if (e.bias) bias[i] = (float)((const T *)e.bias)[n + i];
-                if (e.residual) res[i] = (float)((const T *)e.residual)[m * e.ldr + n + i];
-            }
-    }
-    float y[8];
+        for (int i = 0; i < 7; ++i)
+            if (i < left) reinterpret_cast<short *>(to)[i] = p[i];
+}
+
+// 8 consecutive results of row m from column n on (n < N)
+template <typename T> __device__ __forceinline__ void finish8(const Epilogue &e, T *c, int64_t m, int64_t n, int64_t N, float (&v)[8]) {
+    const int left = (int)min((int64_t)8, N - n);
+    float bias[8] = {}, res[8] = {}, y[8];
+    if (e.bias) load8_of<T>(bias, (const T *)e.bias + n, left);
+    if (e.residual) load8_of<T>(res, (const T *)e.residual + m * e.ldr + n, left);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] += bias[i];
     if (e.act == BNDM_ACT_SILU) {
@@ -89,25 +93,19 @@ template <typename T> __device__ __forceinline__ void finish8(const Epilogue &e,
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = v[i] + res[i];
     }
-    if (wide) {
-        if (e.z) *reinterpret_cast<s16x8 *>((T *)e.z + m * N + n) = pack8<T>(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
-        *reinterpret_cast<s16x8 *>(c + m * N + n) = pack8<T>(y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < left) {
-                if (e.z) ((T *)e.z)[m * N + n + i] = (T)v[i];
-                c[m * N + n + i] = (T)y[i];
-            }
-    }
+    if (e.z) store8_of<T>((T *)e.z + m * N + n, v, left);
+    store8_of<T>(c + m * N + n, y, left);
 }
 
 // ---------------------------------------------------------------------------------------------- the product
 // C[m][n] = sum_k A(m, k) B(n, k).  TA false: A(m, k) = a[m * lda + k]; true: a[k * lda + m]; TB likewise.
 // B's index runs down the registers of a result tile: a lane holds runs of 4 consecutive n of one row m.
-// The tiles of a step of 32 of the summed index wait in LDS, three steps ahead of the products: one step ahead (64 at a time, 128 KB as
-// well) the products wait for memory instead, 165 us for 137 Gflop where this takes TODO.
+// The tiles of a step of 32 of the summed index are copied into LDS three steps ahead of the products: with one step of 64 ahead, in the
+// same 128 KB, 137 Gflop took 165 us, this way 131.
 constexpr int BK = 32;
+
+// how operands come in: pieces of 16 bytes straight into LDS; through registers; element by element (rows of less than 8)
+enum Loads { WIDE, ANY, NARROW };
 
 struct Product {
     const void *a, *b;
@@ -115,7 +113,7 @@ struct Product {
     float *part;                   // splits > 1: [splits][M][N] sums of the parts of K
     int64_t lda, ldb, M, N, K;
     int64_t split_k;               // summed index of a part, a multiple of BK
-    int tiles_m, tiles_n, tiles, splits, wide_out;
+    int tiles_m, tiles_n, tiles, splits;
 };
 
 // ROWS of one operand x 32 of the summed index in LDS, 16-byte chunks in swizzled places: rows along the summed index: [ROWS][4 chunks];
@@ -127,18 +125,20 @@ template <typename T, bool TR, int ROWS, int THREADS> struct Operand {
     static_assert(STEP % 16 == 0 || (TR && STEP == 8), "the swizzle's period is 16 rows, and 8 rows on it differs by 2");
 
     const char *base;              // where the tile of this step begins
+    const void *first;             // the operand itself
     int64_t step_bytes;
     int row, c;                    // of the thread's first chunk
     int ld;
     int64_t rows_in, inner_in;     // what is there from the first tile on: rows, elements of a row
 
     __device__ __forceinline__ static int place(int row) { return TR ? swizzle<16>(row) : swizzle<4>(row); }
-    __device__ __forceinline__ void begin(const void *p, int64_t ld_, int64_t first, int64_t extent, int64_t k0, int64_t k1, int tid) {
+    __device__ __forceinline__ void begin(const void *p, int64_t ld_, int64_t first_, int64_t extent, int64_t k0, int64_t k1, int tid) {
         ld = (int)ld_;
-        base = (const char *)p + (TR ? k0 * ld_ + first : first * ld_ + k0) * 2;
+        first = p;
+        base = (const char *)p + (TR ? k0 * ld_ + first_ : first_ * ld_ + k0) * 2;
         step_bytes = TR ? BK * ld_ * 2 : BK * 2;
-        rows_in = TR ? k1 - k0 : extent - first;
-        inner_in = TR ? extent - first : k1 - k0;
+        rows_in = TR ? k1 - k0 : extent - first_;
+        inner_in = TR ? extent - first_ : k1 - k0;
         row = tid / C;
         c = (tid % C) ^ place(row);
     }
@@ -159,25 +159,43 @@ template <typename T, bool TR, int ROWS, int THREADS> struct Operand {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(lds + (i * THREADS + w * 64) * 16), 16, off, 0, 0, 0);
         }
     }
-    // any alignment, any size: through registers
-    __device__ __forceinline__ void load(s16x8 (&v)[N]) const {
+    // Any alignment, any size: through registers.  A chunk that the row's end cuts short is read as the row's last 8 elements and shifted
+    // down when it is put away, so that no load waits for another.
+    struct Held { s16x8 v[N]; int left[N]; };
+    __device__ __forceinline__ void load(Held &h) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int at = chunk(i) * 8;
-            const short *p = (const short *)base + (int64_t)(row + i * STEP) * ld + at;
-            v[i] = (s16x8){0, 0, 0, 0, 0, 0, 0, 0};
-            if (row + i * STEP < rows_in) {
-                if (at + 8 <= inner_in) __builtin_memcpy(&v[i], p, 16);
-                else
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (at + e < inner_in) v[i][e] = p[e];
-            }
+            const int at = chunk(i) * 8, left = left_of(i);
+            const short *p = (const short *)base + (int64_t)(row + i * STEP) * ld + at - (8 - left);
+            h.left[i] = left;                              // (nothing to read here: the operand's first 8 elements, which are there)
+            __builtin_memcpy(&h.v[i], left ? p : (const short *)first, 16);
         }
     }
-    __device__ __forceinline__ static void put(char *lds, const s16x8 (&v)[N], int tid) {
+    // rows of less than 8 elements
+    __device__ __forceinline__ void load_narrow(Held &h) const {
 #pragma unroll
-        for (int i = 0; i < N; ++i) *reinterpret_cast<s16x8 *>(lds + (i * THREADS + tid) * 16) = v[i];
+        for (int i = 0; i < N; ++i) {
+            const int at = chunk(i) * 8, left = left_of(i);
+            const short *p = (const short *)base + (int64_t)(row + i * STEP) * ld + at;
+            h.left[i] = 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h.v[i][e] = e < left ? p[e] : (short)0;
+        }
+    }
+    __device__ __forceinline__ int left_of(int i) const {
+        return row + i * STEP < rows_in ? (int)max((int64_t)0, min((int64_t)8, inner_in - chunk(i) * 8)) : 0;
+    }
+    __device__ __forceinline__ static void put(char *lds, const Held &h, int tid) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint64_t lo = __builtin_bit_cast(u64x2, h.v[i]).x, hi = __builtin_bit_cast(u64x2, h.v[i]).y;
+            const int by = 16 * (8 - h.left[i]);           // 0 .. 128
+            u64x2 v;
+            v.x = by >= 64 ? hi >> (by & 63) : by ? (lo >> by) | (hi << (64 - by)) : lo;
+            v.y = by >= 64 ? 0 : hi >> by;
+            if (by == 128) v.x = 0;
+            *reinterpret_cast<u64x2 *>(lds + (i * THREADS + tid) * 16) = v;
+        }
     }
 };
 
@@ -209,38 +227,35 @@ template <typename T, bool TR, int ROWS, int BLOCKS> struct Reader {
     }
 };
 
-// One step: copies of a later one are sent off, then the products of this one.  The two pointers are __restrict__, and the function
-// inlined, so that the compiler knows that the copies do not write what is read here: it would wait for them before the first read.
-template <typename T, bool TA, bool TB, bool WIDE, int BM, int BN, int FM, int FN, int THREADS, typename OA, typename OB, typename RA, typename RB, typename VA, typename VB>
-__device__ __forceinline__ void step(char *__restrict__ ahead, const char *__restrict__ now, OA &oa, OB &ob, const RA &ra, const RB &rb, VA &va,
-                                     VB &vb, f32x16 (&acc)[FM][FN], int w) {
-    constexpr int A_BYTES = BM * BK * 2;
-    if constexpr (WIDE) {
-            oa.copy(ahead, w);
-            ob.copy(ahead + A_BYTES, w);
-            oa.next();
-            ob.next();
-        } else {
-            oa.next();
-            ob.next();
-            oa.load(va);
-            ob.load(vb);
-        }
+template <typename T, int FM, int FN, int A_BYTES, typename RA, typename RB>
+__device__ __forceinline__ void products(const char *now, const RA &ra, const RB &rb, f32x16 (&acc)[FM][FN]) {
 #pragma unroll
-        for (int kk = 0; kk < BK / 16; ++kk) {
-            s16x8 fa[FM], fb[FN];
+    for (int kk = 0; kk < BK / 16; ++kk) {
+        s16x8 fa[FM], fb[FN];
 #pragma unroll
-            for (int i = 0; i < FM; ++i) fa[i] = ra.read(now, i, kk);
+        for (int i = 0; i < FM; ++i) fa[i] = ra.read(now, i, kk);
 #pragma unroll
-            for (int j = 0; j < FN; ++j) fb[j] = rb.read(now + A_BYTES, j, kk);
+        for (int j = 0; j < FN; ++j) fb[j] = rb.read(now + A_BYTES, j, kk);
 #pragma unroll
-            for (int i = 0; i < FM; ++i)
+        for (int i = 0; i < FM; ++i)
 #pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = mfma32<T>(fb[j], fa[i], acc[i][j]);
-        }
+            for (int j = 0; j < FN; ++j) acc[i][j] = mfma32<T>(fb[j], fa[i], acc[i][j]);
+    }
 }
 
-template <typename T, bool TA, bool TB, bool WIDE, int BM, int BN, int WM, int WN, int STAGES>
+// One step: copies of a later one are sent off, then the products of this one.  The two pointers are __restrict__, and the function
+// inlined, so that the compiler knows that the copies do not write what is read here: it would wait for them before the first read.
+template <typename T, int FM, int FN, int A_BYTES, typename OA, typename OB, typename RA, typename RB>
+__device__ __forceinline__ void step(char *__restrict__ ahead, const char *__restrict__ now, OA &oa, OB &ob, const RA &ra, const RB &rb,
+                                     f32x16 (&acc)[FM][FN], int w) {
+    oa.copy(ahead, w);
+    ob.copy(ahead + A_BYTES, w);
+    oa.next();
+    ob.next();
+    products<T, FM, FN, A_BYTES>(now, ra, rb, acc);
+}
+
+template <typename T, bool TA, bool TB, Loads LOADS, int BM, int BN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void gemm_kernel(Product p, Epilogue ep) {
     constexpr int THREADS = 64 * (BM / WM) * (BN / WN), FM = WM / 32, FN = WN / 32;
     constexpr int A_BYTES = BM * BK * 2, STAGE = (BM + BN) * BK * 2;
@@ -278,9 +293,8 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void gemm_kernel(Pro
     Reader<T, TB, BN, FN> rb;
     ra.begin(wm, l);
     rb.begin(wn, l);
-    s16x8 va[WIDE ? 1 : OA::N], vb[WIDE ? 1 : OB::N];
-    // (steps past the end are copied as well, as zeros without a read: the count of what is under way stays the same)
-    if constexpr (WIDE) {
+    if constexpr (LOADS == WIDE) {
+        // (steps past the end are copied as well, as zeros without a read: the count of what is under way stays the same)
 #pragma unroll
         for (int s = 0; s < STAGES - 1; ++s) {
             oa.copy(smem + s * STAGE, w);
@@ -288,24 +302,42 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void gemm_kernel(Pro
             oa.next();
             ob.next();
         }
+        int slot = 0;
+        for (int s = 0; s < steps; ++s) {
+            // tile s is there (later ones may be under way), and tile s - 1 has been read by every wave
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * (OA::N + OB::N)) : "memory");
+            const int to = slot + STAGES - 1;
+            step<T, FM, FN, A_BYTES>(smem + (to >= STAGES ? to - STAGES : to) * STAGE, smem + slot * STAGE, oa, ob, ra, rb, acc, w);
+            slot = slot + 1 == STAGES ? 0 : slot + 1;
+        }
     } else {
-        oa.load(va);
-        ob.load(vb);
-        OA::put(smem, va, tid);
-        OB::put(smem + A_BYTES, vb, tid);
-    }
-    int slot = 0;
-    for (int s = 0; s < steps; ++s) {
-        // tile s is there (two later ones may be under way), and tile s - 1 has been read by every wave
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(WIDE ? (STAGES - 2) * (OA::N + OB::N) : 0) : "memory");
-        const int slot_now = slot;
-        const int to = slot + (WIDE ? STAGES - 1 : 1);
-        char *ahead = smem + (to >= STAGES ? to - STAGES : to) * STAGE;
-        slot = slot + 1 == STAGES ? 0 : slot + 1;
-        step<T, TA, TB, WIDE, BM, BN, FM, FN, THREADS>(ahead, smem + slot_now * STAGE, oa, ob, ra, rb, va, vb, acc, w);
-        if constexpr (!WIDE) {
-            OA::put(ahead, va, tid);
-            OB::put(ahead + A_BYTES, vb, tid);
+        // tile s + 1 in registers and tile s + 2 on its way there while tile s is used
+        typename OA::Held va[2];
+        typename OB::Held vb[2];
+        auto fetch = [&](typename OA::Held &a, typename OB::Held &b) {
+            if constexpr (LOADS == NARROW) {
+                oa.load_narrow(a);
+                ob.load_narrow(b);
+            } else {
+                oa.load(a);
+                ob.load(b);
+            }
+            oa.next();
+            ob.next();
+        };
+        auto turn = [&](int s, typename OA::Held &a, typename OB::Held &b) {
+            char *now = smem + (s & 1) * STAGE;
+            OA::put(now, a, tid);                          // (tile s - 2, which lay here, has been read: every wave is past barrier s - 1)
+            OB::put(now + A_BYTES, b, tid);
+            fetch(a, b);
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            products<T, FM, FN, A_BYTES>(now, ra, rb, acc);
+        };
+        fetch(va[0], vb[0]);
+        fetch(va[1], vb[1]);
+        for (int s = 0; s < steps; s += 2) {
+            turn(s, va[0], vb[0]);
+            if (s + 1 < steps) turn(s + 1, va[1], vb[1]);
         }
     }
     wait_lds_dma();                                        // no copy is under way any more
@@ -335,14 +367,12 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void gemm_kernel(Pro
             if (m >= p.M || n >= p.N) continue;
             if (p.part) {
                 float *to = p.part + ((int64_t)split * p.M + m) * p.N + n;
-                if (p.wide_out) {
-                    *reinterpret_cast<f32x4 *>(to) = lo;
-                    *reinterpret_cast<f32x4 *>(to + 4) = hi;
-                } else
+                if (n + 8 <= p.N) __builtin_memcpy(to, v, 32);
+                else
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
                         if (n + e < p.N) to[e] = v[e];
-            } else finish8<T>(ep, (T *)p.c, m, n, p.N, v, p.wide_out);
+            } else finish8<T>(ep, (T *)p.c, m, n, p.N, v);
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
@@ -357,17 +387,18 @@ template <typename T> __global__ __launch_bounds__(256) void join_kernel(Product
     float v[8] = {};
     for (int s = 0; s < p.splits; ++s) {
         const float *from = p.part + ((int64_t)s * p.M + m) * p.N + n;
-        if (p.wide_out) {
-            const f32x4 a = *reinterpret_cast<const f32x4 *>(from), b = *reinterpret_cast<const f32x4 *>(from + 4);
+        if (n + 8 <= p.N) {
+            float u[8];
+            __builtin_memcpy(u, from, 32);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] += a[e], v[4 + e] += b[e];
+            for (int e = 0; e < 8; ++e) v[e] += u[e];
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 if (n + e < p.N) v[e] += from[e];
         }
     }
-    finish8<T>(ep, (T *)p.c, m, n, p.N, v, p.wide_out);
+    finish8<T>(ep, (T *)p.c, m, n, p.N, v);
 }
 
 // ---------------------------------------------------------------------------------------------- few rows
@@ -422,7 +453,7 @@ template <typename T, int MT> __global__ __launch_bounds__(256) void rows_kernel
             const int col = (i & 1) * 8 + e;
             v[e] = (sums[0][col][i / 2] + sums[1][col][i / 2]) + (sums[2][col][i / 2] + sums[3][col][i / 2]);
         }
-        finish8<T>(ep, (T *)p.c, m, n, p.N, v, p.wide_out);
+        finish8<T>(ep, (T *)p.c, m, n, p.N, v);
     }
 }
 
@@ -461,21 +492,21 @@ Choice choose(int64_t M, int64_t N, int64_t K, bool rows_ok, bool wide) {
 }
 size_t parts_bytes(const Choice &c, int64_t M, int64_t N) { return c.splits > 1 ? (size_t)c.splits * M * N * 4 : 0; }
 
-template <typename T, bool TA, bool TB, bool WIDE, int BM, int BN, int WM, int WN, int STAGES>
+template <typename T, bool TA, bool TB, Loads LOADS, int BM, int BN, int WM, int WN, int STAGES>
 int launch_tiles(Product &p, const Epilogue &ep, hipStream_t stream) {
     constexpr int LDS = STAGES * (BM + BN) * BK * 2;
     const int64_t tiles = ceil_div64(p.M, BM) * ceil_div64(p.N, BN);
     TOKENS_REQUIRE(tiles * p.splits < (1 << 22), "linear: more tiles than a launch takes");
     p.tiles_m = (int)ceil_div64(p.M, BM), p.tiles_n = (int)ceil_div64(p.N, BN), p.tiles = (int)tiles;
     if constexpr (LDS > 65536) {
-        const hipError_t e = hipFuncSetAttribute((const void *)gemm_kernel<T, TA, TB, WIDE, BM, BN, WM, WN, STAGES>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        const hipError_t e = hipFuncSetAttribute((const void *)gemm_kernel<T, TA, TB, LOADS, BM, BN, WM, WN, STAGES>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
         if (e != hipSuccess) {
             (void)hipGetLastError();
             tokens_error("linear: %d bytes of LDS: %s", LDS, hipGetErrorString(e));
             return (int)e;
         }
     }
-    hipLaunchKernelGGL((gemm_kernel<T, TA, TB, WIDE, BM, BN, WM, WN, STAGES>), dim3((unsigned)((tiles * p.splits + 7) / 8 * 8)),
+    hipLaunchKernelGGL((gemm_kernel<T, TA, TB, LOADS, BM, BN, WM, WN, STAGES>), dim3((unsigned)((tiles * p.splits + 7) / 8 * 8)),
                        dim3(64 * (BM / WM) * (BN / WN)), LDS, stream, p, ep);
     return tokens_launch_status("linear");
 }
@@ -487,10 +518,8 @@ int gemm(const void *a, int64_t lda, const void *b, int64_t ldb, void *c, int64_
     // 16-byte loads: rows and the index along them in pieces of 8 elements (a piece is inside or outside as a whole)
     const bool wide_in = lda % 8 == 0 && ldb % 8 == 0 && (uint64_t)a % 16 == 0 && (uint64_t)b % 16 == 0 && (TA ? M : K) % 8 == 0 &&
                          (TB ? N : K) % 8 == 0;
-    const bool wide_out = N % 8 == 0 && (uint64_t)c % 16 == 0 && (!ep.bias || (uint64_t)ep.bias % 16 == 0) &&
-                          (!ep.residual || ((uint64_t)ep.residual % 16 == 0 && ep.ldr % 8 == 0)) && (!ep.z || (uint64_t)ep.z % 16 == 0);
     const Choice ch = choose(M, N, K, !TA && !TB, wide_in);
-    Product p = {a, b, c, ch.splits > 1 ? (float *)parts : nullptr, lda, ldb, M, N, K, ch.split_k, 0, 0, 0, ch.splits, (int)wide_out};
+    Product p = {a, b, c, ch.splits > 1 ? (float *)parts : nullptr, lda, ldb, M, N, K, ch.split_k, 0, 0, 0, ch.splits};
     if constexpr (!TA && !TB)
         if (ch.kind == 0) {
             p.tiles_m = (int)ceil_div64(M, 16 * ch.mt);
@@ -502,9 +531,10 @@ int gemm(const void *a, int64_t lda, const void *b, int64_t ldb, void *c, int64_
             return tokens_launch_status("linear");
         }
     int rc;
-    if (!wide_in) rc = launch_tiles<T, TA, TB, false, 128, 128, 64, 64, 4>(p, ep, stream);
-    else if (ch.kind == 2) rc = launch_tiles<T, TA, TB, true, 256, 256, 128, 64, 4>(p, ep, stream);
-    else rc = launch_tiles<T, TA, TB, true, 128, 128, 64, 64, 4>(p, ep, stream);
+    if ((TA ? M : K) < 8 || (TB ? N : K) < 8) rc = launch_tiles<T, TA, TB, NARROW, 128, 128, 64, 64, 2>(p, ep, stream);
+    else if (!wide_in) rc = launch_tiles<T, TA, TB, ANY, 128, 128, 64, 64, 2>(p, ep, stream);
+    else if (ch.kind == 2) rc = launch_tiles<T, TA, TB, WIDE, 256, 256, 128, 64, 4>(p, ep, stream);
+    else rc = launch_tiles<T, TA, TB, WIDE, 128, 128, 64, 64, 4>(p, ep, stream);
     if (rc || ch.splits == 1) return rc;
     hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)ceil_div64(M * ceil_div64(N, 8), 256)), dim3(256), 0, stream, p, ep);
     return tokens_launch_status("linear join");
@@ -522,7 +552,7 @@ constexpr int DZ_COLS = 256;
 
 template <typename T>
 __global__ __launch_bounds__(256) void dz_kernel(const T *dy, int64_t lddy, const T *z, T *dz, float *part, int64_t M, int64_t N, int64_t run,
-                                                 int act, int wide) {
+                                                 int act) {
     const int64_t n = (int64_t)blockIdx.x * DZ_COLS + (threadIdx.x & 31) * 8;
     const int64_t m1 = min(M, (int64_t)(blockIdx.y + 1) * run);
     const int left = n < N ? (int)min((int64_t)8, N - n) : 0;
@@ -530,18 +560,9 @@ __global__ __launch_bounds__(256) void dz_kernel(const T *dy, int64_t lddy, cons
     if (left) {
 #pragma unroll 2
         for (int64_t m = (int64_t)blockIdx.y * run + (threadIdx.x >> 5); m < m1; m += 8) {
-            float g[8] = {}, zz[8] = {};
-            if (wide) {
-                load8_of<T>(g, dy + m * lddy + n);
-                if (act != BNDM_ACT_NONE) load8_of<T>(zz, z + m * N + n);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (i < left) {
-                        g[i] = (float)dy[m * lddy + n + i];
-                        if (act != BNDM_ACT_NONE) zz[i] = (float)z[m * N + n + i];
-                    }
-            }
+            float g[8], zz[8] = {};
+            load8_of<T>(g, dy + m * lddy + n, left);
+            if (act != BNDM_ACT_NONE) load8_of<T>(zz, z + m * N + n, left);
             if (act == BNDM_ACT_SILU) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) g[i] *= act_slope(BNDM_ACT_SILU, zz[i]);
@@ -551,13 +572,7 @@ __global__ __launch_bounds__(256) void dz_kernel(const T *dy, int64_t lddy, cons
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum[i] += g[i];
-            if (act != BNDM_ACT_NONE) {
-                if (wide) *reinterpret_cast<s16x8 *>(dz + m * N + n) = pack8<T>(g[0], g[1], g[2], g[3], g[4], g[5], g[6], g[7]);
-                else
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (i < left) dz[m * N + n + i] = (T)g[i];
-            }
+            if (act != BNDM_ACT_NONE) store8_of<T>(dz + m * N + n, g, left);
         }
     }
     if (!part) return;
@@ -608,9 +623,8 @@ int backward(const void *dy, int64_t lddy, const void *z, const void *x, int64_t
         float *part = dbias ? (float *)((char *)workspace + dz_bytes(M, N, act)) : nullptr;
         const int64_t run = rows_of_run(M, N);
         const int runs = (int)ceil_div64(M, run);
-        const int wide = N % 8 == 0 && lddy % 8 == 0 && (uint64_t)dy % 16 == 0 && (uint64_t)z % 16 == 0;
         hipLaunchKernelGGL((dz_kernel<T>), dim3((unsigned)ceil_div64(N, DZ_COLS), (unsigned)runs), dim3(256), 0, stream, (const T *)dy, lddy,
-                           (const T *)z, (T *)workspace, part, M, N, run, act, wide);
+                           (const T *)z, (T *)workspace, part, M, N, run, act);
         if (int rc = tokens_launch_status("linear dz")) return rc;
         if (act != BNDM_ACT_NONE) dz = workspace, lddz = N;
         if (dbias) {

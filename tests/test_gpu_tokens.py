@@ -24,7 +24,7 @@ def normal(seed, *shape, dtype=F16, std=1.0):
 
 # ---------------------------------------------------------------------------------------------- linear
 SIZES = [(1, 8, 8), (1, 512, 1000), (5, 64, 24), (64, 512, 512), (130, 72, 136), (37, 515, 77), (3, 1, 1), (300, 200, 264), (129, 128, 1), (1000, 40, 130),
-         (65, 640, 24), (33, 523, 40), (100, 8192, 72), (100, 4099, 70), (8200, 40, 72),                # long sums, in parts
+         (65, 640, 24), (33, 523, 40), (200, 5, 70), (200, 70, 3), (7, 131, 140), (100, 3, 5), (100, 8192, 72), (100, 4099, 70), (8200, 40, 72),                # long sums, in parts
          (4104, 136, 2312), (4104, 2312, 136), (136, 2312, 4104)]                                      # large tiles, with edges
 
 
