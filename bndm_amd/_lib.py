@@ -43,7 +43,7 @@ class AttentionShape(C.Structure):
     _fields_ = [
         ("B", C.c_int64), ("Nq", C.c_int64), ("Nk", C.c_int64),
         ("H", C.c_int), ("Hk", C.c_int), ("D", C.c_int), ("Dv", C.c_int),
-        ("q_strides", C.c_int64 * 3), ("k_strides", C.c_int64 * 3), ("v_strides", C.c_int64 * 3),
+        *((t + i, C.c_int64) for t in "qkv" for i in ("_batch", "_token", "_head")),       # q_strides, k_strides, v_strides
         ("causal", C.c_int), ("dtype", C.c_int), ("lam_f32", C.c_int), ("scale", C.c_float),
     ]
 

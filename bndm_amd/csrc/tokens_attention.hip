@@ -44,7 +44,7 @@ struct Args {
     float *delta;                   // [B, 2H, Nq]: D1, D2
 };
 
-// tile of `R` rows of `C` chunks at `base` (rows `stride` elements apart) into LDS; rows >= rows_in and chunks >= chunks_in are zeros.
+// Tile of `R` rows of `C` chunks at `base` (rows `stride` elements apart) into LDS; rows >= rows_in and chunks >= chunks_in are zeros.
 // NW waves share the work; R * C is a multiple of 64 * NW
 template <int R, int C, int NW>
 __device__ __forceinline__ void stage_rows(char *lds, const void *base, int stride, int rows_in, int chunks_in, int w, int l) {
@@ -58,19 +58,26 @@ __device__ __forceinline__ void stage_rows(char *lds, const void *base, int stri
     }
 }
 
-// 8 values (chunk c) of row `row` of a tile
-template <int C> __device__ __forceinline__ s16x8 row_fragment(const char *lds, int row, int c) {
-    return *reinterpret_cast<const s16x8 *>(lds + row * (C * 16) + ((c ^ swizzle<C>(row)) << 4));
-}
-
-// operand whose rows are the tile's COLUMNS col0 .. + 31 and whose k are 16 of its rows, in the order in which a result tile holds
-// them: lane half h has rows row0 + 4 h + {0..3} and row0 + 8 + 4 h + {0..3}
-template <int C> __device__ __forceinline__ s16x8 column_fragment(const char *lds, int row0, int col0, int l) {
-    const int i = l & 15, col = col0 + (l & 16) + 4 * (i & 3), row = row0 + 4 * (l >> 5) + (i >> 2);
-    const s16x4 lo = lds_read_tr(lds + row * (C * 16) + (((col >> 3) ^ swizzle<C>(row)) << 4) + (col & 4) * 2);
-    const s16x4 hi = lds_read_tr(lds + (row + 8) * (C * 16) + (((col >> 3) ^ swizzle<C>(row + 8)) << 4) + (col & 4) * 2);
-    return join(lo, hi);
-}
+// Reads of a tile with rows of C chunks.  The swizzle is an exclusive or of a row's bits, which 32-row blocks (16 for columns) do not
+// reach, so that a lane's addresses differ by constants and by constant bits of the chunk.
+template <int C> struct RowReader {                    // 8 values (chunk 2 s + l / 32) of row block * 32 + l % 32
+    int at;
+    __device__ __forceinline__ void begin(int l) { at = (l & 31) * (C * 16) + (((l >> 5) ^ swizzle<C>(l & 31)) << 4); }
+    __device__ __forceinline__ s16x8 read(const char *lds, int block, int s) const {
+        return *reinterpret_cast<const s16x8 *>(lds + (at ^ ((s & 7) << 5)) + (s >> 3) * 256 + block * (32 * C * 16));
+    }
+};
+template <int C> struct ColumnReader {                 // operand whose rows are the tile's COLUMNS 32 t .. + 31 and whose k are its rows
+    int at;                                            // row0 .. row0 + 15 in the order in which a result tile holds them: lane half h has
+    __device__ __forceinline__ void begin(int l) {     // rows row0 + 4 h + {0..3} and row0 + 8 + 4 h + {0..3}
+        const int i = l & 15, col = (l & 16) + 4 * (i & 3), row = 4 * (l >> 5) + (i >> 2);
+        at = row * (C * 16) + (((col >> 3) ^ swizzle<C>(row)) << 4) + (col & 4) * 2;
+    }
+    __device__ __forceinline__ s16x8 read(const char *lds, int row0, int t) const {
+        const char *p = lds + row0 * (C * 16) + (t >> 2) * 256;
+        return join(lds_read_tr(p + (at ^ ((t & 3) << 6))), lds_read_tr(p + (at ^ ((t & 3) << 6) ^ 32) + 8 * C * 16));
+    }
+};
 
 // registers 8 s .. 8 s + 7 of a result tile as an operand whose k are rows 16 s .. 16 s + 15 in that order
 template <typename T> __device__ __forceinline__ s16x8 as_operand(const f32x16 &p, int s) {
@@ -86,8 +93,47 @@ template <int N> __device__ __forceinline__ void clear(f32x16 (&x)[N]) {
         for (int r = 0; r < 16; ++r) x[i][r] = 0.f;
 }
 
-__device__ __forceinline__ float both_halves_max(float x) { return fmaxf(x, __shfl_xor(x, 32)); }
-__device__ __forceinline__ float both_halves_sum(float x) { return x + __shfl_xor(x, 32); }
+// of the two lanes that hold one query
+__device__ __forceinline__ float both_halves_max(float x) {
+    const u32x2 r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+    const uint32_t a = r.x, b = r.y;
+    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+__device__ __forceinline__ float both_halves_sum(float x) {
+    const u32x2 r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+    const uint32_t a = r.x, b = r.y;
+    return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+}
+
+// the wave's copies into LDS have landed and its reads of LDS have been answered; then every wave's
+template <int NW> __device__ __forceinline__ void tile_there() {
+    if constexpr (NW == 1) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// 32 rows of DV results, a lane's row in result-tile order, through LDS (`own`: the wave's 32 DV elements) to rows of 16-byte pieces:
+// row r goes to to[offset of lane r], where `in`; f(t, r) is the value in register r of tile t.
+template <typename T, int DV, typename F>
+__device__ __forceinline__ void store_rows(char *own, T *to, int64_t offset, bool in, int Dv, int l, F f) {
+    constexpr int C = DV / 8;
+#pragma unroll
+    for (int t = 0; t < DV / 32; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int row = l & 31, col = 32 * t + tile_row(r, l >> 5);
+            *reinterpret_cast<s16x4 *>(own + row * (DV * 2) + (((col >> 3) ^ (row & (C - 1))) << 4) + (col & 4) * 2) =
+                pack4<T>(f(t, r), f(t, r + 1), f(t, r + 2), f(t, r + 3));
+        }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32 * C / 64; ++i) {
+        const int row = i * (64 / C) + l / C, c = l % C;
+        const int64_t at = __shfl(offset, row);
+        if (__shfl((int)in, row) && c * 8 < Dv)
+            *reinterpret_cast<s16x8 *>(to + at + c * 8) = *reinterpret_cast<const s16x8 *>(own + row * (DV * 2) + ((c ^ (row & (C - 1))) << 4));
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
 
 // 8 elements of a row at `p` as an operand, zeros where !in
 __device__ __forceinline__ s16x8 load8(const void *p, bool in) {
@@ -105,12 +151,15 @@ __device__ __forceinline__ int64_t length_of(const Args &a, int b) {
 }
 
 // ---------------------------------------------------------------------------------------------- forward
-// NW waves, 32 rows (queries) each; KT keys a tile.  DT: head size rounded up to 32, 64, 128; values are up to 2 DT wide.
+// NW waves, 32 rows (queries) each; KT keys a tile, 32 of them at a time.  DT: head size rounded up to 32, 64, 128; values are up to 2 DT
+// wide.  The running maximum is followed loosely: sums are scaled down only when it has grown by a factor of 2^8 (weights stay below 2^8
+// until then, and the final division takes care of them).
 template <typename T, int DT, int NW, int KT>
-__global__ __launch_bounds__(64 * NW) void attention_kernel(Args a) {
+__global__ __launch_bounds__(64 * NW, DT == 128 ? 1 : 2) void attention_kernel(Args a) {
     constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT;
     constexpr int K_BYTES = KT * CK * 16, V_BYTES = KT * CV * 16, STAGE = 2 * K_BYTES + V_BYTES;
-    __shared__ __attribute__((aligned(16))) char smem[2][STAGE];
+    static_assert(NW * 32 * DV * 2 <= 2 * STAGE, "results go through the same memory");
+    __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
     const int tid = threadIdx.x, l = tid & 63, h32 = l >> 5;
     const int w = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
 
@@ -144,6 +193,16 @@ __global__ __launch_bounds__(64 * NW) void attention_kernel(Args a) {
     }
     const int64_t j_begin = (int64_t)split * a.split_keys, j_end = min(most, j_begin + a.split_keys);
 
+    const T *kp = (const T *)a.k + (int64_t)b * a.kb + (int64_t)(2 * hk) * a.kh;
+    const T *vp = (const T *)a.v + (int64_t)b * a.vb + (int64_t)hk * a.vh;
+    auto fetch = [&](char *to, int64_t j) __attribute__((always_inline)) {
+        const int in = (int)min((int64_t)KT, len - j);
+        stage_rows<KT, CK, NW>(to, kp + j * a.kn, (int)a.kn, in, a.D / 8, w, l);
+        stage_rows<KT, CK, NW>(to + K_BYTES, kp + a.kh + j * a.kn, (int)a.kn, in, a.D / 8, w, l);
+        stage_rows<KT, CV, NW>(to + 2 * K_BYTES, vp + j * a.vn, (int)a.vn, in, a.Dv / 8, w, l);
+    };
+    if (j_begin < j_end) fetch(smem, j_begin);
+
     // ---- queries: right operands, in registers
     s16x8 qf[2][DT / 16];
 #pragma unroll
@@ -155,6 +214,10 @@ __global__ __launch_bounds__(64 * NW) void attention_kernel(Args a) {
             qf[m][s] = load8(p + c * 8, row_in && c * 8 < a.D);
         }
     }
+    RowReader<CK> keys;
+    ColumnReader<CV> values;
+    keys.begin(l);
+    values.begin(l);
 
     f32x16 acc[2][DV / 32];
     clear(acc[0]);
@@ -162,82 +225,70 @@ __global__ __launch_bounds__(64 * NW) void attention_kernel(Args a) {
     float top[2] = {kLowest, kLowest}, total[2] = {0.f, 0.f};
     const float to_log2 = a.scale * kLog2e;
 
-    const T *kp[2] = {(const T *)a.k + (int64_t)b * a.kb + (int64_t)(2 * hk) * a.kh, nullptr};
-    kp[1] = kp[0] + a.kh;
-    const T *vp = (const T *)a.v + (int64_t)b * a.vb + (int64_t)hk * a.vh;
-    auto fetch = [&](char *to, int64_t j) {
-        const int in = (int)min((int64_t)KT, len - j);
-        stage_rows<KT, CK, NW>(to, kp[0] + j * a.kn, (int)a.kn, in, a.D / 8, w, l);
-        stage_rows<KT, CK, NW>(to + K_BYTES, kp[1] + j * a.kn, (int)a.kn, in, a.D / 8, w, l);
-        stage_rows<KT, CV, NW>(to + 2 * K_BYTES, vp + j * a.vn, (int)a.vn, in, a.Dv / 8, w, l);
-    };
-
-    if (j_begin < j_end) fetch(smem[0], j_begin);
-    int buf = 0;
-    for (int64_t j = j_begin; j < j_end; j += KT, buf ^= 1) {
-        wait_lds_dma();
-        __syncthreads();
-        if (j + KT < j_end) fetch(smem[buf ^ 1], j + KT);
-        const char *ks = smem[buf], *vs = ks + 2 * K_BYTES;
-        const bool masked = j + KT > fewest;
-
-        s16x8 pf[2][KT / 16];
+    // One tile; the next one is on its way to `ahead`.  (__restrict__: the compiler would have it arrive before the first read of `now`.)
+    auto turn = [&](char *__restrict__ ahead, const char *__restrict__ now, int64_t j) __attribute__((always_inline)) {
+        tile_there<NW>();
+        if (j + KT < j_end) fetch(ahead, j + KT);
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            f32x16 s[KT / 32];
+        for (int t = 0; t < KT / 32; ++t) {
+            const bool masked = j + 32 * t + 32 > fewest;
+            f32x16 s[2];
+            s16x8 pf[2][2];
             clear(s);
 #pragma unroll
-            for (int t = 0; t < KT / 32; ++t)
+            for (int m = 0; m < 2; ++m)
 #pragma unroll
-                for (int d = 0; d < DT / 16; ++d)
-                    s[t] = mfma32<T>(row_fragment<CK>(ks + m * K_BYTES, 32 * t + (l & 31), 2 * d + h32), qf[m][d], s[t]);
-            if (masked) {
-                const int n = (int)min((int64_t)KT, max((int64_t)0, sees - j));
+                for (int d = 0; d < DT / 16; ++d) s[m] = mfma32<T>(keys.read(now + m * K_BYTES, t, d), qf[m][d], s[m]);
 #pragma unroll
-                for (int t = 0; t < KT / 32; ++t)
+            for (int m = 0; m < 2; ++m) {
+                if (masked) {
+                    const int n = (int)min((int64_t)32, max((int64_t)0, sees - j - 32 * t));
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
-                        if (32 * t + tile_row(r, h32) >= n) s[t][r] = -INFINITY;
-            }
-            float high = s[0][0];
+                        if (tile_row(r, h32) >= n) s[m][r] = -INFINITY;
+                }
+                float high = s[m][0];
 #pragma unroll
-            for (int t = 0; t < KT / 32; ++t)
+                for (int r = 1; r < 16; ++r) high = fmaxf(high, s[m][r]);
+                high = both_halves_max(high) * to_log2;
+                if (__any(high > top[m] + 8.0f)) {
+                    const float next = fmaxf(top[m], high), shrink = __builtin_amdgcn_exp2f(top[m] - next);
+                    top[m] = next;
+                    total[m] *= shrink;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) high = fmaxf(high, s[t][r]);
-            high = both_halves_max(high) * to_log2;
-            const float next = fmaxf(top[m], high);
-            const float shrink = __builtin_amdgcn_exp2f(top[m] - next);
-            top[m] = next;
-            float sum = 0.f;
+                    for (int v = 0; v < DV / 32; ++v)
 #pragma unroll
-            for (int t = 0; t < KT / 32; ++t)
+                        for (int r = 0; r < 16; ++r) acc[m][v][r] *= shrink;
+                }
+                float sum = 0.f;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    s[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], to_log2, -next));
-                    sum += s[t][r];
+                    s[m][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][r], to_log2, -top[m]));
+                    sum += s[m][r];
                 }
-            total[m] = total[m] * shrink + sum;
-#pragma unroll
-            for (int t = 0; t < DV / 32; ++t)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) acc[m][t][r] *= shrink;
-#pragma unroll
-            for (int t = 0; t < KT / 16; ++t) pf[m][t] = as_operand<T>(s[t / 2], t & 1);
-        }
-#pragma unroll
-        for (int t = 0; t < DV / 32; ++t)
-#pragma unroll
-            for (int s = 0; s < KT / 16; ++s) {
-                const s16x8 vf = column_fragment<CV>(vs, 16 * s, 32 * t, l);
-                acc[0][t] = mfma32<T>(vf, pf[0][s], acc[0][t]);
-                acc[1][t] = mfma32<T>(vf, pf[1][s], acc[1][t]);
+                total[m] += sum;
+                pf[m][0] = as_operand<T>(s[m], 0);
+                pf[m][1] = as_operand<T>(s[m], 1);
             }
+#pragma unroll
+            for (int v = 0; v < DV / 32; ++v)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const s16x8 vf = values.read(now + 2 * K_BYTES, 32 * t + 16 * x, v);
+                    acc[0][v] = mfma32<T>(vf, pf[0][x], acc[0][v]);
+                    acc[1][v] = mfma32<T>(vf, pf[1][x], acc[1][v]);
+                }
+        }
+    };
+    for (int64_t j = j_begin; j < j_end; j += 2 * KT) {
+        turn(smem + STAGE, smem, j);
+        if (j + KT < j_end) turn(smem, smem + STAGE, j + KT);
     }
     total[0] = both_halves_sum(total[0]);
     total[1] = both_halves_sum(total[1]);
-    if (!row_in) return;
 
     if (a.part) {                                           // unfinished sums of this part
+        if (!row_in) return;
         float *to = a.part + ((((int64_t)b * a.H + head) * a.Nq + i) * a.splits + split) * (2 * a.Dv + 4);
 #pragma unroll
         for (int m = 0; m < 2; ++m)
@@ -255,71 +306,75 @@ __global__ __launch_bounds__(64 * NW) void attention_kernel(Args a) {
     const float lam = lam_of<T>(a, head);
     const float w1 = total[0] == 0.f ? 0.f : 1.0f / total[0], w2 = total[1] == 0.f ? 0.f : 1.0f / total[1];
     const int64_t at = (((int64_t)b * a.Nq + i) * a.H + head) * a.Dv;
-#pragma unroll
-    for (int t = 0; t < DV / 32; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const int d = 32 * t + tile_row(r, h32);
-            if (d < a.Dv) {
-                float x[4], y[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    y[e] = acc[1][t][r + e] * w2;
-                    x[e] = acc[0][t][r + e] * w1 - lam * y[e];
-                }
-                *reinterpret_cast<s16x4 *>((T *)a.o + at + d) = pack4<T>(x[0], x[1], x[2], x[3]);
-                if (a.o2) *reinterpret_cast<s16x4 *>((T *)a.o2 + at + d) = pack4<T>(y[0], y[1], y[2], y[3]);
-            }
-        }
-    if (a.lse && h32 == 0)
+    tile_there<NW>();                                       // (every wave is through with the tiles)
+    char *own = smem + w * 32 * DV * 2;
+    store_rows<T, DV>(own, (T *)a.o, at, row_in, a.Dv, l, [&](int t, int r) { return acc[0][t][r] * w1 - lam * (acc[1][t][r] * w2); });
+    if (a.o2) store_rows<T, DV>(own, (T *)a.o2, at, row_in, a.Dv, l, [&](int t, int r) { return acc[1][t][r] * w2; });
+    if (a.lse && row_in && h32 == 0)
 #pragma unroll
         for (int m = 0; m < 2; ++m)
             a.lse[((int64_t)b * 2 * a.H + 2 * head + m) * a.Nq + i] = total[m] == 0.f ? INFINITY : top[m] + __log2f(total[m]);
 }
 
-// joins the parts of a row: one wave a row, each lane every 64th value
-template <typename T> __global__ __launch_bounds__(256) void attention_join_kernel(Args a) {
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int l = threadIdx.x & 63;
-    if (row >= (int64_t)a.B * a.H * a.Nq) return;
-    const int width = 2 * a.Dv + 4;
+// Joins the parts of a row: a workgroup a row, a thread a value of one map.  The parts' weights first, in LDS.
+constexpr int MAX_SPLITS = 128;
+template <typename T> __global__ __launch_bounds__(512) void attention_join_kernel(Args a) {
+    __shared__ float weight[2][MAX_SPLITS], first[256];
+    const int64_t row = blockIdx.x;
+    const int tid = threadIdx.x, width = 2 * a.Dv + 4;
     const float *p = a.part + row * a.splits * width;
-    float top[2] = {kLowest, kLowest}, total[2] = {0.f, 0.f};
-    for (int s = 0; s < a.splits; ++s)
+    if (tid < 128) {                                        // one wave a map
+        const int m = tid >> 6, l = tid & 63;
+        float t[2], s[2], top = kLowest, total = 0.f;
 #pragma unroll
-        for (int m = 0; m < 2; ++m) top[m] = fmaxf(top[m], p[(int64_t)s * width + 2 * a.Dv + m]);
-    for (int s = 0; s < a.splits; ++s)
+        for (int u = 0; u < 2; ++u) {
+            const bool in = l + 64 * u < a.splits;
+            t[u] = in ? p[(int64_t)(l + 64 * u) * width + 2 * a.Dv + m] : kLowest;
+            s[u] = in ? p[(int64_t)(l + 64 * u) * width + 2 * a.Dv + 2 + m] : 0.f;
+            top = fmaxf(top, t[u]);
+        }
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
-            total[m] += p[(int64_t)s * width + 2 * a.Dv + 2 + m] * __builtin_amdgcn_exp2f(p[(int64_t)s * width + 2 * a.Dv + m] - top[m]);
-    const float w[2] = {total[0] == 0.f ? 0.f : 1.0f / total[0], total[1] == 0.f ? 0.f : 1.0f / total[1]};
-    const int64_t i = row % a.Nq, bh = row / a.Nq;
-    const int head = (int)(bh % a.H);
-    const int64_t b = bh / a.H;
-    const float lam = lam_of<T>(a, head);
-    const int64_t at = ((b * a.Nq + i) * a.H + head) * a.Dv;
-    for (int d = l; d < a.Dv; d += 64) {
-        float x[2] = {0.f, 0.f};
-        for (int s = 0; s < a.splits; ++s)
+        for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
-                x[m] += p[(int64_t)s * width + m * a.Dv + d] * __builtin_amdgcn_exp2f(p[(int64_t)s * width + 2 * a.Dv + m] - top[m]);
-        ((T *)a.o)[at + d] = (T)(x[0] * w[0] - lam * (x[1] * w[1]));
-        if (a.o2) ((T *)a.o2)[at + d] = (T)(x[1] * w[1]);
+        for (int u = 0; u < 2; ++u) {
+            t[u] = __builtin_amdgcn_exp2f(t[u] - top);
+            total += s[u] * t[u];
+        }
+#pragma unroll
+        for (int x = 1; x < 64; x *= 2) total += __shfl_xor(total, x);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) weight[m][l + 64 * u] = total == 0.f ? 0.f : t[u] / total;
+        if (a.lse && l == 0) {
+            const int64_t i = row % a.Nq, bh = row / a.Nq;
+            a.lse[(2 * bh + m) * a.Nq + i] = total == 0.f ? INFINITY : top + __log2f(total);
+        }
     }
-    if (a.lse && l < 2) {
-        const float t = l ? total[1] : total[0], m = l ? top[1] : top[0];
-        a.lse[(b * 2 * a.H + 2 * head + l) * a.Nq + i] = t == 0.f ? INFINITY : m + __log2f(t);
+    __syncthreads();
+    const int m = tid >> 8, d = tid & 255;
+    float x = 0.f;
+    if (d < a.Dv) {
+#pragma unroll 8
+        for (int s = 0; s < a.splits; ++s) x += p[(int64_t)s * width + m * a.Dv + d] * weight[m][s];
+    }
+    if (m == 1) first[d] = x;
+    __syncthreads();
+    if (m == 0 && d < a.Dv) {
+        const int64_t i = row % a.Nq, bh = row / a.Nq;
+        const int head = (int)(bh % a.H);
+        const int64_t at = ((bh / a.H * a.Nq + i) * a.H + head) * a.Dv + d;
+        ((T *)a.o)[at] = (T)(x - lam_of<T>(a, head) * first[d]);
+        if (a.o2) ((T *)a.o2)[at] = (T)first[d];
     }
 }
 
 // ---------------------------------------------------------------------------------------------- gradients of the queries
 // As the forward pass: a lane holds one query, dS^T is at once the right operand of  dq^T += k^T dS^T.  Also D1, D2 for the next kernel.
 template <typename T, int DT, int KT>
-__global__ __launch_bounds__(THREADS) void attention_dq_kernel(Args a) {
+__global__ __launch_bounds__(THREADS, DT == 128 ? 1 : 2) void attention_dq_kernel(Args a) {
     constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT, NW = 4;
     constexpr int K_BYTES = KT * CK * 16, V_BYTES = KT * CV * 16, STAGE = 2 * K_BYTES + V_BYTES;
-    __shared__ __attribute__((aligned(16))) char smem[2][STAGE];
+    __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
+    static_assert(NW * 32 * DT * 2 <= 2 * STAGE, "results go through the same memory");
     const int tid = threadIdx.x, l = tid & 63, h32 = l >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int tiles = (int)((a.Nq + 127) / 128);
@@ -338,6 +393,7 @@ __global__ __launch_bounds__(THREADS) void attention_dq_kernel(Args a) {
         fewest = min(len, max((int64_t)0, start + (int64_t)tile * 128 + w * 32 + 1));
     }
 
+    const bool single = __any(sees == 1);
     s16x8 qf[2][DT / 16], gf[DV / 16];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
@@ -384,92 +440,121 @@ __global__ __launch_bounds__(THREADS) void attention_dq_kernel(Args a) {
     clear(acc[0]);
     clear(acc[1]);
     const float to_log2 = a.scale * kLog2e;
-    const T *kp[2] = {(const T *)a.k + (int64_t)b * a.kb + (int64_t)(2 * hk) * a.kh, nullptr};
-    kp[1] = kp[0] + a.kh;
+    const T *kp = (const T *)a.k + (int64_t)b * a.kb + (int64_t)(2 * hk) * a.kh;
     const T *vp = (const T *)a.v + (int64_t)b * a.vb + (int64_t)hk * a.vh;
-    auto fetch = [&](char *to, int64_t j) {
+    auto fetch = [&](char *to, int64_t j) __attribute__((always_inline)) {
         const int in = (int)min((int64_t)KT, len - j);
-        stage_rows<KT, CK, NW>(to, kp[0] + j * a.kn, (int)a.kn, in, a.D / 8, w, l);
-        stage_rows<KT, CK, NW>(to + K_BYTES, kp[1] + j * a.kn, (int)a.kn, in, a.D / 8, w, l);
+        stage_rows<KT, CK, NW>(to, kp + j * a.kn, (int)a.kn, in, a.D / 8, w, l);
+        stage_rows<KT, CK, NW>(to + K_BYTES, kp + a.kh + j * a.kn, (int)a.kn, in, a.D / 8, w, l);
         stage_rows<KT, CV, NW>(to + 2 * K_BYTES, vp + j * a.vn, (int)a.vn, in, a.Dv / 8, w, l);
     };
-    if (0 < j_end) fetch(smem[0], 0);
-    int buf = 0;
-    for (int64_t j = 0; j < j_end; j += KT, buf ^= 1) {
-        wait_lds_dma();
-        __syncthreads();
-        if (j + KT < j_end) fetch(smem[buf ^ 1], j + KT);
-        const char *ks = smem[buf], *vs = ks + 2 * K_BYTES;
-        const bool masked = j + KT > fewest || sees == 1;
+    RowReader<CK> keys;
+    RowReader<CV> values;
+    ColumnReader<CK> key_columns;
+    keys.begin(l);
+    values.begin(l);
+    key_columns.begin(l);
+    if (0 < j_end) fetch(smem, 0);
+    auto turn = [&](char *__restrict__ ahead, const char *__restrict__ now, int64_t j) __attribute__((always_inline)) {
+        tile_there<NW>();
+        if (j + KT < j_end) fetch(ahead, j + KT);
 #pragma unroll
         for (int t = 0; t < KT / 32; ++t) {
-            f32x16 dp[1], s[1];
+            const bool masked = j + 32 * t + 32 > fewest || single;
+            f32x16 dp[1], s[2];
             clear(dp);
+            clear(s);
 #pragma unroll
-            for (int d = 0; d < DV / 16; ++d) dp[0] = mfma32<T>(row_fragment<CV>(vs, 32 * t + (l & 31), 2 * d + h32), gf[d], dp[0]);
+            for (int d = 0; d < DV / 16; ++d) dp[0] = mfma32<T>(values.read(now + 2 * K_BYTES, t, d), gf[d], dp[0]);
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int d = 0; d < DT / 16; ++d) s[m] = mfma32<T>(keys.read(now + m * K_BYTES, t, d), qf[m][d], s[m]);
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
-                clear(s);
-#pragma unroll
-                for (int d = 0; d < DT / 16; ++d)
-                    s[0] = mfma32<T>(row_fragment<CK>(ks + m * K_BYTES, 32 * t + (l & 31), 2 * d + h32), qf[m][d], s[0]);
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    s[0][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], to_log2, -lse[m])) * (dp[0][r] - delta[m]);
+                    s[m][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][r], to_log2, -lse[m])) * (dp[0][r] - delta[m]);
                 if (masked) {                               // (a row that sees one key has weight 1 there whatever its score)
-                    const int n = sees == 1 ? 0 : (int)min((int64_t)KT, max((int64_t)0, sees - j));
+                    const int n = sees == 1 ? 0 : (int)min((int64_t)32, max((int64_t)0, sees - j - 32 * t));
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
-                        if (32 * t + tile_row(r, h32) >= n) s[0][r] = 0.f;
+                        if (tile_row(r, h32) >= n) s[m][r] = 0.f;
                 }
 #pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    const s16x8 ds = as_operand<T>(s[0], g);
+                for (int x = 0; x < 2; ++x) {
+                    const s16x8 ds = as_operand<T>(s[m], x);
 #pragma unroll
-                    for (int d = 0; d < DT / 32; ++d)
-                        acc[m][d] = mfma32<T>(column_fragment<CK>(ks + m * K_BYTES, 32 * t + 16 * g, 32 * d, l), ds, acc[m][d]);
+                    for (int d = 0; d < DT / 32; ++d) acc[m][d] = mfma32<T>(key_columns.read(now + m * K_BYTES, 32 * t + 16 * x, d), ds, acc[m][d]);
                 }
             }
         }
+    };
+    for (int64_t j = 0; j < j_end; j += 2 * KT) {
+        turn(smem + STAGE, smem, j);
+        if (j + KT < j_end) turn(smem, smem + STAGE, j + KT);
     }
-    if (!row_in) return;
+    tile_there<NW>();
+    char *own = smem + w * 32 * DT * 2;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
         const float f = m ? -lam * a.scale : a.scale;
-        T *to = (T *)a.dq + (((int64_t)b * a.Nq + i) * 2 * a.H + 2 * head + m) * a.D;
-#pragma unroll
-        for (int t = 0; t < DT / 32; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const int d = 32 * t + tile_row(r, h32);
-                if (d < a.D)
-                    *reinterpret_cast<s16x4 *>(to + d) = pack4<T>(acc[m][t][r] * f, acc[m][t][r + 1] * f, acc[m][t][r + 2] * f, acc[m][t][r + 3] * f);
-            }
+        store_rows<T, DT>(own, (T *)a.dq, (((int64_t)b * a.Nq + i) * 2 * a.H + 2 * head + m) * a.D, row_in, a.D, l,
+                          [&](int t, int r) { return acc[m][t][r] * f; });
     }
 }
 
 // ---------------------------------------------------------------------------------------------- gradients of keys and values
 // The other way round: a lane holds one key, scores have queries down and keys across, W = P1 - lam P2 and dS_m are the right operands
-// of  dv^T += do^T W  and  dk_m^T += q_m^T dS_m.  Keys and values of 128 rows stay in registers while the queries of every head that
-// reads them pass through LDS, so shared heads' gradients are summed here.
-template <typename T, int DT, int QT>
-__global__ __launch_bounds__(THREADS) void attention_dkv_kernel(Args a) {
-    constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT, NW = 4;
-    constexpr int Q_BYTES = QT * CK * 16, G_BYTES = QT * CV * 16, STAGE = 2 * Q_BYTES + G_BYTES;
-    __shared__ __attribute__((aligned(16))) char smem[2][STAGE];
-    __shared__ __attribute__((aligned(16))) float stats[2][4][QT];     // lse1, lse2, D1, D2 of the queries of a tile
+// of  dv^T += do^T W  and  dk_m^T += q_m^T dS_m.  A workgroup owns 64 keys, whose operands stay in registers while the queries of every
+// head that reads them pass through LDS, 64 at a time, so shared heads' gradients are summed here.  Two waves take the first half of the
+// queries in a tile, two the second; their sums are added at the end, in order.
+// WHAT: 1 dv, 2 dk, 3 both.  Both need 450 registers for heads of 128: there dv and dk are summed by a launch each.
+template <typename T, int DT, int WHAT>
+__global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
+    constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT, NW = 4, QT = 64;
+    constexpr bool VALUES = WHAT & 1, KEYS = (WHAT & 2) != 0;
+    constexpr int Q_BYTES = QT * CK * 16, G_BYTES = QT * CV * 16, STATS = 4 * QT * 4, STAGE = 2 * Q_BYTES + G_BYTES + STATS;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, l = tid & 63, h32 = l >> 5;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int tiles = (int)((a.Nk + 127) / 128);
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6), kw = w & 1, qw = w >> 1;
+    const int tiles = (int)((a.Nk + 63) / 64);
+    // (with a causal mask the first keys are seen by the most queries: they begin first)
     int id = blockIdx.x;
-    const int tile = id % tiles; id /= tiles;
-    const int hk = id % a.Hk, b = id / a.Hk;
+    const int hk = id % a.Hk; id /= a.Hk;
+    const int b = id % a.B, tile = id / a.B;
+    if (tile >= tiles) return;
     const int per = a.H / a.Hk;
     const int64_t start = start_of(a, b), len = length_of(a, b);
-    const int64_t key0 = (int64_t)tile * 128 + w * 32, key = key0 + (l & 31);
+    const int64_t first_key = (int64_t)tile * 64, key0 = first_key + kw * 32, key = key0 + (l & 31);
     const bool key_in = key < len;
 
-    s16x8 kf[2][DT / 16], vf[DV / 16];
+    // queries that see any key of this workgroup
+    int64_t i_first = 0;
+    if (a.causal) i_first = max((int64_t)0, first_key - start) / QT * QT;
+    if (first_key >= len) i_first = a.Nq;
+    const int per_head = i_first < a.Nq ? (int)((a.Nq - i_first + QT - 1) / QT) : 0;
+    int g_next = 0;                                         // the tile that is fetched next
+    int64_t i_next = i_first;
+    int steps = per_head * per;
+
+    auto fetch = [&](char *to) __attribute__((always_inline)) {
+        const int head = hk * per + g_next, in = (int)min((int64_t)QT, a.Nq - i_next);
+        const T *qp = (const T *)a.q + (int64_t)b * a.qb + i_next * a.qn + (int64_t)(2 * head) * a.qh;
+        stage_rows<QT, CK, NW>(to, qp, (int)a.qn, in, a.D / 8, w, l);
+        stage_rows<QT, CK, NW>(to + Q_BYTES, qp + a.qh, (int)a.qn, in, a.D / 8, w, l);
+        stage_rows<QT, CV, NW>(to + 2 * Q_BYTES, (const T *)a.dout + (int64_t)b * a.dob + i_next * a.don + (int64_t)head * a.doh, (int)a.don, in,
+                               a.Dv / 8, w, l);
+        // one of lse1, lse2, D1, D2 a wave.  (Queries past the end have zeros everywhere: their weight of 1 meets do = 0.)
+        const float *from = (w < 2 ? a.lse : a.delta) + ((int64_t)b * 2 * a.H + 2 * head + (w & 1)) * a.Nq + i_next;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(uniform_rsrc(from, kAnywhere), (lds_ptr_t)(to + 2 * Q_BYTES + G_BYTES + w * QT * 4), 4,
+                                                 l < in ? (uint32_t)l * 4u : kNowhere, 0, 0, 0);
+        i_next += QT;
+        if (i_next >= a.Nq) i_next = i_first, ++g_next;
+    };
+    if (steps) fetch(smem);
+
+    s16x8 kf[2][DT / 16], vf[KEYS ? DV / 16 : 1];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
         const T *p = (const T *)a.k + (int64_t)b * a.kb + (key_in ? key : 0) * a.kn + (int64_t)(2 * hk + m) * a.kh;
@@ -479,7 +564,7 @@ __global__ __launch_bounds__(THREADS) void attention_dkv_kernel(Args a) {
             kf[m][s] = load8(p + c * 8, key_in && c * 8 < a.D);
         }
     }
-    {
+    if constexpr (KEYS) {
         const T *p = (const T *)a.v + (int64_t)b * a.vb + (key_in ? key : 0) * a.vn + (int64_t)hk * a.vh;
 #pragma unroll
         for (int s = 0; s < DV / 16; ++s) {
@@ -487,119 +572,126 @@ __global__ __launch_bounds__(THREADS) void attention_dkv_kernel(Args a) {
             vf[s] = load8(p + c * 8, key_in && c * 8 < a.Dv);
         }
     }
-    f32x16 dk[2][DT / 32], dv[DV / 32];
+    RowReader<CK> queries;
+    RowReader<CV> grads;
+    ColumnReader<CK> query_columns;
+    ColumnReader<CV> grad_columns;
+    queries.begin(l);
+    grads.begin(l);
+    query_columns.begin(l);
+    grad_columns.begin(l);
+    f32x16 dk[KEYS ? 2 : 1][DT / 32], dv[VALUES ? DV / 32 : 1];
     clear(dk[0]);
-    clear(dk[1]);
+    clear(dk[KEYS ? 1 : 0]);
     clear(dv);
     const float to_log2 = a.scale * kLog2e;
 
-    // queries that see any key of this workgroup
-    int64_t i_begin = 0;
-    if (a.causal) i_begin = max((int64_t)0, (int64_t)tile * 128 - start) / QT * QT;
-    if ((int64_t)tile * 128 >= len) i_begin = a.Nq;
-    const int64_t i_first = i_begin;
-    const int per_head = i_first < a.Nq ? (int)((a.Nq - i_first + QT - 1) / QT) : 0;
-    const int steps = per_head * per;
-
-    auto fetch = [&](int to, int step) {
-        const int g = step / per_head;
-        const int64_t i = i_first + (int64_t)(step - g * per_head) * QT;
-        const int head = hk * per + g, in = (int)min((int64_t)QT, a.Nq - i);
-        const T *qp = (const T *)a.q + (int64_t)b * a.qb + i * a.qn + (int64_t)(2 * head) * a.qh;
-        stage_rows<QT, CK, NW>(smem[to], qp, (int)a.qn, in, a.D / 8, w, l);
-        stage_rows<QT, CK, NW>(smem[to] + Q_BYTES, qp + a.qh, (int)a.qn, in, a.D / 8, w, l);
-        stage_rows<QT, CV, NW>(smem[to] + 2 * Q_BYTES, (const T *)a.dout + (int64_t)b * a.dob + i * a.don + (int64_t)head * a.doh, (int)a.don, in,
-                               a.Dv / 8, w, l);
-        // (queries past the end: P = exp2(s - inf) = 0)
-        for (int e = tid; e < 4 * QT; e += THREADS) {
-            const int what = e / QT, r = e % QT;
-            const float *from = (what < 2 ? a.lse : a.delta) + ((int64_t)b * 2 * a.H + 2 * head + (what & 1)) * a.Nq + i;
-            stats[to][what][r] = r < in ? from[r] : what < 2 ? INFINITY : 0.f;
-        }
-    };
-    if (steps) fetch(0, 0);
-    for (int step = 0; step < steps; ++step) {
-        const int buf = step & 1;
-        wait_lds_dma();
-        __syncthreads();
-        if (step + 1 < steps) fetch(buf ^ 1, step + 1);
-        const int g = step / per_head;
-        const int64_t i0 = i_first + (int64_t)(step - g * per_head) * QT;
+    int g = 0;
+    int64_t i0 = i_first;
+    auto turn = [&](char *__restrict__ ahead, const char *__restrict__ now) __attribute__((always_inline)) {
+        tile_there<NW>();
+        if (steps > 1) fetch(ahead);
         const float lam = lam_of<T>(a, hk * per + g);
-        const char *qs = smem[buf], *gs = qs + 2 * Q_BYTES;
+        const char *gs = now + 2 * Q_BYTES;
+        const float *stats = reinterpret_cast<const float *>(gs + G_BYTES) + 32 * qw + 4 * h32;
+        const int64_t it = i0 + 32 * qw;
+        // some pair is hidden, or some row sees one key only
+        const bool masked = key0 + 32 > len || (a.causal && key0 + 31 > start + it) || len == 1 || (a.causal && start + it <= 0);
+        f32x16 dp[1], s[2];
+        clear(dp);
+        clear(s);
 #pragma unroll
-        for (int t = 0; t < QT / 32; ++t) {
-            const int64_t it = i0 + 32 * t;
-            // some pair is hidden, or some row sees one key only
-            const bool masked = key0 + 32 > len || (a.causal && key0 + 31 > start + it) || len == 1 || (a.causal && start + it <= 0);
-            f32x16 dp[1], s[1], wt;
-            clear(dp);
+        for (int m = 0; m < 2; ++m)
 #pragma unroll
-            for (int d = 0; d < DV / 16; ++d) dp[0] = mfma32<T>(row_fragment<CV>(gs, 32 * t + (l & 31), 2 * d + h32), vf[d], dp[0]);
+            for (int d = 0; d < DT / 16; ++d) s[m] = mfma32<T>(queries.read(now + m * Q_BYTES, qw, d), kf[m][d], s[m]);
+        if constexpr (KEYS)
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                clear(s);
+            for (int d = 0; d < DV / 16; ++d) dp[0] = mfma32<T>(grads.read(gs, qw, d), vf[d], dp[0]);
+        f32x16 wt;
 #pragma unroll
-                for (int d = 0; d < DT / 16; ++d)
-                    s[0] = mfma32<T>(row_fragment<CK>(qs + m * Q_BYTES, 32 * t + (l & 31), 2 * d + h32), kf[m][d], s[0]);
+        for (int m = 0; m < 2; ++m) {
 #pragma unroll
-                for (int r = 0; r < 16; r += 4) {
-                    const f32x4 ls = *reinterpret_cast<const f32x4 *>(&stats[buf][m][32 * t + tile_row(r, h32)]);
-                    const f32x4 de = *reinterpret_cast<const f32x4 *>(&stats[buf][2 + m][32 * t + tile_row(r, h32)]);
+            for (int r = 0; r < 16; r += 4) {
+                const f32x4 ls = *reinterpret_cast<const f32x4 *>(stats + m * QT + 2 * r);
+                f32x4 de = {0.f, 0.f, 0.f, 0.f};
+                if constexpr (KEYS) de = *reinterpret_cast<const f32x4 *>(stats + (2 + m) * QT + 2 * r);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r + e], to_log2, -ls[e]));
-                        float ds = p * (dp[0][r + e] - de[e]);
-                        if (masked) {
-                            const int64_t last = start + it + tile_row(r + e, h32);     // the last key that this query sees
-                            if (key >= len || (a.causal && key > last)) p = ds = 0.f;
-                            if (len == 1 || (a.causal && last == 0)) ds = 0.f;
-                        }
-                        if (m == 0) wt[r + e] = p;
-                        else {
-                            wt[r + e] -= lam * p;
-                            ds *= -lam;
-                        }
-                        s[0][r + e] = ds;
+                for (int e = 0; e < 4; ++e) {
+                    float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][r + e], to_log2, -ls[e]));
+                    float ds = p * (dp[0][r + e] - de[e]);
+                    if (masked) {
+                        const int64_t last = start + it + tile_row(r + e, h32);         // the last key that this query sees
+                        if (key >= len || (a.causal && key > last)) p = ds = 0.f;
+                        if (len == 1 || (a.causal && last == 0)) ds = 0.f;
                     }
-                }
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const s16x8 ds = as_operand<T>(s[0], x);
-#pragma unroll
-                    for (int d = 0; d < DT / 32; ++d)
-                        dk[m][d] = mfma32<T>(column_fragment<CK>(qs + m * Q_BYTES, 32 * t + 16 * x, 32 * d, l), ds, dk[m][d]);
+                    if (m == 0) wt[r + e] = p;
+                    else {
+                        wt[r + e] -= lam * p;
+                        ds *= -lam;
+                    }
+                    s[m][r + e] = ds;
                 }
             }
+            if constexpr (KEYS)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const s16x8 ds = as_operand<T>(s[m], x);
+#pragma unroll
+                    for (int d = 0; d < DT / 32; ++d) dk[m][d] = mfma32<T>(query_columns.read(now + m * Q_BYTES, 32 * qw + 16 * x, d), ds, dk[m][d]);
+                }
+        }
+        if constexpr (VALUES)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const s16x8 wf = as_operand<T>(wt, x);
 #pragma unroll
-                for (int d = 0; d < DV / 32; ++d) dv[d] = mfma32<T>(column_fragment<CV>(gs, 32 * t + 16 * x, 32 * d, l), wf, dv[d]);
+                for (int d = 0; d < DV / 32; ++d) dv[d] = mfma32<T>(grad_columns.read(gs, 32 * qw + 16 * x, d), wf, dv[d]);
+            }
+        i0 += QT;
+        if (i0 >= a.Nq) i0 = i_first, ++g;
+        --steps;
+    };
+    while (steps > 0) {
+        turn(smem + STAGE, smem);
+        if (steps > 0) turn(smem, smem + STAGE);
+    }
+    // ---- the second half's sums are added to the first's, 32 registers of a lane at a time
+    auto add = [&](f32x16 &x, f32x16 &y) __attribute__((always_inline)) {
+        tile_there<NW>();
+        f32x4 *at = reinterpret_cast<f32x4 *>(smem) + kw * 512 + l;
+        if (qw) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                at[r * 64] = (f32x4){x[4 * r], x[4 * r + 1], x[4 * r + 2], x[4 * r + 3]};
+                at[(4 + r) * 64] = (f32x4){y[4 * r], y[4 * r + 1], y[4 * r + 2], y[4 * r + 3]};
             }
         }
-    }
-    if (key >= a.Nk) return;
+        tile_there<NW>();
+        if (!qw) {
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        T *to = (T *)a.dk + (((int64_t)b * a.Nk + key) * 2 * a.Hk + 2 * hk + m) * a.D;
+            for (int r = 0; r < 4; ++r) {
+                const f32x4 u = at[r * 64], v = at[(4 + r) * 64];
 #pragma unroll
-        for (int t = 0; t < DT / 32; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const int d = 32 * t + tile_row(r, h32);
-                if (d < a.D)
-                    *reinterpret_cast<s16x4 *>(to + d) = pack4<T>(dk[m][t][r] * a.scale, dk[m][t][r + 1] * a.scale, dk[m][t][r + 2] * a.scale, dk[m][t][r + 3] * a.scale);
+                for (int e = 0; e < 4; ++e) x[4 * r + e] += u[e], y[4 * r + e] += v[e];
             }
-    }
-    T *to = (T *)a.dv + (((int64_t)b * a.Nk + key) * a.Hk + hk) * a.Dv;
-#pragma unroll
-    for (int t = 0; t < DV / 32; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const int d = 32 * t + tile_row(r, h32);
-            if (d < a.Dv) *reinterpret_cast<s16x4 *>(to + d) = pack4<T>(dv[t][r], dv[t][r + 1], dv[t][r + 2], dv[t][r + 3]);
         }
+    };
+    if constexpr (VALUES)
+#pragma unroll
+        for (int d = 0; d < DV / 32; d += 2) add(dv[d], dv[d + 1]);
+    if constexpr (KEYS)
+#pragma unroll
+        for (int d = 0; d < DT / 32; ++d) add(dk[0][d], dk[1][d]);
+    tile_there<NW>();
+    if (qw) return;
+    char *own = smem + kw * 32 * DV * 2;
+    const bool to_write = key < a.Nk;
+    const int64_t at = (int64_t)b * a.Nk + (to_write ? key : 0);
+    if constexpr (KEYS)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+            store_rows<T, DT>(own, (T *)a.dk, (at * 2 * a.Hk + 2 * hk + m) * a.D, to_write, a.D, l, [&](int t, int r) { return dk[m][t][r] * a.scale; });
+    if constexpr (VALUES) store_rows<T, DV>(own, (T *)a.dv, (at * a.Hk + hk) * a.Dv, to_write, a.Dv, l, [&](int t, int r) { return dv[t][r]; });
 }
 
 // dlam[h] = - sum over sequences and queries of D2: one workgroup a head, in a fixed order
@@ -644,6 +736,7 @@ Plan plan_of(const bndm_attention_shape &s) {
     int64_t splits = tiles >= want ? 1 : ceil_div64(want, tiles);
     const int64_t most = s.Nk / 256 < 1 ? 1 : s.Nk / 256;
     if (splits > most) splits = most;
+    if (splits > MAX_SPLITS) splits = MAX_SPLITS;
     p.split_keys = ceil_div64(ceil_div64(s.Nk, splits), 64) * 64;
     if (p.split_keys < 64) p.split_keys = 64;
     p.splits = (int)ceil_div64(s.Nk > 0 ? s.Nk : 1, p.split_keys);
@@ -657,20 +750,35 @@ template <typename T, int DT> int forward(const Args &a, const Plan &p, hipStrea
     else hipLaunchKernelGGL((attention_kernel<T, DT, 4, KT>), dim3((unsigned)p.blocks), dim3(256), 0, stream, a);
     if (int rc = tokens_launch_status("attention")) return rc;
     if (a.part) {
-        hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)ceil_div64((int64_t)a.B * a.H * a.Nq, 4)), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)((int64_t)a.B * a.H * a.Nq)), dim3(512), 0, stream, a);
         return tokens_launch_status("attention join");
     }
     return 0;
 }
 
+template <typename T, int DT, int WHAT> int launch_dkv(const Args &a, hipStream_t stream) {
+    constexpr int LDS = 2 * (64 * DT * 8 + 4 * 64 * 4);
+    const void *kernel = (const void *)attention_dkv_kernel<T, DT, WHAT>;
+    const hipError_t e = LDS > 65536 ? hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) : hipSuccess;
+    if (e != hipSuccess) {
+        (void)hipGetLastError();
+        tokens_error("attention dkv: %d bytes of LDS: %s", LDS, hipGetErrorString(e));
+        return (int)e;
+    }
+    hipLaunchKernelGGL((attention_dkv_kernel<T, DT, WHAT>), dim3((unsigned)(ceil_div64(a.Nk, 64) * a.Hk * a.B)), dim3(THREADS), LDS, stream, a);
+    return tokens_launch_status("attention dkv");
+}
+
 template <typename T, int DT> int backward(const Args &a, hipStream_t stream) {
     constexpr int KT = DT == 128 ? 32 : 64;
-    const int64_t nq = ceil_div64(a.Nq, 128) * a.H * a.B, nk = ceil_div64(a.Nk, 128) * a.Hk * a.B;
+    const int64_t nq = ceil_div64(a.Nq, 128) * a.H * a.B;
     hipLaunchKernelGGL((attention_dq_kernel<T, DT, KT>), dim3((unsigned)nq), dim3(THREADS), 0, stream, a);
     if (int rc = tokens_launch_status("attention dq")) return rc;
-    if (nk) {
-        hipLaunchKernelGGL((attention_dkv_kernel<T, DT, KT>), dim3((unsigned)nk), dim3(THREADS), 0, stream, a);
-        if (int rc = tokens_launch_status("attention dkv")) return rc;
+    if (a.Nk > 0) {
+        if constexpr (DT == 128) {
+            if (int rc = launch_dkv<T, DT, 1>(a, stream)) return rc;
+            if (int rc = launch_dkv<T, DT, 2>(a, stream)) return rc;
+        } else if (int rc = launch_dkv<T, DT, 3>(a, stream)) return rc;
     }
     hipLaunchKernelGGL((attention_dlam_kernel<T>), dim3(a.H), dim3(THREADS), 0, stream, a);
     return tokens_launch_status("attention dlam");
@@ -689,7 +797,7 @@ int check(const char *what, const bndm_attention_shape *s) {
         for (int i = 0; i < 3; ++i)
             TOKENS_REQUIRE(all[t][i] >= 0 && all[t][i] % 8 == 0 && (i != 1 || all[t][i] <= (1 << 23)), "%s: stride %lld: a multiple of 8, between tokens up to 2^23",
                            what, (long long)all[t][i]);
-    TOKENS_REQUIRE(ceil_div64(s->Nq, 32) * s->H * s->B < (1 << 24) && ceil_div64(s->Nk, 128) * s->Hk * s->B < (1 << 24), "%s: more tiles than a launch takes", what);
+    TOKENS_REQUIRE(ceil_div64(s->Nq, 32) * s->H * s->B < (1 << 24) && ceil_div64(s->Nk, 64) * s->Hk * s->B < (1 << 24), "%s: more tiles than a launch takes", what);
     return 0;
 }
 

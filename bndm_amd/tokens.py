@@ -24,13 +24,20 @@ _POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 _Strides = C.c_int64 * 3
 
 
+# the handle of a device's current stream: what torch.cuda.current_stream(index).cuda_stream is, without making the Stream (2.6 us, more
+# than some of these kernels take)
+_stream_of = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    lambda index: torch.cuda.current_stream(index).cuda_stream
+
+
 def _launch(fn, what, device, *args):
     """fn(*args, stream) on the current stream of ``device``."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _stream_of(index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+            rc = fn(*args, _stream_of(index))
     if rc:
         _lib.check_tokens(rc, what)
 
@@ -41,8 +48,9 @@ def _ptr(t):
 
 def _same(what, first, **others):
     """The tensors have the first one's type and device."""
+    dtype, device = first.dtype, first.device
     for name, t in others.items():
-        if t is not None and (t.dtype != first.dtype or t.device != first.device):
+        if t is not None and (t.dtype != dtype or t.device != device):
             raise ValueError(f"{what}: {name} is {t.dtype} on {t.device}, not {first.dtype} on {first.device}")
 
 
@@ -54,13 +62,18 @@ def _type_of(what, t, types):
 
 
 def _recording(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 # ---------------------------------------------------------------------------------------------- linear
 def _rows(t, width):
     """``t`` as rows of ``width`` next to each other's elements, and the distance of two rows."""
-    t = t.reshape(-1, width)
+    if t.dim() != 2:
+        t = t.reshape(-1, width)
     if width > 1 and t.stride(1) != 1:
         t = t.contiguous()
     return t, t.stride(0) if t.shape[0] > 1 else width
@@ -214,28 +227,23 @@ def rotary(q, k, positions, sections, base=10000.0, interleaved=False):
 
 
 # ---------------------------------------------------------------------------------------------- differential attention
-def _strides(t):
-    return [0 if s == 1 else d for s, d in zip(t.shape[:3], t.stride())]
-
-
 def _aligned(t):
-    """``t`` [B, N, H, D] as the kernels read it: heads' elements next to each other, all else in steps of 16 bytes."""
-    if (t.stride(3) == 1 or t.shape[3] == 1) and t.data_ptr() % 16 == 0 and all(s % 8 == 0 and s >= 0 for s in _strides(t)):
-        return t
+    """``t`` [B, N, H, D] as the kernels read it -- heads' elements next to each other, all else in steps of 16 bytes -- and its strides."""
+    b, n, h, d = t.shape
+    sb, sn, sh, sd = t.stride()
+    sb, sn, sh = 0 if b == 1 else sb, 0 if n == 1 else sn, 0 if h == 1 else sh
+    if (sd == 1 or d == 1) and not (t.data_ptr() % 16 or sb % 8 or sn % 8 or sh % 8):
+        return t, (sb, sn, sh)
     t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
-
-
-def _shape_of(q, k, v, lam, causal, scale, dtype):
-    b, nq, maps, d = q.shape
-    return _lib.AttentionShape(b, nq, k.shape[1], maps // 2, v.shape[2], d, v.shape[3], _Strides(*_strides(q)), _Strides(*_strides(k)),
-                               _Strides(*_strides(v)), causal, dtype, int(lam.dtype == torch.float32), scale)
+    if t.data_ptr() % 16 or d % 8:                          # (a head size that the kernels refuse: any strides will do)
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t, (n * h * d, h * d, d)
 
 
 def _attention_forward(q, k, v, lam, q_start, kv_lengths, causal, scale, dtype, keep):
-    q, k, v = _aligned(q), _aligned(k), _aligned(v)
-    b, nq, maps, _ = q.shape
-    shape = _shape_of(q, k, v, lam, causal, scale, dtype)
+    b, nq, maps, d = q.shape
+    (q, qs), (k, ks), (v, vs) = _aligned(q), _aligned(k), _aligned(v)
+    shape = _lib.AttentionShape(b, nq, k.shape[1], maps // 2, v.shape[2], d, v.shape[3], *qs, *ks, *vs, causal, dtype, lam.dtype == torch.float32, scale)
     o = torch.empty((b, nq, maps // 2, v.shape[3]), dtype=q.dtype, device=q.device)
     o2 = torch.empty_like(o) if keep else None
     lse = torch.empty((b, maps, nq), dtype=torch.float32, device=q.device) if keep else None
@@ -266,14 +274,16 @@ class _DifferentialAttention(torch.autograd.Function):
             for t in (dq, dk, dv, dlam):
                 t.zero_()
         else:
-            q, k, v, dout = _aligned(q), _aligned(k), _aligned(v), _aligned(dout)
-            shape = _shape_of(q, k, v, lam, causal, scale, dtype)
+            b, nq, maps, d = q.shape
+            (q, qs), (k, ks), (v, vs), (dout, ds) = _aligned(q), _aligned(k), _aligned(v), _aligned(dout)
+            shape = _lib.AttentionShape(b, nq, k.shape[1], maps // 2, v.shape[2], d, v.shape[3], *qs, *ks, *vs, causal, dtype,
+                                        lam.dtype == torch.float32, scale)
             lib = _lib.load_tokens()
             need = lib.bndm_tokens_attention_backward_workspace_bytes(shape)
             work = torch.empty(need, dtype=torch.uint8, device=q.device)
             _launch(lib.bndm_tokens_attention_backward, "differential_attention backward", q.device, shape, q.data_ptr(), k.data_ptr(),
                     v.data_ptr(), lam.data_ptr(), _ptr(q_start), _ptr(kv_lengths), o.data_ptr(), o2.data_ptr(), lse.data_ptr(),
-                    dout.data_ptr(), _Strides(*_strides(dout)), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr(), work.data_ptr(),
+                    dout.data_ptr(), _Strides(*ds), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr(), work.data_ptr(),
                     need)
         want = ctx.needs_input_grad
         return (dq if want[0] else None, dk if want[1] else None, dv if want[2] else None, dlam if want[3] else None) + (None,) * 5

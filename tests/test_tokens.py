@@ -85,7 +85,9 @@ def test_attention_refusals(lib):
     def shape(**change):
         v = dict(B=2, Nq=1, Nk=4096, H=4, Hk=2, D=64, Dv=128, q=S(512, 512, 64), k=S(1024, 256, 64), v=S(1024, 256, 128), causal=0, dtype=0, lam_f32=0,
                  scale=0.125)
-        return AttentionShape(*{**v, **change}.values())
+        v.update(change)
+        flat = [x for key in v for x in (v[key] if key in "qkv" else [v[key]])]
+        return AttentionShape(*flat)
 
     need = lib.bndm_tokens_attention_workspace_bytes(shape())
     assert need > 0                                          # few queries, many keys: split
