@@ -44,19 +44,34 @@ struct Args {
     float *delta;                   // [B, 2H, Nq]: D1, D2
 };
 
-// Tile of `R` rows of `C` chunks at `base` (rows `stride` elements apart) into LDS; rows >= rows_in and chunks >= chunks_in are zeros.
-// NW waves share the work; R * C is a multiple of 64 * NW
-template <int R, int C, int NW>
-__device__ __forceinline__ void stage_rows(char *lds, const void *base, int stride, int rows_in, int chunks_in, int w, int l) {
-    const __amdgpu_buffer_rsrc_t rs = uniform_rsrc(base, kAnywhere);
+// Copies tiles of R rows of C chunks into LDS, NW waves together.  Rows past rows_in and chunks past the head's size become zeros.  A lane's
+// offset is the same for all its pieces but for whole rows, which the scalar offset adds.
+template <int R, int C, int NW> struct Stager {
+    static constexpr int N = R * C < 64 * NW ? 1 : R * C / (64 * NW), STEP = 64 * NW / C;  // pieces of a lane, rows between them
+    int row;
+    uint32_t off[STEP % 16 ? 16 / STEP : 1];                // (the swizzle's period is 16 rows)
+    int step_bytes;
+
+    __device__ __forceinline__ void begin(int64_t stride, int chunks_in, int w, int l) {
+        const int at = w * 64 + l;
+        row = at / C;
+        step_bytes = (int)stride * STEP * 2;
 #pragma unroll
-    for (int i = 0; i < R * C / (64 * NW); ++i) {
-        const int at = (i * NW + w) * 64 + l, row = at / C, c = (at % C) ^ swizzle<C>(row);
-        const bool in = row < rows_in && c < chunks_in;
-        const uint32_t off = in ? (uint32_t)(row * stride + c * 8) * 2u : kNowhere;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(lds + (i * NW + w) * 1024), 16, off, 0, 0, 0);
+        for (int i = 0; i < (int)(sizeof(off) / 4); ++i) {
+            const int c = (at % C) ^ swizzle<C>(row + i * STEP);
+            off[i] = c < chunks_in ? (uint32_t)(row * (int)stride + c * 8) * 2u : kNowhere;
+        }
     }
-}
+    __device__ __forceinline__ void copy(char *lds, const void *base, int rows_in, int w) const {
+        if (R * C < 64 * NW && w * 64 >= R * C) return;     // (fewer pieces than lanes: the first waves')
+        const __amdgpu_buffer_rsrc_t rs = uniform_rsrc(base, kAnywhere);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t o = row < rows_in - i * STEP ? off[i % (sizeof(off) / 4)] : kNowhere;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(lds + (i * NW + w) * 1024), 16, o, i * step_bytes, 0, 0);
+        }
+    }
+};
 
 // Reads of a tile with rows of C chunks.  The swizzle is an exclusive or of a row's bits, which 32-row blocks (16 for columns) do not
 // reach, so that a lane's addresses differ by constants and by constant bits of the chunk.
@@ -151,169 +166,178 @@ __device__ __forceinline__ int64_t length_of(const Args &a, int b) {
 }
 
 // ---------------------------------------------------------------------------------------------- forward
-// NW waves, 32 rows (queries) each; KT keys a tile, 32 of them at a time.  DT: head size rounded up to 32, 64, 128; values are up to 2 DT
-// wide.  The running maximum is followed loosely: sums are scaled down only when it has grown by a factor of 2^8 (weights stay below 2^8
-// until then, and the final division takes care of them).
-template <typename T, int DT, int NW, int KT>
-__global__ __launch_bounds__(64 * NW, DT == 128 ? 1 : 2) void attention_kernel(Args a) {
-    constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT;
+// NQ groups of 32 rows (queries), two waves each: one a map, so that a map's sums are all that a wave holds (with both maps in one wave,
+// heads of 64 spilled at two waves a SIMD: 570 us where this takes TODO).  KT keys a tile, 32 of them at a time.  DT: head size rounded up
+// to 32, 64, 128; values are up to 2 DT wide.  The running maximum is followed loosely: sums are scaled down only when it has grown by a
+// factor of 2^8 (weights stay below 2^8 until then, and the final division takes care of them).
+template <typename T, int DT, int NQ, int KT>
+__global__ __launch_bounds__(128 * NQ, DT == 32 ? 3 : 2) void attention_kernel(Args a) {
+    constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT, NW = 2 * NQ;
     constexpr int K_BYTES = KT * CK * 16, V_BYTES = KT * CV * 16, STAGE = 2 * K_BYTES + V_BYTES;
-    static_assert(NW * 32 * DV * 2 <= 2 * STAGE, "results go through the same memory");
+    static_assert(NQ * 32 * DV * 2 <= 2 * STAGE && NQ * 8192 <= 2 * STAGE, "results go through the same memory");
     __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
     const int tid = threadIdx.x, l = tid & 63, h32 = l >> 5;
-    const int w = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6), m = w & 1, qw = w >> 1;
 
     // ---- which rows: (batch, group of query heads, tile of rows, part of the keys)
     const int64_t rows = a.Nq * a.heads_per_row;
-    const int tiles = (int)((rows + 32 * NW - 1) / (32 * NW));
+    const int tiles = (int)((rows + 32 * NQ - 1) / (32 * NQ));
     int id = blockIdx.x;
     const int split = id % a.splits; id /= a.splits;
     const int tile = id % tiles; id /= tiles;
     const int groups = a.H / a.heads_per_row;
     const int group = id % groups, b = id / groups;
     const int hk = group * a.heads_per_row / (a.H / a.Hk);
-    const int64_t row = (int64_t)tile * 32 * NW + w * 32 + (l & 31);
+    const int64_t row = (int64_t)tile * 32 * NQ + qw * 32 + (l & 31);
     const bool row_in = row < rows;
     const int sub = row_in ? (int)(row / a.Nq) : 0;
     const int64_t i = row_in ? row - (int64_t)sub * a.Nq : 0;
     const int head = group * a.heads_per_row + sub;
 
-    const int64_t start = start_of(a, b), len = length_of(a, b);
-    const int64_t sees = !row_in ? 0 : a.causal ? min(len, max((int64_t)0, start + i + 1)) : len;   // keys that this row sees
-    // (rows of one head are in order; several heads in one tile: the last query's keys for all)
-    int64_t most = len;
-    if (a.causal) {
-        const int64_t last = a.heads_per_row > 1 ? a.Nq - 1 : min(a.Nq - 1, (int64_t)(tile + 1) * 32 * NW - 1);
-        most = min(len, max((int64_t)0, start + last + 1));
-    }
-    int64_t fewest = len;                                   // keys that every row of the wave sees
-    if (a.causal) {
-        const int64_t first = a.heads_per_row > 1 ? 0 : (int64_t)tile * 32 * NW + w * 32;
-        fewest = min(len, max((int64_t)0, start + first + 1));
-    }
-    const int64_t j_begin = (int64_t)split * a.split_keys, j_end = min(most, j_begin + a.split_keys);
+    const int64_t start = start_of(a, b);
+    const int len = (int)length_of(a, b);
+    auto upto = [&](int64_t i) { return a.causal ? (int)min((int64_t)len, max((int64_t)0, start + i + 1)) : len; };   // keys that query i sees
+    const int sees = row_in ? upto(i) : 0;
+    // (rows of one head are in order; several heads in one tile: from the first query's keys to the last one's)
+    const bool packed = a.heads_per_row > 1;
+    const int most = upto(packed ? a.Nq - 1 : min(a.Nq - 1, (int64_t)(tile + 1) * 32 * NQ - 1));
+    const int fewest = upto(packed ? 0 : (int64_t)tile * 32 * NQ + qw * 32);    // that every row of the wave sees
+    const int j_begin = (int)((int64_t)split * a.split_keys), j_end = (int)min((int64_t)most, j_begin + a.split_keys);
 
     const T *kp = (const T *)a.k + (int64_t)b * a.kb + (int64_t)(2 * hk) * a.kh;
     const T *vp = (const T *)a.v + (int64_t)b * a.vb + (int64_t)hk * a.vh;
-    auto fetch = [&](char *to, int64_t j) __attribute__((always_inline)) {
-        const int in = (int)min((int64_t)KT, len - j);
-        stage_rows<KT, CK, NW>(to, kp + j * a.kn, (int)a.kn, in, a.D / 8, w, l);
-        stage_rows<KT, CK, NW>(to + K_BYTES, kp + a.kh + j * a.kn, (int)a.kn, in, a.D / 8, w, l);
-        stage_rows<KT, CV, NW>(to + 2 * K_BYTES, vp + j * a.vn, (int)a.vn, in, a.Dv / 8, w, l);
+    Stager<KT, CK, NW> stage_k;
+    Stager<KT, CV, NW> stage_v;
+    stage_k.begin(a.kn, a.D / 8, w, l);
+    stage_v.begin(a.vn, a.Dv / 8, w, l);
+    auto fetch = [&](char *to, int j) __attribute__((always_inline)) {
+        stage_k.copy(to, kp + j * a.kn, len - j, w);
+        stage_k.copy(to + K_BYTES, kp + a.kh + j * a.kn, len - j, w);
+        stage_v.copy(to + 2 * K_BYTES, vp + j * a.vn, len - j, w);
     };
     if (j_begin < j_end) fetch(smem, j_begin);
 
     // ---- queries: right operands, in registers
-    s16x8 qf[2][DT / 16];
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
+    s16x8 qf[DT / 16];
+    {
         const T *p = (const T *)a.q + (int64_t)b * a.qb + i * a.qn + (int64_t)(2 * head + m) * a.qh;
 #pragma unroll
         for (int s = 0; s < DT / 16; ++s) {
             const int c = 2 * s + h32;
-            qf[m][s] = load8(p + c * 8, row_in && c * 8 < a.D);
+            qf[s] = load8(p + c * 8, row_in && c * 8 < a.D);
         }
     }
     RowReader<CK> keys;
     ColumnReader<CV> values;
     keys.begin(l);
     values.begin(l);
+    keys.at += m * K_BYTES;
 
-    f32x16 acc[2][DV / 32];
-    clear(acc[0]);
-    clear(acc[1]);
-    float top[2] = {kLowest, kLowest}, total[2] = {0.f, 0.f};
+    f32x16 acc[DV / 32];
+    clear(acc);
+    float top = kLowest, total = 0.f;
     const float to_log2 = a.scale * kLog2e;
 
     // One tile; the next one is on its way to `ahead`.  (__restrict__: the compiler would have it arrive before the first read of `now`.)
-    auto turn = [&](char *__restrict__ ahead, const char *__restrict__ now, int64_t j) __attribute__((always_inline)) {
+    auto turn = [&](char *__restrict__ ahead, const char *__restrict__ now, int j) __attribute__((always_inline)) {
         tile_there<NW>();
         if (j + KT < j_end) fetch(ahead, j + KT);
 #pragma unroll
         for (int t = 0; t < KT / 32; ++t) {
-            const bool masked = j + 32 * t + 32 > fewest;
-            f32x16 s[2];
-            s16x8 pf[2][2];
+            f32x16 s[1];
             clear(s);
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
+            for (int d = 0; d < DT / 16; ++d) s[0] = mfma32<T>(keys.read(now, t, d), qf[d], s[0]);
+            if (j + 32 * t + 32 > fewest) {
+                const int n = sees - j - 32 * t;
 #pragma unroll
-                for (int d = 0; d < DT / 16; ++d) s[m] = mfma32<T>(keys.read(now + m * K_BYTES, t, d), qf[m][d], s[m]);
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                if (masked) {
-                    const int n = (int)min((int64_t)32, max((int64_t)0, sees - j - 32 * t));
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (tile_row(r, h32) >= n) s[m][r] = -INFINITY;
-                }
-                float high = s[m][0];
-#pragma unroll
-                for (int r = 1; r < 16; ++r) high = fmaxf(high, s[m][r]);
-                high = both_halves_max(high) * to_log2;
-                if (__any(high > top[m] + 8.0f)) {
-                    const float next = fmaxf(top[m], high), shrink = __builtin_amdgcn_exp2f(top[m] - next);
-                    top[m] = next;
-                    total[m] *= shrink;
-#pragma unroll
-                    for (int v = 0; v < DV / 32; ++v)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) acc[m][v][r] *= shrink;
-                }
-                float sum = 0.f;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s[m][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][r], to_log2, -top[m]));
-                    sum += s[m][r];
-                }
-                total[m] += sum;
-                pf[m][0] = as_operand<T>(s[m], 0);
-                pf[m][1] = as_operand<T>(s[m], 1);
+                for (int r = 0; r < 16; ++r)
+                    if (tile_row(r, h32) >= n) s[0][r] = -INFINITY;
             }
+            float high = s[0][0];
 #pragma unroll
-            for (int v = 0; v < DV / 32; ++v)
+            for (int r = 1; r < 16; ++r) high = fmaxf(high, s[0][r]);
+            high = both_halves_max(high) * to_log2;
+            if (__any(high > top + 8.0f)) {
+                const float next = fmaxf(top, high), shrink = __builtin_amdgcn_exp2f(top - next);
+                top = next;
+                total *= shrink;
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const s16x8 vf = values.read(now + 2 * K_BYTES, 32 * t + 16 * x, v);
-                    acc[0][v] = mfma32<T>(vf, pf[0][x], acc[0][v]);
-                    acc[1][v] = mfma32<T>(vf, pf[1][x], acc[1][v]);
-                }
+                for (int v = 0; v < DV / 32; ++v)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[v][r] *= shrink;
+            }
+            float sum = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[0][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], to_log2, -top));
+                sum += s[0][r];
+            }
+            total += sum;
+            const s16x8 pf[2] = {as_operand<T>(s[0], 0), as_operand<T>(s[0], 1)};
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int v = 0; v < DV / 32; ++v) acc[v] = mfma32<T>(values.read(now + 2 * K_BYTES, 32 * t + 16 * x, v), pf[x], acc[v]);
         }
     };
-    for (int64_t j = j_begin; j < j_end; j += 2 * KT) {
+    for (int j = j_begin; j < j_end; j += 2 * KT) {
         turn(smem + STAGE, smem, j);
         if (j + KT < j_end) turn(smem, smem + STAGE, j + KT);
     }
-    total[0] = both_halves_sum(total[0]);
-    total[1] = both_halves_sum(total[1]);
+    total = both_halves_sum(total);
 
     if (a.part) {                                           // unfinished sums of this part
         if (!row_in) return;
         float *to = a.part + ((((int64_t)b * a.H + head) * a.Nq + i) * a.splits + split) * (2 * a.Dv + 4);
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int t = 0; t < DV / 32; ++t)
 #pragma unroll
-            for (int t = 0; t < DV / 32; ++t)
-#pragma unroll
-                for (int r = 0; r < 16; r += 4) {
-                    const int d = 32 * t + tile_row(r, h32);
-                    const f32x4 v = {acc[m][t][r], acc[m][t][r + 1], acc[m][t][r + 2], acc[m][t][r + 3]};
-                    if (d < a.Dv) *reinterpret_cast<f32x4 *>(to + m * a.Dv + d) = v;
-                }
-        if (h32 == 0) *reinterpret_cast<f32x4 *>(to + 2 * a.Dv) = (f32x4){top[0], top[1], total[0], total[1]};
+            for (int r = 0; r < 16; r += 4) {
+                const int d = 32 * t + tile_row(r, h32);
+                const f32x4 v = {acc[t][r], acc[t][r + 1], acc[t][r + 2], acc[t][r + 3]};
+                if (d < a.Dv) *reinterpret_cast<f32x4 *>(to + m * a.Dv + d) = v;
+            }
+        if (h32 == 0) to[2 * a.Dv + m] = top, to[2 * a.Dv + 2 + m] = total;
         return;
     }
-    const float lam = lam_of<T>(a, head);
-    const float w1 = total[0] == 0.f ? 0.f : 1.0f / total[0], w2 = total[1] == 0.f ? 0.f : 1.0f / total[1];
-    const int64_t at = (((int64_t)b * a.Nq + i) * a.H + head) * a.Dv;
-    tile_there<NW>();                                       // (every wave is through with the tiles)
-    char *own = smem + w * 32 * DV * 2;
-    store_rows<T, DV>(own, (T *)a.o, at, row_in, a.Dv, l, [&](int t, int r) { return acc[0][t][r] * w1 - lam * (acc[1][t][r] * w2); });
-    if (a.o2) store_rows<T, DV>(own, (T *)a.o2, at, row_in, a.Dv, l, [&](int t, int r) { return acc[1][t][r] * w2; });
-    if (a.lse && row_in && h32 == 0)
+    const float weight = total == 0.f ? 0.f : 1.0f / total;
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
-            a.lse[((int64_t)b * 2 * a.H + 2 * head + m) * a.Nq + i] = total[m] == 0.f ? INFINITY : top[m] + __log2f(total[m]);
+    for (int t = 0; t < DV / 32; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[t][r] *= weight;
+    const int64_t at = (((int64_t)b * a.Nq + i) * a.H + head) * a.Dv;
+    const float lam = lam_of<T>(a, head);
+    // the first map's wave takes off the second's, two tiles at a time
+#pragma unroll
+    for (int t = 0; t < DV / 32; t += 2) {
+        tile_there<NW>();                                   // (every wave is through with what lies there)
+        f32x4 *by = reinterpret_cast<f32x4 *>(smem) + qw * 512 + l;
+        if (m)
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                const f32x16 &x = acc[t + r / 4];
+                const int e = r % 4 * 4;
+                by[r * 64] = (f32x4){x[e], x[e + 1], x[e + 2], x[e + 3]};
+            }
+        tile_there<NW>();
+        if (!m)
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                const f32x4 y = by[r * 64];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[t + r / 4][r % 4 * 4 + e] -= lam * y[e];
+            }
+    }
+    char *own = smem + qw * 32 * DV * 2;
+    tile_there<NW>();
+    if (!m) store_rows<T, DV>(own, (T *)a.o, at, row_in, a.Dv, l, [&](int t, int r) { return acc[t][r]; });
+    if (a.o2) {
+        tile_there<NW>();
+        if (m) store_rows<T, DV>(own, (T *)a.o2, at, row_in, a.Dv, l, [&](int t, int r) { return acc[t][r]; });
+    }
+    if (a.lse && row_in && h32 == 0)
+        a.lse[((int64_t)b * 2 * a.H + 2 * head + m) * a.Nq + i] = total == 0.f ? INFINITY : top + __log2f(total);
 }
 
 // Joins the parts of a row: a workgroup a row, a thread a value of one map.  The parts' weights first, in LDS.
@@ -370,7 +394,7 @@ template <typename T> __global__ __launch_bounds__(512) void attention_join_kern
 // ---------------------------------------------------------------------------------------------- gradients of the queries
 // As the forward pass: a lane holds one query, dS^T is at once the right operand of  dq^T += k^T dS^T.  Also D1, D2 for the next kernel.
 template <typename T, int DT, int KT>
-__global__ __launch_bounds__(THREADS, DT == 128 ? 1 : 2) void attention_dq_kernel(Args a) {
+__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 128 ? 1 : 2, DT == 128 ? 1 : 2))) void attention_dq_kernel(Args a) {
     constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT, NW = 4;
     constexpr int K_BYTES = KT * CK * 16, V_BYTES = KT * CV * 16, STAGE = 2 * K_BYTES + V_BYTES;
     __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
@@ -385,14 +409,10 @@ __global__ __launch_bounds__(THREADS, DT == 128 ? 1 : 2) void attention_dq_kerne
     const int64_t row = (int64_t)tile * 128 + w * 32 + (l & 31);
     const bool row_in = row < a.Nq;
     const int64_t i = row_in ? row : 0;
-    const int64_t start = start_of(a, b), len = length_of(a, b);
-    const int64_t sees = !row_in ? 0 : a.causal ? min(len, max((int64_t)0, start + i + 1)) : len;
-    int64_t j_end = len, fewest = len;
-    if (a.causal) {
-        j_end = min(len, max((int64_t)0, start + min(a.Nq, (int64_t)(tile + 1) * 128)));
-        fewest = min(len, max((int64_t)0, start + (int64_t)tile * 128 + w * 32 + 1));
-    }
-
+    const int64_t start = start_of(a, b);
+    const int len = (int)length_of(a, b);
+    auto upto = [&](int64_t i) { return a.causal ? (int)min((int64_t)len, max((int64_t)0, start + i + 1)) : len; };
+    const int sees = row_in ? upto(i) : 0, j_end = upto(min(a.Nq - 1, (int64_t)tile * 128 + 127)), fewest = upto((int64_t)tile * 128 + w * 32);
     const bool single = __any(sees == 1);
     s16x8 qf[2][DT / 16], gf[DV / 16];
 #pragma unroll
@@ -442,11 +462,14 @@ __global__ __launch_bounds__(THREADS, DT == 128 ? 1 : 2) void attention_dq_kerne
     const float to_log2 = a.scale * kLog2e;
     const T *kp = (const T *)a.k + (int64_t)b * a.kb + (int64_t)(2 * hk) * a.kh;
     const T *vp = (const T *)a.v + (int64_t)b * a.vb + (int64_t)hk * a.vh;
-    auto fetch = [&](char *to, int64_t j) __attribute__((always_inline)) {
-        const int in = (int)min((int64_t)KT, len - j);
-        stage_rows<KT, CK, NW>(to, kp + j * a.kn, (int)a.kn, in, a.D / 8, w, l);
-        stage_rows<KT, CK, NW>(to + K_BYTES, kp + a.kh + j * a.kn, (int)a.kn, in, a.D / 8, w, l);
-        stage_rows<KT, CV, NW>(to + 2 * K_BYTES, vp + j * a.vn, (int)a.vn, in, a.Dv / 8, w, l);
+    Stager<KT, CK, NW> stage_k;
+    Stager<KT, CV, NW> stage_v;
+    stage_k.begin(a.kn, a.D / 8, w, l);
+    stage_v.begin(a.vn, a.Dv / 8, w, l);
+    auto fetch = [&](char *to, int j) __attribute__((always_inline)) {
+        stage_k.copy(to, kp + j * a.kn, len - j, w);
+        stage_k.copy(to + K_BYTES, kp + a.kh + j * a.kn, len - j, w);
+        stage_v.copy(to + 2 * K_BYTES, vp + j * a.vn, len - j, w);
     };
     RowReader<CK> keys;
     RowReader<CV> values;
@@ -455,28 +478,27 @@ __global__ __launch_bounds__(THREADS, DT == 128 ? 1 : 2) void attention_dq_kerne
     values.begin(l);
     key_columns.begin(l);
     if (0 < j_end) fetch(smem, 0);
-    auto turn = [&](char *__restrict__ ahead, const char *__restrict__ now, int64_t j) __attribute__((always_inline)) {
+    auto turn = [&](char *__restrict__ ahead, const char *__restrict__ now, int j) __attribute__((always_inline)) {
         tile_there<NW>();
         if (j + KT < j_end) fetch(ahead, j + KT);
 #pragma unroll
         for (int t = 0; t < KT / 32; ++t) {
             const bool masked = j + 32 * t + 32 > fewest || single;
-            f32x16 dp[1], s[2];
+            f32x16 dp[1];
             clear(dp);
-            clear(s);
 #pragma unroll
             for (int d = 0; d < DV / 16; ++d) dp[0] = mfma32<T>(values.read(now + 2 * K_BYTES, t, d), gf[d], dp[0]);
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
+            for (int m = 0; m < 2; ++m) {
+                f32x16 s[2];
+                clear(s);
 #pragma unroll
                 for (int d = 0; d < DT / 16; ++d) s[m] = mfma32<T>(keys.read(now + m * K_BYTES, t, d), qf[m][d], s[m]);
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                     s[m][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][r], to_log2, -lse[m])) * (dp[0][r] - delta[m]);
                 if (masked) {                               // (a row that sees one key has weight 1 there whatever its score)
-                    const int n = sees == 1 ? 0 : (int)min((int64_t)32, max((int64_t)0, sees - j - 32 * t));
+                    const int n = sees == 1 ? 0 : sees - j - 32 * t;
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
                         if (tile_row(r, h32) >= n) s[m][r] = 0.f;
@@ -490,7 +512,7 @@ __global__ __launch_bounds__(THREADS, DT == 128 ? 1 : 2) void attention_dq_kerne
             }
         }
     };
-    for (int64_t j = 0; j < j_end; j += 2 * KT) {
+    for (int j = 0; j < j_end; j += 2 * KT) {
         turn(smem + STAGE, smem, j);
         if (j + KT < j_end) turn(smem, smem + STAGE, j + KT);
     }
@@ -525,8 +547,8 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
     const int b = id % a.B, tile = id / a.B;
     if (tile >= tiles) return;
     const int per = a.H / a.Hk;
-    const int64_t start = start_of(a, b), len = length_of(a, b);
-    const int64_t first_key = (int64_t)tile * 64, key0 = first_key + kw * 32, key = key0 + (l & 31);
+    const int64_t start = start_of(a, b);
+    const int len = (int)length_of(a, b), first_key = tile * 64, key0 = first_key + kw * 32, key = key0 + (l & 31);
     const bool key_in = key < len;
 
     // queries that see any key of this workgroup
@@ -538,13 +560,16 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
     int64_t i_next = i_first;
     int steps = per_head * per;
 
+    Stager<QT, CK, NW> stage_q;
+    Stager<QT, CV, NW> stage_g;
+    stage_q.begin(a.qn, a.D / 8, w, l);
+    stage_g.begin(a.don, a.Dv / 8, w, l);
     auto fetch = [&](char *to) __attribute__((always_inline)) {
         const int head = hk * per + g_next, in = (int)min((int64_t)QT, a.Nq - i_next);
         const T *qp = (const T *)a.q + (int64_t)b * a.qb + i_next * a.qn + (int64_t)(2 * head) * a.qh;
-        stage_rows<QT, CK, NW>(to, qp, (int)a.qn, in, a.D / 8, w, l);
-        stage_rows<QT, CK, NW>(to + Q_BYTES, qp + a.qh, (int)a.qn, in, a.D / 8, w, l);
-        stage_rows<QT, CV, NW>(to + 2 * Q_BYTES, (const T *)a.dout + (int64_t)b * a.dob + i_next * a.don + (int64_t)head * a.doh, (int)a.don, in,
-                               a.Dv / 8, w, l);
+        stage_q.copy(to, qp, in, w);
+        stage_q.copy(to + Q_BYTES, qp + a.qh, in, w);
+        stage_g.copy(to + 2 * Q_BYTES, (const T *)a.dout + (int64_t)b * a.dob + i_next * a.don + (int64_t)head * a.doh, in, w);
         // one of lse1, lse2, D1, D2 a wave.  (Queries past the end have zeros everywhere: their weight of 1 meets do = 0.)
         const float *from = (w < 2 ? a.lse : a.delta) + ((int64_t)b * 2 * a.H + 2 * head + (w & 1)) * a.Nq + i_next;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(uniform_rsrc(from, kAnywhere), (lds_ptr_t)(to + 2 * Q_BYTES + G_BYTES + w * QT * 4), 4,
@@ -557,7 +582,7 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
     s16x8 kf[2][DT / 16], vf[KEYS ? DV / 16 : 1];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-        const T *p = (const T *)a.k + (int64_t)b * a.kb + (key_in ? key : 0) * a.kn + (int64_t)(2 * hk + m) * a.kh;
+        const T *p = (const T *)a.k + (int64_t)b * a.kb + (int64_t)(key_in ? key : 0) * a.kn + (int64_t)(2 * hk + m) * a.kh;
 #pragma unroll
         for (int s = 0; s < DT / 16; ++s) {
             const int c = 2 * s + h32;
@@ -565,7 +590,7 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
         }
     }
     if constexpr (KEYS) {
-        const T *p = (const T *)a.v + (int64_t)b * a.vb + (key_in ? key : 0) * a.vn + (int64_t)hk * a.vh;
+        const T *p = (const T *)a.v + (int64_t)b * a.vb + (int64_t)(key_in ? key : 0) * a.vn + (int64_t)hk * a.vh;
 #pragma unroll
         for (int s = 0; s < DV / 16; ++s) {
             const int c = 2 * s + h32;
@@ -594,9 +619,10 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
         const float lam = lam_of<T>(a, hk * per + g);
         const char *gs = now + 2 * Q_BYTES;
         const float *stats = reinterpret_cast<const float *>(gs + G_BYTES) + 32 * qw + 4 * h32;
-        const int64_t it = i0 + 32 * qw;
+        // the last key that the first of these queries sees (clamped: only its place among the keys counts)
+        const int last0 = a.causal ? (int)max((int64_t)-64, min((int64_t)1 << 30, start + i0 + 32 * qw)) : 1 << 30;
         // some pair is hidden, or some row sees one key only
-        const bool masked = key0 + 32 > len || (a.causal && key0 + 31 > start + it) || len == 1 || (a.causal && start + it <= 0);
+        const bool masked = key0 + 32 > len || key0 + 31 > last0 || len == 1 || last0 <= 0;
         f32x16 dp[1], s[2];
         clear(dp);
         clear(s);
@@ -620,9 +646,9 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
                     float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][r + e], to_log2, -ls[e]));
                     float ds = p * (dp[0][r + e] - de[e]);
                     if (masked) {
-                        const int64_t last = start + it + tile_row(r + e, h32);         // the last key that this query sees
-                        if (key >= len || (a.causal && key > last)) p = ds = 0.f;
-                        if (len == 1 || (a.causal && last == 0)) ds = 0.f;
+                        const int last = last0 + tile_row(r + e, h32);
+                        if (key >= len || key > last) p = ds = 0.f;
+                        if (len == 1 || last == 0) ds = 0.f;
                     }
                     if (m == 0) wt[r + e] = p;
                     else {
@@ -746,8 +772,8 @@ Plan plan_of(const bndm_attention_shape &s) {
 
 template <typename T, int DT> int forward(const Args &a, const Plan &p, hipStream_t stream) {
     constexpr int KT = DT == 128 ? 32 : 64;
-    if (p.waves == 1) hipLaunchKernelGGL((attention_kernel<T, DT, 1, 32>), dim3((unsigned)p.blocks), dim3(64), 0, stream, a);
-    else hipLaunchKernelGGL((attention_kernel<T, DT, 4, KT>), dim3((unsigned)p.blocks), dim3(256), 0, stream, a);
+    if (p.waves == 1) hipLaunchKernelGGL((attention_kernel<T, DT, 1, 32>), dim3((unsigned)p.blocks), dim3(128), 0, stream, a);
+    else hipLaunchKernelGGL((attention_kernel<T, DT, 4, KT>), dim3((unsigned)p.blocks), dim3(512), 0, stream, a);
     if (int rc = tokens_launch_status("attention")) return rc;
     if (a.part) {
         hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)((int64_t)a.B * a.H * a.Nq)), dim3(512), 0, stream, a);
