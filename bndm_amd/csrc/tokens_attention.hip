@@ -14,6 +14,7 @@
 // of 16-bit operands are what those take.
 #include "tokens_common.hpp"
 #include <cmath>
+#include <type_traits>
 
 namespace bndm {
 namespace {
@@ -94,6 +95,13 @@ template <int C> struct ColumnReader {                 // operand whose rows are
     }
 };
 
+// Workgroups go to the 8 XCDs in turn: what this gives out in their place are runs for each, so that workgroups that read the same keys (or
+// queries) run behind one L2.  1024 workgroups over 32 heads of 2 MB each: 447 us in the order of launch, TODO this way.
+__device__ __forceinline__ int of_this_xcd(int id, int n) {
+    const int per = n / 8, more = n % 8, x = id & 7;
+    return x * per + min(x, more) + (id >> 3);
+}
+
 // registers 8 s .. 8 s + 7 of a result tile as an operand whose k are rows 16 s .. 16 s + 15 in that order
 template <typename T> __device__ __forceinline__ s16x8 as_operand(const f32x16 &p, int s) {
     return pack8<T>(p[8 * s], p[8 * s + 1], p[8 * s + 2], p[8 * s + 3], p[8 * s + 4], p[8 * s + 5], p[8 * s + 6], p[8 * s + 7]);
@@ -170,19 +178,23 @@ __device__ __forceinline__ int64_t length_of(const Args &a, int b) {
 // heads of 64 spilled at two waves a SIMD: 570 us where this takes TODO).  KT keys a tile, 32 of them at a time.  DT: head size rounded up
 // to 32, 64, 128; values are up to 2 DT wide.  The running maximum is followed loosely: sums are scaled down only when it has grown by a
 // factor of 2^8 (weights stay below 2^8 until then, and the final division takes care of them).
-template <typename T, int DT, int NQ, int KT>
-__global__ __launch_bounds__(128 * NQ, DT == 32 ? 3 : 2) void attention_kernel(Args a) {
-    constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT, NW = 2 * NQ;
+//
+// AHEAD: the products of a step are interleaved with the exponentials of another, as the matrix and the vector units of a SIMD work side by
+// side only on different instructions of a wave (or of two waves that are not in step, and a barrier a tile keeps them in step): while the
+// weights of step t are formed, the scores of t + 1 and the values' sums of t - 1 are.  Without it the two add up, TODO us against TODO.
+template <typename T, int DT, int NQ, int KT, bool AHEAD>
+__global__ __launch_bounds__(128 * NQ) __attribute__((amdgpu_waves_per_eu(2, DT == 32 || NQ == 1 ? 4 : 2))) void attention_kernel(Args a) {
+    constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT, NW = 2 * NQ, BUFFERS = AHEAD ? 3 : 2;
     constexpr int K_BYTES = KT * CK * 16, V_BYTES = KT * CV * 16, STAGE = 2 * K_BYTES + V_BYTES;
-    static_assert(NQ * 32 * DV * 2 <= 2 * STAGE && NQ * 8192 <= 2 * STAGE, "results go through the same memory");
-    __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
+    static_assert(NQ * 32 * DV * 2 <= BUFFERS * STAGE && NQ * 8192 <= BUFFERS * STAGE, "results go through the same memory");
+    extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, l = tid & 63, h32 = l >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6), m = w & 1, qw = w >> 1;
 
     // ---- which rows: (batch, group of query heads, tile of rows, part of the keys)
     const int64_t rows = a.Nq * a.heads_per_row;
     const int tiles = (int)((rows + 32 * NQ - 1) / (32 * NQ));
-    int id = blockIdx.x;
+    int id = of_this_xcd(blockIdx.x, gridDim.x);
     const int split = id % a.splits; id /= a.splits;
     const int tile = id % tiles; id /= tiles;
     const int groups = a.H / a.heads_per_row;
@@ -216,6 +228,7 @@ __global__ __launch_bounds__(128 * NQ, DT == 32 ? 3 : 2) void attention_kernel(A
         stage_v.copy(to + 2 * K_BYTES, vp + j * a.vn, len - j, w);
     };
     if (j_begin < j_end) fetch(smem, j_begin);
+    if (AHEAD && j_begin + KT < j_end) fetch(smem + STAGE, j_begin + KT);
 
     // ---- queries: right operands, in registers
     s16x8 qf[DT / 16];
@@ -238,52 +251,136 @@ __global__ __launch_bounds__(128 * NQ, DT == 32 ? 3 : 2) void attention_kernel(A
     float top = kLowest, total = 0.f;
     const float to_log2 = a.scale * kLog2e;
 
-    // One tile; the next one is on its way to `ahead`.  (__restrict__: the compiler would have it arrive before the first read of `now`.)
-    auto turn = [&](char *__restrict__ ahead, const char *__restrict__ now, int j) __attribute__((always_inline)) {
-        tile_there<NW>();
-        if (j + KT < j_end) fetch(ahead, j + KT);
+    auto hide = [&](f32x16 &s, int j) __attribute__((always_inline)) {      // keys from j on, those that the row does not see
+        const int n = sees - j;
 #pragma unroll
-        for (int t = 0; t < KT / 32; ++t) {
-            f32x16 s[1];
-            clear(s);
+        for (int r = 0; r < 16; ++r)
+            if (tile_row(r, h32) >= n) s[r] = -INFINITY;
+    };
+    // The maximum, as a whole power of two, so that what is scaled down with it stays exact.  `held`: weights that are yet to meet their values.
+    auto follow = [&](const f32x16 &s, s16x8 (&held)[2]) __attribute__((always_inline)) {
+        float high = s[0];
 #pragma unroll
-            for (int d = 0; d < DT / 16; ++d) s[0] = mfma32<T>(keys.read(now, t, d), qf[d], s[0]);
-            if (j + 32 * t + 32 > fewest) {
-                const int n = sees - j - 32 * t;
+        for (int r = 1; r < 16; ++r) high = fmaxf(high, s[r]);
+        high = both_halves_max(high) * to_log2;
+        if (__any(high > top + 8.0f)) {
+            const float up = fmaxf(top, ceilf(high)), shrink = __builtin_amdgcn_exp2f(top - up);
+            top = up;
+            total *= shrink;
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (tile_row(r, h32) >= n) s[0][r] = -INFINITY;
-            }
-            float high = s[0][0];
+            for (int v = 0; v < DV / 32; ++v)
 #pragma unroll
-            for (int r = 1; r < 16; ++r) high = fmaxf(high, s[0][r]);
-            high = both_halves_max(high) * to_log2;
-            if (__any(high > top + 8.0f)) {
-                const float next = fmaxf(top, high), shrink = __builtin_amdgcn_exp2f(top - next);
-                top = next;
-                total *= shrink;
+                for (int r = 0; r < 16; ++r) acc[v][r] *= shrink;
+            if constexpr (AHEAD)
 #pragma unroll
-                for (int v = 0; v < DV / 32; ++v)
+                for (int x = 0; x < 2; ++x)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) acc[v][r] *= shrink;
-            }
-            float sum = 0.f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[0][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], to_log2, -top));
-                sum += s[0][r];
-            }
-            total += sum;
-            const s16x8 pf[2] = {as_operand<T>(s[0], 0), as_operand<T>(s[0], 1)};
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int v = 0; v < DV / 32; ++v) acc[v] = mfma32<T>(values.read(now + 2 * K_BYTES, 32 * t + 16 * x, v), pf[x], acc[v]);
+                    for (int e = 0; e < 8; ++e) {
+                        const short h = held[x][e];
+                        held[x][e] = __builtin_bit_cast(short, (T)(widen<T>(h) * shrink));
+                    }
         }
     };
-    for (int j = j_begin; j < j_end; j += 2 * KT) {
-        turn(smem + STAGE, smem, j);
-        if (j + KT < j_end) turn(smem, smem + STAGE, j + KT);
+    auto weigh = [&](f32x16 &s, s16x8 (&pf)[2]) __attribute__((always_inline)) {
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], to_log2, -top));
+            sum += s[r];
+        }
+        total += sum;
+        pf[0] = as_operand<T>(s, 0);
+        pf[1] = as_operand<T>(s, 1);
+    };
+    // (__restrict__ below: the compiler would have the copies to `ahead` arrive before the first read of the other tiles)
+    if constexpr (!AHEAD) {
+        auto turn = [&](char *__restrict__ ahead, const char *__restrict__ now, int j) __attribute__((always_inline)) {
+            tile_there<NW>();
+            if (j + KT < j_end) fetch(ahead, j + KT);
+#pragma unroll
+            for (int t = 0; t < KT / 32; ++t) {
+                f32x16 s[1];
+                s16x8 pf[2];
+                clear(s);
+#pragma unroll
+                for (int d = 0; d < DT / 16; ++d) s[0] = mfma32<T>(keys.read(now, t, d), qf[d], s[0]);
+                if (j + 32 * t + 32 > fewest) hide(s[0], j + 32 * t);
+                follow(s[0], pf);
+                weigh(s[0], pf);
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int v = 0; v < DV / 32; ++v) acc[v] = mfma32<T>(values.read(now + 2 * K_BYTES, 32 * t + 16 * x, v), pf[x], acc[v]);
+            }
+        };
+        for (int j = j_begin; j < j_end; j += 2 * KT) {
+            turn(smem + STAGE, smem, j);
+            if (j + KT < j_end) turn(smem, smem + STAGE, j + KT);
+        }
+    } else if (j_begin < j_end) {
+        static_assert(!AHEAD || KT == 64, "two steps a tile");
+        f32x16 s[2];
+        s16x8 kf[DT / 16], vf[2][DV / 32], pf[2];           // keys of t + 1, values and weights of t - 1
+        auto scores = [&](f32x16 &s) __attribute__((always_inline)) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+            for (int d = 0; d < DT / 16; ++d) s = mfma32<T>(kf[d], qf[d], s);
+        };
+        const s16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+        // the tile's two steps; its scores are there (the first's) or its keys are (the second's); `next` has the tile after it
+        auto turn = [&](char *__restrict__ ahead, const char *__restrict__ now, const char *__restrict__ next, int j, auto masked) __attribute__((always_inline)) {
+            tile_there<NW>();                               // the next tile is there, the one before this has been read
+            if (j + 2 * KT < j_end) fetch(ahead, j + 2 * KT);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if (decltype(masked)::value) hide(s[t], j + 32 * t);
+                follow(s[t], pf);
+                s16x8 weights[2];
+                scores(s[t ^ 1]);
+#pragma unroll
+                for (int d = 0; d < DT / 16; ++d) kf[d] = keys.read(next, t, d);
+                weigh(s[t], weights);
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int v = 0; v < DV / 32; ++v) {
+                        acc[v] = mfma32<T>(vf[x][v], pf[x], acc[v]);
+                        vf[x][v] = values.read(now + 2 * K_BYTES, 32 * t + 16 * x, v);
+                    }
+                pf[0] = weights[0], pf[1] = weights[1];
+#pragma unroll
+                for (int n = 0; n < DT / 16 + DV / 16; ++n) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);     // one product,
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);     // two reads of LDS,
+                    __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);     // six vector instructions, and so on
+                }
+            }
+        };
+        tile_there<NW>();
+#pragma unroll
+        for (int d = 0; d < DT / 16; ++d) kf[d] = keys.read(smem, 0, d);
+        scores(s[0]);
+#pragma unroll
+        for (int d = 0; d < DT / 16; ++d) kf[d] = keys.read(smem, 1, d);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            pf[x] = zero;
+#pragma unroll
+            for (int v = 0; v < DV / 32; ++v) vf[x][v] = zero;
+        }
+        int j = j_begin, slot = 0;
+        auto around = [&](auto masked) __attribute__((always_inline)) {
+            const int after = slot == 2 ? 0 : slot + 1, last = slot == 0 ? 2 : slot - 1;
+            turn(smem + last * STAGE, smem + slot * STAGE, smem + after * STAGE, j, masked);
+            slot = after;
+        };
+        for (; j + KT <= min(fewest, j_end); j += KT) around(std::false_type());
+        for (; j < j_end; j += KT) around(std::true_type());
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int v = 0; v < DV / 32; ++v) acc[v] = mfma32<T>(vf[x][v], pf[x], acc[v]);
     }
     total = both_halves_sum(total);
 
@@ -402,7 +499,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
     const int tid = threadIdx.x, l = tid & 63, h32 = l >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int tiles = (int)((a.Nq + 127) / 128);
-    int id = blockIdx.x;
+    int id = of_this_xcd(blockIdx.x, gridDim.x);
     const int tile = id % tiles; id /= tiles;
     const int head = id % a.H, b = id / a.H;
     const int hk = head / (a.H / a.Hk);
@@ -770,10 +867,25 @@ Plan plan_of(const bndm_attention_shape &s) {
     return p;
 }
 
+template <typename F> int allow_lds(F kernel, int bytes, const char *what) {
+    if (bytes <= 65536) return 0;
+    const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) return 0;
+    (void)hipGetLastError();
+    tokens_error("%s: %d bytes of LDS: %s", what, bytes, hipGetErrorString(e));
+    return (int)e;
+}
+
+template <typename T, int DT, int NQ, int KT, bool AHEAD> int launch_attention(const Args &a, int64_t blocks, hipStream_t stream) {
+    constexpr int LDS = (AHEAD ? 3 : 2) * KT * DT * 8;
+    if (int rc = allow_lds(attention_kernel<T, DT, NQ, KT, AHEAD>, LDS, "attention")) return rc;
+    hipLaunchKernelGGL((attention_kernel<T, DT, NQ, KT, AHEAD>), dim3((unsigned)blocks), dim3(128 * NQ), LDS, stream, a);
+    return 0;
+}
+
 template <typename T, int DT> int forward(const Args &a, const Plan &p, hipStream_t stream) {
     constexpr int KT = DT == 128 ? 32 : 64;
-    if (p.waves == 1) hipLaunchKernelGGL((attention_kernel<T, DT, 1, 32>), dim3((unsigned)p.blocks), dim3(128), 0, stream, a);
-    else hipLaunchKernelGGL((attention_kernel<T, DT, 4, KT>), dim3((unsigned)p.blocks), dim3(512), 0, stream, a);
+    if (int rc = p.waves == 1 ? launch_attention<T, DT, 1, 32, false>(a, p.blocks, stream) : launch_attention<T, DT, 4, KT, DT != 128>(a, p.blocks, stream)) return rc;
     if (int rc = tokens_launch_status("attention")) return rc;
     if (a.part) {
         hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)((int64_t)a.B * a.H * a.Nq)), dim3(512), 0, stream, a);
@@ -784,13 +896,7 @@ template <typename T, int DT> int forward(const Args &a, const Plan &p, hipStrea
 
 template <typename T, int DT, int WHAT> int launch_dkv(const Args &a, hipStream_t stream) {
     constexpr int LDS = 2 * (64 * DT * 8 + 4 * 64 * 4);
-    const void *kernel = (const void *)attention_dkv_kernel<T, DT, WHAT>;
-    const hipError_t e = LDS > 65536 ? hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) : hipSuccess;
-    if (e != hipSuccess) {
-        (void)hipGetLastError();
-        tokens_error("attention dkv: %d bytes of LDS: %s", LDS, hipGetErrorString(e));
-        return (int)e;
-    }
+    if (int rc = allow_lds(attention_dkv_kernel<T, DT, WHAT>, LDS, "attention dkv")) return rc;
     hipLaunchKernelGGL((attention_dkv_kernel<T, DT, WHAT>), dim3((unsigned)(ceil_div64(a.Nk, 64) * a.Hk * a.B)), dim3(THREADS), LDS, stream, a);
     return tokens_launch_status("attention dkv");
 }
