@@ -184,7 +184,7 @@ __device__ __forceinline__ int64_t length_of(const Args &a, int b) {
 // weights of step t are formed, the scores of t + 1 and the values' sums of t - 1 are.  Without it the two add up, TODO us against TODO.
 template <typename T, int DT, int NQ, int KT, bool AHEAD>
 __global__ __launch_bounds__(128 * NQ) __attribute__((amdgpu_waves_per_eu(2, DT == 32 || NQ == 1 ? 4 : 2))) void attention_kernel(Args a) {
-    constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT, NW = 2 * NQ, BUFFERS = AHEAD ? 3 : 2;
+    constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT, NW = 2 * NQ, BUFFERS = AHEAD ? 4 : 2;
     constexpr int K_BYTES = KT * CK * 16, V_BYTES = KT * CV * 16, STAGE = 2 * K_BYTES + V_BYTES;
     static_assert(NQ * 32 * DV * 2 <= BUFFERS * STAGE && NQ * 8192 <= BUFFERS * STAGE, "results go through the same memory");
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -222,13 +222,25 @@ __global__ __launch_bounds__(128 * NQ) __attribute__((amdgpu_waves_per_eu(2, DT 
     Stager<KT, CV, NW> stage_v;
     stage_k.begin(a.kn, a.D / 8, w, l);
     stage_v.begin(a.vn, a.Dv / 8, w, l);
-    auto fetch = [&](char *to, int j) __attribute__((always_inline)) {
-        stage_k.copy(to, kp + j * a.kn, len - j, w);
-        stage_k.copy(to + K_BYTES, kp + a.kh + j * a.kn, len - j, w);
-        stage_v.copy(to + 2 * K_BYTES, vp + j * a.vn, len - j, w);
+    // the tile that is copied next, a third at a time
+    int j_next = j_begin;
+    const T *k_next = kp + j_begin * a.kn, *v_next = vp + j_begin * a.vn;
+    const int64_t k_step = KT * a.kn, v_step = KT * a.vn;
+    auto fetch = [&](char *to, int what) __attribute__((always_inline)) {
+        if (what == 0) stage_k.copy(to, k_next, len - j_next, w);
+        else if (what == 1) stage_k.copy(to + K_BYTES, k_next + a.kh, len - j_next, w);
+        else {
+            stage_v.copy(to + 2 * K_BYTES, v_next, len - j_next, w);
+            k_next += k_step;
+            v_next += v_step;
+            j_next += KT;
+        }
     };
-    if (j_begin < j_end) fetch(smem, j_begin);
-    if (AHEAD && j_begin + KT < j_end) fetch(smem + STAGE, j_begin + KT);
+    if (j_begin < j_end)
+#pragma unroll
+        for (int n = 0; n < (AHEAD ? 2 : 1); ++n)
+#pragma unroll
+            for (int what = 0; what < 3; ++what) fetch(smem + n * STAGE, what);
 
     // ---- queries: right operands, in registers
     s16x8 qf[DT / 16];
@@ -257,11 +269,15 @@ __global__ __launch_bounds__(128 * NQ) __attribute__((amdgpu_waves_per_eu(2, DT 
         for (int r = 0; r < 16; ++r)
             if (tile_row(r, h32) >= n) s[r] = -INFINITY;
     };
-    // The maximum, as a whole power of two, so that what is scaled down with it stays exact.  `held`: weights that are yet to meet their values.
-    auto follow = [&](const f32x16 &s, s16x8 (&held)[2]) __attribute__((always_inline)) {
+    auto highest = [&](const f32x16 &s) __attribute__((always_inline)) {
         float high = s[0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) high = fmaxf(high, s[r]);
+        return high;
+    };
+    // `high`: a lane's highest score.  The maximum is kept as a whole power of two, so that what is scaled down with it stays exact.  `held`:
+    // weights that are yet to meet their values.
+    auto follow = [&](float high, s16x8 (&held)[2]) __attribute__((always_inline)) {
         high = both_halves_max(high) * to_log2;
         if (__any(high > top + 8.0f)) {
             const float up = fmaxf(top, ceilf(high)), shrink = __builtin_amdgcn_exp2f(top - up);
@@ -296,7 +312,9 @@ __global__ __launch_bounds__(128 * NQ) __attribute__((amdgpu_waves_per_eu(2, DT 
     if constexpr (!AHEAD) {
         auto turn = [&](char *__restrict__ ahead, const char *__restrict__ now, int j) __attribute__((always_inline)) {
             tile_there<NW>();
-            if (j + KT < j_end) fetch(ahead, j + KT);
+            if (j + KT < j_end)
+#pragma unroll
+                for (int what = 0; what < 3; ++what) fetch(ahead, what);
 #pragma unroll
             for (int t = 0; t < KT / 32; ++t) {
                 f32x16 s[1];
@@ -305,7 +323,7 @@ __global__ __launch_bounds__(128 * NQ) __attribute__((amdgpu_waves_per_eu(2, DT 
 #pragma unroll
                 for (int d = 0; d < DT / 16; ++d) s[0] = mfma32<T>(keys.read(now, t, d), qf[d], s[0]);
                 if (j + 32 * t + 32 > fewest) hide(s[0], j + 32 * t);
-                follow(s[0], pf);
+                follow(highest(s[0]), pf);
                 weigh(s[0], pf);
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
@@ -328,41 +346,69 @@ __global__ __launch_bounds__(128 * NQ) __attribute__((amdgpu_waves_per_eu(2, DT 
             for (int d = 0; d < DT / 16; ++d) s = mfma32<T>(kf[d], qf[d], s);
         };
         const s16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
-        // the tile's two steps; its scores are there (the first's) or its keys are (the second's); `next` has the tile after it
+        float high;
+        constexpr int S = DT / 16, V = DV / 32, G = S + 2 * V, E = 16 * 3 / (2 * G);   // products of a step; exponentials that go with one of the first 16 / E
+        // The tile's two steps; its scores are there (the first's) or its keys are (the second's); `next` has the tile after it.  Each product
+        // goes with a share of the vector work, and the compiler is kept from regrouping them.
         auto turn = [&](char *__restrict__ ahead, const char *__restrict__ now, const char *__restrict__ next, int j, auto masked) __attribute__((always_inline)) {
-            tile_there<NW>();                               // the next tile is there, the one before this has been read
-            if (j + 2 * KT < j_end) fetch(ahead, j + 2 * KT);
+            // The next tile is there.  What `ahead` held was last read a whole tile ago, so that no wave waits for its reads here.
+            // (Tiles past the end are copied too, as far as the sequence goes, and never used.)
+            asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                if (decltype(masked)::value) hide(s[t], j + 32 * t);
-                follow(s[t], pf);
-                s16x8 weights[2];
-                scores(s[t ^ 1]);
+                follow(high, pf);
+                uint32_t weights[8];
+                float sum[2] = {0.f, 0.f};
+                f32x16 &cur = s[t], &nxt = s[t ^ 1];
 #pragma unroll
-                for (int d = 0; d < DT / 16; ++d) kf[d] = keys.read(next, t, d);
-                weigh(s[t], weights);
+                for (int r = 0; r < 16; ++r) nxt[r] = 0.f;
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                    for (int v = 0; v < DV / 32; ++v) {
+                for (int g = 0; g < G; ++g) {
+                    if (g < S) {
+                        nxt = mfma32<T>(kf[g], qf[g], nxt);
+                        kf[g] = keys.read(next, t, g);
+                    } else {
+                        const int x = (g - S) / V, v = (g - S) % V;
                         acc[v] = mfma32<T>(vf[x][v], pf[x], acc[v]);
                         vf[x][v] = values.read(now + 2 * K_BYTES, 32 * t + 16 * x, v);
                     }
-                pf[0] = weights[0], pf[1] = weights[1];
+                    if (t == 0 && g < 3) fetch(ahead, g);
+                    if (g * E < 16) {
 #pragma unroll
-                for (int n = 0; n < DT / 16 + DV / 16; ++n) {
-                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);     // one product,
-                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);     // two reads of LDS,
-                    __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);     // six vector instructions, and so on
+                        for (int e = 0; e < E; ++e) {
+                            cur[g * E + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[g * E + e], to_log2, -top));
+                            sum[e & 1] += cur[g * E + e];
+                        }
+#pragma unroll
+                        for (int e = 0; e < E; e += 2) weights[(g * E + e) / 2] = pack2<T>(cur[g * E + e], cur[g * E + e + 1]);
+                    } else {
+                        constexpr int M = 16 / (G - 16 / E);
+                        const int r0 = (g - 16 / E) * M;
+                        if (r0 == 0) {
+                            if (decltype(masked)::value) hide(nxt, j + 32 * t + 32);
+                            high = nxt[0];
+                        }
+#pragma unroll
+                        for (int r = r0; r < r0 + M; ++r) high = fmaxf(high, nxt[r]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+                total += sum[0] + sum[1];
+                pf[0] = __builtin_bit_cast(s16x8, (u32x4){weights[0], weights[1], weights[2], weights[3]});
+                pf[1] = __builtin_bit_cast(s16x8, (u32x4){weights[4], weights[5], weights[6], weights[7]});
             }
         };
         tile_there<NW>();
 #pragma unroll
         for (int d = 0; d < DT / 16; ++d) kf[d] = keys.read(smem, 0, d);
         scores(s[0]);
+        hide(s[0], j_begin);
+        high = highest(s[0]);
 #pragma unroll
         for (int d = 0; d < DT / 16; ++d) kf[d] = keys.read(smem, 1, d);
+        // (answered before the loop begins: the loop would wait in every turn for as many reads as are under way here)
+        __builtin_amdgcn_s_waitcnt(0xc07f);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             pf[x] = zero;
@@ -371,16 +417,17 @@ __global__ __launch_bounds__(128 * NQ) __attribute__((amdgpu_waves_per_eu(2, DT 
         }
         int j = j_begin, slot = 0;
         auto around = [&](auto masked) __attribute__((always_inline)) {
-            const int after = slot == 2 ? 0 : slot + 1, last = slot == 0 ? 2 : slot - 1;
-            turn(smem + last * STAGE, smem + slot * STAGE, smem + after * STAGE, j, masked);
+            const int after = (slot + 1) & 3;
+            turn(smem + (slot ^ 2) * STAGE, smem + slot * STAGE, smem + after * STAGE, j, masked);
             slot = after;
         };
-        for (; j + KT <= min(fewest, j_end); j += KT) around(std::false_type());
+        for (; j + KT + 32 <= min(fewest, j_end); j += KT) around(std::false_type());   // (it hides for the step after it)
         for (; j < j_end; j += KT) around(std::true_type());
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
             for (int v = 0; v < DV / 32; ++v) acc[v] = mfma32<T>(vf[x][v], pf[x], acc[v]);
+        wait_lds_dma();                                     // no copy is under way any more
     }
     total = both_halves_sum(total);
 
@@ -877,7 +924,7 @@ template <typename F> int allow_lds(F kernel, int bytes, const char *what) {
 }
 
 template <typename T, int DT, int NQ, int KT, bool AHEAD> int launch_attention(const Args &a, int64_t blocks, hipStream_t stream) {
-    constexpr int LDS = (AHEAD ? 3 : 2) * KT * DT * 8;
+    constexpr int LDS = (AHEAD ? 4 : 2) * KT * DT * 8;
     if (int rc = allow_lds(attention_kernel<T, DT, NQ, KT, AHEAD>, LDS, "attention")) return rc;
     hipLaunchKernelGGL((attention_kernel<T, DT, NQ, KT, AHEAD>), dim3((unsigned)blocks), dim3(128 * NQ), LDS, stream, a);
     return 0;
