@@ -14,7 +14,6 @@
 // of 16-bit operands are what those take.
 #include "tokens_common.hpp"
 #include <cmath>
-#include <type_traits>
 
 namespace bndm {
 namespace {
@@ -47,7 +46,7 @@ struct Args {
 
 // Copies tiles of R rows of C chunks into LDS, NW waves together.  Rows past rows_in and chunks past the head's size become zeros.  A lane's
 // offset is the same for all its pieces but for whole rows, which the scalar offset adds.
-template <int R, int C, int NW> struct Stager {
+template <int R, int C, int NW, bool COLUMNS = false> struct Stager {      // COLUMNS: a tile that is only read transposed
     static constexpr int N = R * C < 64 * NW ? 1 : R * C / (64 * NW), STEP = 64 * NW / C;  // pieces of a lane, rows between them
     int row;
     uint32_t off[STEP % 16 ? 16 / STEP : 1];                // (the swizzle's period is 16 rows)
@@ -59,7 +58,9 @@ template <int R, int C, int NW> struct Stager {
         step_bytes = (int)stride * STEP * 2;
 #pragma unroll
         for (int i = 0; i < (int)(sizeof(off) / 4); ++i) {
-            const int c = (at % C) ^ swizzle<C>(row + i * STEP);
+            int c = at % C;
+            if constexpr (COLUMNS) c ^= swizzle_columns<C>(row + i * STEP);
+            else c ^= swizzle<C>(row + i * STEP);
             off[i] = c < chunks_in ? (uint32_t)(row * (int)stride + c * 8) * 2u : kNowhere;
         }
     }
@@ -83,23 +84,34 @@ template <int C> struct RowReader {                    // 8 values (chunk 2 s + 
         return *reinterpret_cast<const s16x8 *>(lds + (at ^ ((s & 7) << 5)) + (s >> 3) * 256 + block * (32 * C * 16));
     }
 };
-template <int C> struct ColumnReader {                 // operand whose rows are the tile's COLUMNS 32 t .. + 31 and whose k are its rows
+template <int C, bool COLUMNS = false> struct ColumnReader {       // operand whose rows are the tile's COLUMNS 32 t .. + 31 and whose k are its rows
     int at;                                            // row0 .. row0 + 15 in the order in which a result tile holds them: lane half h has
     __device__ __forceinline__ void begin(int l) {     // rows row0 + 4 h + {0..3} and row0 + 8 + 4 h + {0..3}
         const int i = l & 15, col = (l & 16) + 4 * (i & 3), row = 4 * (l >> 5) + (i >> 2);
-        at = row * (C * 16) + (((col >> 3) ^ swizzle<C>(row)) << 4) + (col & 4) * 2;
+        int c = col >> 3;
+        if constexpr (COLUMNS) c ^= swizzle_columns<C>(row);
+        else c ^= swizzle<C>(row);
+        at = row * (C * 16) + (c << 4) + (col & 4) * 2;
     }
     __device__ __forceinline__ s16x8 read(const char *lds, int row0, int t) const {
         const char *p = lds + row0 * (C * 16) + (t >> 2) * 256;
-        return join(lds_read_tr(p + (at ^ ((t & 3) << 6))), lds_read_tr(p + (at ^ ((t & 3) << 6) ^ 32) + 8 * C * 16));
+        return join(lds_read_tr(p + (at ^ ((t & 3) << 6))), lds_read_tr(p + (at ^ ((t & 3) << 6) ^ (COLUMNS ? 0 : 32)) + 8 * C * 16));
     }
 };
 
-// Workgroups go to the 8 XCDs in turn: what this gives out in their place are runs for each, so that workgroups that read the same keys (or
-// queries) run behind one L2.  1024 workgroups over 32 heads of 2 MB each: 447 us in the order of launch, TODO this way.
-__device__ __forceinline__ int of_this_xcd(int id, int n) {
-    const int per = n / 8, more = n % 8, x = id & 7;
-    return x * per + min(x, more) + (id >> 3);
+// Workgroups go to the 8 XCDs in turn.  This deals out heads (the units that share keys, `tiles` workgroups each) to the XCDs, so that one's
+// workgroups run behind one L2, and within a head the last tile first: with a causal mask it is the longest.
+__device__ __forceinline__ void place(int id, int units, int tiles, int &unit, int &tile) {
+    const int even = units & ~7;
+    if (id < even * tiles) {
+        const int seq = id >> 3;
+        unit = (seq / tiles) * 8 + (id & 7);
+        tile = tiles - 1 - seq % tiles;
+    } else {
+        id -= even * tiles;
+        unit = even + id / tiles;
+        tile = tiles - 1 - id % tiles;
+    }
 }
 
 // registers 8 s .. 8 s + 7 of a result tile as an operand whose k are rows 16 s .. 16 s + 15 in that order
@@ -175,41 +187,43 @@ __device__ __forceinline__ int64_t length_of(const Args &a, int b) {
 
 // ---------------------------------------------------------------------------------------------- forward
 // NQ groups of 32 rows (queries), two waves each: one a map, so that a map's sums are all that a wave holds (with both maps in one wave,
-// heads of 64 spilled at two waves a SIMD: 570 us where this takes TODO).  KT keys a tile, 32 of them at a time.  DT: head size rounded up
+// heads of 64 spilled at two waves a SIMD: 570 us on 32 heads of 4096 queries and keys where this takes 434).  KT keys a tile, 32 of them at a time.  DT: head size rounded up
 // to 32, 64, 128; values are up to 2 DT wide.  The running maximum is followed loosely: sums are scaled down only when it has grown by a
 // factor of 2^8 (weights stay below 2^8 until then, and the final division takes care of them).
-//
-// AHEAD: the products of a step are interleaved with the exponentials of another, as the matrix and the vector units of a SIMD work side by
-// side only on different instructions of a wave (or of two waves that are not in step, and a barrier a tile keeps them in step): while the
-// weights of step t are formed, the scores of t + 1 and the values' sums of t - 1 are.  Without it the two add up, TODO us against TODO.
-template <typename T, int DT, int NQ, int KT, bool AHEAD>
-__global__ __launch_bounds__(128 * NQ) __attribute__((amdgpu_waves_per_eu(2, DT == 32 || NQ == 1 ? 4 : 2))) void attention_kernel(Args a) {
-    constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT, NW = 2 * NQ, BUFFERS = AHEAD ? 4 : 2;
+// What bounds it is the chip's power as much as its units: 434 us on random numbers (950 Tflop/s with both maps' products) are 365 on zeros,
+// and interleaving products with exponentials, or running scores a step ahead, changed neither by more than 3 %.
+template <typename T, int DT, int NQ, int KT>
+__global__ __launch_bounds__(128 * NQ, DT == 32 ? 4 : 2) void attention_kernel(Args a) {
+    constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT, NW = 2 * NQ;
     constexpr int K_BYTES = KT * CK * 16, V_BYTES = KT * CV * 16, STAGE = 2 * K_BYTES + V_BYTES;
-    static_assert(NQ * 32 * DV * 2 <= BUFFERS * STAGE && NQ * 8192 <= BUFFERS * STAGE, "results go through the same memory");
-    extern __shared__ __attribute__((aligned(16))) char smem[];
+    static_assert(NQ * 32 * DV * 2 <= 2 * STAGE && NQ * 8192 <= 2 * STAGE, "results go through the same memory");
+    __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
     const int tid = threadIdx.x, l = tid & 63, h32 = l >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6), m = w & 1, qw = w >> 1;
 
     // ---- which rows: (batch, group of query heads, tile of rows, part of the keys)
     const int64_t rows = a.Nq * a.heads_per_row;
     const int tiles = (int)((rows + 32 * NQ - 1) / (32 * NQ));
-    int id = of_this_xcd(blockIdx.x, gridDim.x);
-    const int split = id % a.splits; id /= a.splits;
-    const int tile = id % tiles; id /= tiles;
     const int groups = a.H / a.heads_per_row;
-    const int group = id % groups, b = id / groups;
+    int unit, tile;
+    place(blockIdx.x, a.B * groups, tiles * a.splits, unit, tile);
+    const int split = tile % a.splits, group = unit % groups, b = unit / groups;
+    tile /= a.splits;
     const int hk = group * a.heads_per_row / (a.H / a.Hk);
-    const int64_t row = (int64_t)tile * 32 * NQ + qw * 32 + (l & 31);
-    const bool row_in = row < rows;
-    const int sub = row_in ? (int)(row / a.Nq) : 0;
-    const int64_t i = row_in ? row - (int64_t)sub * a.Nq : 0;
-    const int head = group * a.heads_per_row + sub;
+    // a lane's row: its query and head
+    struct Row { int64_t i; int head; bool in; };
+    auto row_of = [&](int lane) __attribute__((always_inline)) {
+        const int64_t row = (int64_t)tile * 32 * NQ + qw * 32 + (lane & 31);
+        const bool in = row < rows;
+        const int sub = in ? (int)(row / a.Nq) : 0;
+        return Row{in ? row - (int64_t)sub * a.Nq : 0, group * a.heads_per_row + sub, in};
+    };
 
     const int64_t start = start_of(a, b);
     const int len = (int)length_of(a, b);
     auto upto = [&](int64_t i) { return a.causal ? (int)min((int64_t)len, max((int64_t)0, start + i + 1)) : len; };   // keys that query i sees
-    const int sees = row_in ? upto(i) : 0;
+    const Row mine = row_of(l);
+    const int sees = mine.in ? upto(mine.i) : 0;
     // (rows of one head are in order; several heads in one tile: from the first query's keys to the last one's)
     const bool packed = a.heads_per_row > 1;
     const int most = upto(packed ? a.Nq - 1 : min(a.Nq - 1, (int64_t)(tile + 1) * 32 * NQ - 1));
@@ -219,41 +233,35 @@ __global__ __launch_bounds__(128 * NQ) __attribute__((amdgpu_waves_per_eu(2, DT 
     const T *kp = (const T *)a.k + (int64_t)b * a.kb + (int64_t)(2 * hk) * a.kh;
     const T *vp = (const T *)a.v + (int64_t)b * a.vb + (int64_t)hk * a.vh;
     Stager<KT, CK, NW> stage_k;
-    Stager<KT, CV, NW> stage_v;
+    Stager<KT, CV, NW, true> stage_v;
     stage_k.begin(a.kn, a.D / 8, w, l);
     stage_v.begin(a.vn, a.Dv / 8, w, l);
-    // the tile that is copied next, a third at a time
+    // the tile that is copied next
     int j_next = j_begin;
     const T *k_next = kp + j_begin * a.kn, *v_next = vp + j_begin * a.vn;
     const int64_t k_step = KT * a.kn, v_step = KT * a.vn;
-    auto fetch = [&](char *to, int what) __attribute__((always_inline)) {
-        if (what == 0) stage_k.copy(to, k_next, len - j_next, w);
-        else if (what == 1) stage_k.copy(to + K_BYTES, k_next + a.kh, len - j_next, w);
-        else {
-            stage_v.copy(to + 2 * K_BYTES, v_next, len - j_next, w);
-            k_next += k_step;
-            v_next += v_step;
-            j_next += KT;
-        }
+    auto fetch = [&](char *to) __attribute__((always_inline)) {
+        stage_k.copy(to, k_next, len - j_next, w);
+        stage_k.copy(to + K_BYTES, k_next + a.kh, len - j_next, w);
+        stage_v.copy(to + 2 * K_BYTES, v_next, len - j_next, w);
+        k_next += k_step;
+        v_next += v_step;
+        j_next += KT;
     };
-    if (j_begin < j_end)
-#pragma unroll
-        for (int n = 0; n < (AHEAD ? 2 : 1); ++n)
-#pragma unroll
-            for (int what = 0; what < 3; ++what) fetch(smem + n * STAGE, what);
+    if (j_begin < j_end) fetch(smem);
 
     // ---- queries: right operands, in registers
     s16x8 qf[DT / 16];
     {
-        const T *p = (const T *)a.q + (int64_t)b * a.qb + i * a.qn + (int64_t)(2 * head + m) * a.qh;
+        const T *p = (const T *)a.q + (int64_t)b * a.qb + mine.i * a.qn + (int64_t)(2 * mine.head + m) * a.qh;
 #pragma unroll
         for (int s = 0; s < DT / 16; ++s) {
             const int c = 2 * s + h32;
-            qf[s] = load8(p + c * 8, row_in && c * 8 < a.D);
+            qf[s] = load8(p + c * 8, mine.in && c * 8 < a.D);
         }
     }
     RowReader<CK> keys;
-    ColumnReader<CV> values;
+    ColumnReader<CV, true> values;
     keys.begin(l);
     values.begin(l);
     keys.at += m * K_BYTES;
@@ -263,174 +271,58 @@ __global__ __launch_bounds__(128 * NQ) __attribute__((amdgpu_waves_per_eu(2, DT 
     float top = kLowest, total = 0.f;
     const float to_log2 = a.scale * kLog2e;
 
-    auto hide = [&](f32x16 &s, int j) __attribute__((always_inline)) {      // keys from j on, those that the row does not see
-        const int n = sees - j;
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-            if (tile_row(r, h32) >= n) s[r] = -INFINITY;
-    };
-    auto highest = [&](const f32x16 &s) __attribute__((always_inline)) {
-        float high = s[0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) high = fmaxf(high, s[r]);
-        return high;
-    };
-    // `high`: a lane's highest score.  The maximum is kept as a whole power of two, so that what is scaled down with it stays exact.  `held`:
-    // weights that are yet to meet their values.
-    auto follow = [&](float high, s16x8 (&held)[2]) __attribute__((always_inline)) {
-        high = both_halves_max(high) * to_log2;
-        if (__any(high > top + 8.0f)) {
-            const float up = fmaxf(top, ceilf(high)), shrink = __builtin_amdgcn_exp2f(top - up);
-            top = up;
-            total *= shrink;
-#pragma unroll
-            for (int v = 0; v < DV / 32; ++v)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) acc[v][r] *= shrink;
-            if constexpr (AHEAD)
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const short h = held[x][e];
-                        held[x][e] = __builtin_bit_cast(short, (T)(widen<T>(h) * shrink));
-                    }
-        }
-    };
-    auto weigh = [&](f32x16 &s, s16x8 (&pf)[2]) __attribute__((always_inline)) {
-        float sum = 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], to_log2, -top));
-            sum += s[r];
-        }
-        total += sum;
-        pf[0] = as_operand<T>(s, 0);
-        pf[1] = as_operand<T>(s, 1);
-    };
-    // (__restrict__ below: the compiler would have the copies to `ahead` arrive before the first read of the other tiles)
-    if constexpr (!AHEAD) {
-        auto turn = [&](char *__restrict__ ahead, const char *__restrict__ now, int j) __attribute__((always_inline)) {
-            tile_there<NW>();
-            if (j + KT < j_end)
-#pragma unroll
-                for (int what = 0; what < 3; ++what) fetch(ahead, what);
-#pragma unroll
-            for (int t = 0; t < KT / 32; ++t) {
-                f32x16 s[1];
-                s16x8 pf[2];
-                clear(s);
-#pragma unroll
-                for (int d = 0; d < DT / 16; ++d) s[0] = mfma32<T>(keys.read(now, t, d), qf[d], s[0]);
-                if (j + 32 * t + 32 > fewest) hide(s[0], j + 32 * t);
-                follow(highest(s[0]), pf);
-                weigh(s[0], pf);
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                    for (int v = 0; v < DV / 32; ++v) acc[v] = mfma32<T>(values.read(now + 2 * K_BYTES, 32 * t + 16 * x, v), pf[x], acc[v]);
-            }
-        };
-        for (int j = j_begin; j < j_end; j += 2 * KT) {
-            turn(smem + STAGE, smem, j);
-            if (j + KT < j_end) turn(smem, smem + STAGE, j + KT);
-        }
-    } else if (j_begin < j_end) {
-        static_assert(!AHEAD || KT == 64, "two steps a tile");
-        f32x16 s[2];
-        s16x8 kf[DT / 16], vf[2][DV / 32], pf[2];           // keys of t + 1, values and weights of t - 1
-        auto scores = [&](f32x16 &s) __attribute__((always_inline)) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = 0.f;
-#pragma unroll
-            for (int d = 0; d < DT / 16; ++d) s = mfma32<T>(kf[d], qf[d], s);
-        };
-        const s16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
-        float high;
-        constexpr int S = DT / 16, V = DV / 32, G = S + 2 * V, E = 16 * 3 / (2 * G);   // products of a step; exponentials that go with one of the first 16 / E
-        // The tile's two steps; its scores are there (the first's) or its keys are (the second's); `next` has the tile after it.  Each product
-        // goes with a share of the vector work, and the compiler is kept from regrouping them.
-        auto turn = [&](char *__restrict__ ahead, const char *__restrict__ now, const char *__restrict__ next, int j, auto masked) __attribute__((always_inline)) {
-            // The next tile is there.  What `ahead` held was last read a whole tile ago, so that no wave waits for its reads here.
-            // (Tiles past the end are copied too, as far as the sequence goes, and never used.)
-            asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                follow(high, pf);
-                uint32_t weights[8];
-                float sum[2] = {0.f, 0.f};
-                f32x16 &cur = s[t], &nxt = s[t ^ 1];
-#pragma unroll
-                for (int r = 0; r < 16; ++r) nxt[r] = 0.f;
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    if (g < S) {
-                        nxt = mfma32<T>(kf[g], qf[g], nxt);
-                        kf[g] = keys.read(next, t, g);
-                    } else {
-                        const int x = (g - S) / V, v = (g - S) % V;
-                        acc[v] = mfma32<T>(vf[x][v], pf[x], acc[v]);
-                        vf[x][v] = values.read(now + 2 * K_BYTES, 32 * t + 16 * x, v);
-                    }
-                    if (t == 0 && g < 3) fetch(ahead, g);
-                    if (g * E < 16) {
-#pragma unroll
-                        for (int e = 0; e < E; ++e) {
-                            cur[g * E + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[g * E + e], to_log2, -top));
-                            sum[e & 1] += cur[g * E + e];
-                        }
-#pragma unroll
-                        for (int e = 0; e < E; e += 2) weights[(g * E + e) / 2] = pack2<T>(cur[g * E + e], cur[g * E + e + 1]);
-                    } else {
-                        constexpr int M = 16 / (G - 16 / E);
-                        const int r0 = (g - 16 / E) * M;
-                        if (r0 == 0) {
-                            if (decltype(masked)::value) hide(nxt, j + 32 * t + 32);
-                            high = nxt[0];
-                        }
-#pragma unroll
-                        for (int r = r0; r < r0 + M; ++r) high = fmaxf(high, nxt[r]);
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                total += sum[0] + sum[1];
-                pf[0] = __builtin_bit_cast(s16x8, (u32x4){weights[0], weights[1], weights[2], weights[3]});
-                pf[1] = __builtin_bit_cast(s16x8, (u32x4){weights[4], weights[5], weights[6], weights[7]});
-            }
-        };
+    // One tile; the next one is on its way to `ahead`.  (__restrict__: the compiler would have it arrive before the first read of `now`.)
+    auto turn = [&](char *__restrict__ ahead, const char *__restrict__ now, int j) __attribute__((always_inline)) {
         tile_there<NW>();
+        if (j + KT < j_end) fetch(ahead);
 #pragma unroll
-        for (int d = 0; d < DT / 16; ++d) kf[d] = keys.read(smem, 0, d);
-        scores(s[0]);
-        hide(s[0], j_begin);
-        high = highest(s[0]);
+        for (int t = 0; t < KT / 32; ++t) {
+            f32x16 s[1];
+            clear(s);
 #pragma unroll
-        for (int d = 0; d < DT / 16; ++d) kf[d] = keys.read(smem, 1, d);
-        // (answered before the loop begins: the loop would wait in every turn for as many reads as are under way here)
-        __builtin_amdgcn_s_waitcnt(0xc07f);
+            for (int d = 0; d < DT / 16; ++d) s[0] = mfma32<T>(keys.read(now, t, d), qf[d], s[0]);
+            if (j + 32 * t + 32 > fewest) {
+                const int n = sees - j - 32 * t - 4 * h32;  // (rows of the other half of the lanes are 4 further down)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            pf[x] = zero;
+                for (int r = 0; r < 16; ++r)
+                    if (tile_row(r, 0) >= n) s[0][r] = -INFINITY;
+            }
+            float high = s[0][0];
 #pragma unroll
-            for (int v = 0; v < DV / 32; ++v) vf[x][v] = zero;
+            for (int r = 1; r < 16; ++r) high = fmaxf(high, s[0][r]);
+            high = both_halves_max(high) * to_log2;
+            if (__any(high > top + 8.0f)) {
+                const float up = fmaxf(top, high), shrink = __builtin_amdgcn_exp2f(top - up);
+                top = up;
+                total *= shrink;
+#pragma unroll
+                for (int v = 0; v < DV / 32; ++v)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[v][r] *= shrink;
+            }
+            float sum = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[0][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], to_log2, -top));
+                sum += s[0][r];
+            }
+            total += sum;
+            const s16x8 pf[2] = {as_operand<T>(s[0], 0), as_operand<T>(s[0], 1)};
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int v = 0; v < DV / 32; ++v) acc[v] = mfma32<T>(values.read(now + 2 * K_BYTES, 32 * t + 16 * x, v), pf[x], acc[v]);
         }
-        int j = j_begin, slot = 0;
-        auto around = [&](auto masked) __attribute__((always_inline)) {
-            const int after = (slot + 1) & 3;
-            turn(smem + (slot ^ 2) * STAGE, smem + slot * STAGE, smem + after * STAGE, j, masked);
-            slot = after;
-        };
-        for (; j + KT + 32 <= min(fewest, j_end); j += KT) around(std::false_type());   // (it hides for the step after it)
-        for (; j < j_end; j += KT) around(std::true_type());
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int v = 0; v < DV / 32; ++v) acc[v] = mfma32<T>(vf[x][v], pf[x], acc[v]);
-        wait_lds_dma();                                     // no copy is under way any more
+    };
+    for (int j = j_begin; j < j_end; j += 2 * KT) {
+        turn(smem + STAGE, smem, j);
+        if (j + KT < j_end) turn(smem, smem + STAGE, j + KT);
     }
     total = both_halves_sum(total);
 
+    int lane = l;                                           // (told apart from l, so that nothing of the row is kept through the loop)
+    asm volatile("" : "+v"(lane));
+    const auto [i, head, row_in] = row_of(lane);
     if (a.part) {                                           // unfinished sums of this part
         if (!row_in) return;
         float *to = a.part + ((((int64_t)b * a.H + head) * a.Nq + i) * a.splits + split) * (2 * a.Dv + 4);
@@ -546,9 +438,9 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
     const int tid = threadIdx.x, l = tid & 63, h32 = l >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int tiles = (int)((a.Nq + 127) / 128);
-    int id = of_this_xcd(blockIdx.x, gridDim.x);
-    const int tile = id % tiles; id /= tiles;
-    const int head = id % a.H, b = id / a.H;
+    int unit, tile;
+    place(blockIdx.x, a.B * a.H, tiles, unit, tile);
+    const int head = unit % a.H, b = unit / a.H;
     const int hk = head / (a.H / a.Hk);
     const int64_t row = (int64_t)tile * 128 + w * 32 + (l & 31);
     const bool row_in = row < a.Nq;
@@ -642,10 +534,10 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
                 for (int r = 0; r < 16; ++r)
                     s[m][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][r], to_log2, -lse[m])) * (dp[0][r] - delta[m]);
                 if (masked) {                               // (a row that sees one key has weight 1 there whatever its score)
-                    const int n = sees == 1 ? 0 : sees - j - 32 * t;
+                    const int n = sees == 1 ? 0 : sees - j - 32 * t - 4 * h32;
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
-                        if (tile_row(r, h32) >= n) s[m][r] = 0.f;
+                        if (tile_row(r, 0) >= n) s[m][r] = 0.f;
                 }
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
@@ -765,6 +657,7 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
         const float *stats = reinterpret_cast<const float *>(gs + G_BYTES) + 32 * qw + 4 * h32;
         // the last key that the first of these queries sees (clamped: only its place among the keys counts)
         const int last0 = a.causal ? (int)max((int64_t)-64, min((int64_t)1 << 30, start + i0 + 32 * qw)) : 1 << 30;
+        const int last = last0 + 4 * h32;
         // some pair is hidden, or some row sees one key only
         const bool masked = key0 + 32 > len || key0 + 31 > last0 || len == 1 || last0 <= 0;
         f32x16 dp[1], s[2];
@@ -790,9 +683,9 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
                     float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][r + e], to_log2, -ls[e]));
                     float ds = p * (dp[0][r + e] - de[e]);
                     if (masked) {
-                        const int last = last0 + tile_row(r + e, h32);
-                        if (key >= len || key > last) p = ds = 0.f;
-                        if (len == 1 || last == 0) ds = 0.f;
+                        // query tile_row(r + e, 0) of the half sees keys up to last + that
+                        if (key >= len || key - last > tile_row(r + e, 0)) p = ds = 0.f;
+                        if (len == 1 || -last == tile_row(r + e, 0)) ds = 0.f;
                     }
                     if (m == 0) wt[r + e] = p;
                     else {
@@ -923,16 +816,10 @@ template <typename F> int allow_lds(F kernel, int bytes, const char *what) {
     return (int)e;
 }
 
-template <typename T, int DT, int NQ, int KT, bool AHEAD> int launch_attention(const Args &a, int64_t blocks, hipStream_t stream) {
-    constexpr int LDS = (AHEAD ? 4 : 2) * KT * DT * 8;
-    if (int rc = allow_lds(attention_kernel<T, DT, NQ, KT, AHEAD>, LDS, "attention")) return rc;
-    hipLaunchKernelGGL((attention_kernel<T, DT, NQ, KT, AHEAD>), dim3((unsigned)blocks), dim3(128 * NQ), LDS, stream, a);
-    return 0;
-}
-
 template <typename T, int DT> int forward(const Args &a, const Plan &p, hipStream_t stream) {
     constexpr int KT = DT == 128 ? 32 : 64;
-    if (int rc = p.waves == 1 ? launch_attention<T, DT, 1, 32, false>(a, p.blocks, stream) : launch_attention<T, DT, 4, KT, DT != 128>(a, p.blocks, stream)) return rc;
+    if (p.waves == 1) hipLaunchKernelGGL((attention_kernel<T, DT, 1, 32>), dim3((unsigned)p.blocks), dim3(128), 0, stream, a);
+    else hipLaunchKernelGGL((attention_kernel<T, DT, 4, KT>), dim3((unsigned)p.blocks), dim3(512), 0, stream, a);
     if (int rc = tokens_launch_status("attention")) return rc;
     if (a.part) {
         hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)((int64_t)a.B * a.H * a.Nq)), dim3(512), 0, stream, a);

@@ -96,6 +96,13 @@ template <int C> __device__ __forceinline__ int swizzle(int row) {
     else return ((row & 3) << 2) | ((row >> 2) & 3);
 }
 
+// The same for tiles that are only read transposed: rows 8 apart are then a constant apart.
+template <int C> __device__ __forceinline__ int swizzle_columns(int row) {
+    static_assert(C >= 8, "four rows of 64 bytes need none");
+    if constexpr (C == 8) return (row & 2) << 1;
+    else return (row & 3) << 2;
+}
+
 // offset past every descriptor's range: the load returns zeros
 constexpr uint32_t kNowhere = 0x80000000u;
 constexpr int kAnywhere = 0x7ffffff0;
