@@ -314,6 +314,7 @@ __global__ __launch_bounds__(128 * NQ, DT == 32 ? 4 : 2) void attention_kernel(A
                 for (int v = 0; v < DV / 32; ++v) acc[v] = mfma32<T>(values.read(now + 2 * K_BYTES, 32 * t + 16 * x, v), pf[x], acc[v]);
         }
     };
+    __builtin_amdgcn_s_waitcnt(0);                          // (what came before the loop is there, or its turns would wait for as much)
     for (int j = j_begin; j < j_end; j += 2 * KT) {
         turn(smem + STAGE, smem, j);
         if (j + KT < j_end) turn(smem, smem + STAGE, j + KT);
@@ -526,28 +527,29 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
             for (int d = 0; d < DV / 16; ++d) dp[0] = mfma32<T>(values.read(now + 2 * K_BYTES, t, d), gf[d], dp[0]);
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
-                f32x16 s[2];
+                f32x16 s[1];
                 clear(s);
 #pragma unroll
-                for (int d = 0; d < DT / 16; ++d) s[m] = mfma32<T>(keys.read(now + m * K_BYTES, t, d), qf[m][d], s[m]);
+                for (int d = 0; d < DT / 16; ++d) s[0] = mfma32<T>(keys.read(now + m * K_BYTES, t, d), qf[m][d], s[0]);
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    s[m][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][r], to_log2, -lse[m])) * (dp[0][r] - delta[m]);
+                    s[0][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], to_log2, -lse[m])) * (dp[0][r] - delta[m]);
                 if (masked) {                               // (a row that sees one key has weight 1 there whatever its score)
                     const int n = sees == 1 ? 0 : sees - j - 32 * t - 4 * h32;
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
-                        if (tile_row(r, 0) >= n) s[m][r] = 0.f;
+                        if (tile_row(r, 0) >= n) s[0][r] = 0.f;
                 }
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    const s16x8 ds = as_operand<T>(s[m], x);
+                    const s16x8 ds = as_operand<T>(s[0], x);
 #pragma unroll
                     for (int d = 0; d < DT / 32; ++d) acc[m][d] = mfma32<T>(key_columns.read(now + m * K_BYTES, 32 * t + 16 * x, d), ds, acc[m][d]);
                 }
             }
         }
     };
+    __builtin_amdgcn_s_waitcnt(0);                          // (what came before the loop is there, or its turns would wait for as much)
     for (int j = 0; j < j_end; j += 2 * KT) {
         turn(smem + STAGE, smem, j);
         if (j + KT < j_end) turn(smem, smem + STAGE, j + KT);
@@ -592,28 +594,45 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
     if (a.causal) i_first = max((int64_t)0, first_key - start) / QT * QT;
     if (first_key >= len) i_first = a.Nq;
     const int per_head = i_first < a.Nq ? (int)((a.Nq - i_first + QT - 1) / QT) : 0;
-    int g_next = 0;                                         // the tile that is fetched next
-    int64_t i_next = i_first;
     int steps = per_head * per;
 
+    // the tile of queries that is copied next
     Stager<QT, CK, NW> stage_q;
     Stager<QT, CV, NW> stage_g;
     stage_q.begin(a.qn, a.D / 8, w, l);
     stage_g.begin(a.don, a.Dv / 8, w, l);
-    auto fetch = [&](char *to) __attribute__((always_inline)) {
-        const int head = hk * per + g_next, in = (int)min((int64_t)QT, a.Nq - i_next);
-        const T *qp = (const T *)a.q + (int64_t)b * a.qb + i_next * a.qn + (int64_t)(2 * head) * a.qh;
-        stage_q.copy(to, qp, in, w);
-        stage_q.copy(to + Q_BYTES, qp + a.qh, in, w);
-        stage_g.copy(to + 2 * Q_BYTES, (const T *)a.dout + (int64_t)b * a.dob + i_next * a.don + (int64_t)head * a.doh, in, w);
+    int g_next = 0;
+    int64_t i_next = i_first;
+    const T *q_next = nullptr, *d_next = nullptr;
+    const float *s_next = nullptr;
+    auto first_of_head = [&]() __attribute__((always_inline)) {
+        const int head = hk * per + g_next;
+        q_next = (const T *)a.q + (int64_t)b * a.qb + i_first * a.qn + (int64_t)(2 * head) * a.qh;
+        d_next = (const T *)a.dout + (int64_t)b * a.dob + i_first * a.don + (int64_t)head * a.doh;
         // one of lse1, lse2, D1, D2 a wave.  (Queries past the end have zeros everywhere: their weight of 1 meets do = 0.)
-        const float *from = (w < 2 ? a.lse : a.delta) + ((int64_t)b * 2 * a.H + 2 * head + (w & 1)) * a.Nq + i_next;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(uniform_rsrc(from, kAnywhere), (lds_ptr_t)(to + 2 * Q_BYTES + G_BYTES + w * QT * 4), 4,
-                                                 l < in ? (uint32_t)l * 4u : kNowhere, 0, 0, 0);
-        i_next += QT;
-        if (i_next >= a.Nq) i_next = i_first, ++g_next;
+        s_next = (w < 2 ? a.lse : a.delta) + ((int64_t)b * 2 * a.H + 2 * head + (w & 1)) * a.Nq + i_first;
+        i_next = i_first;
     };
-    if (steps) fetch(smem);
+    auto fetch = [&](char *to) __attribute__((always_inline)) {
+        const int in = (int)min((int64_t)QT, a.Nq - i_next);
+        stage_q.copy(to, q_next, in, w);
+        stage_q.copy(to + Q_BYTES, q_next + a.qh, in, w);
+        stage_g.copy(to + 2 * Q_BYTES, d_next, in, w);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(uniform_rsrc(s_next, kAnywhere), (lds_ptr_t)(to + 2 * Q_BYTES + G_BYTES + w * QT * 4), 4,
+                                                 l < in ? (uint32_t)l * 4u : kNowhere, 0, 0, 0);
+        q_next += QT * a.qn;
+        d_next += QT * a.don;
+        s_next += QT;
+        i_next += QT;
+        if (i_next >= a.Nq) {
+            ++g_next;
+            first_of_head();
+        }
+    };
+    if (steps) {
+        first_of_head();
+        fetch(smem);
+    }
 
     s16x8 kf[2][DT / 16], vf[KEYS ? DV / 16 : 1];
 #pragma unroll
@@ -649,10 +668,15 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
 
     int g = 0;
     int64_t i0 = i_first;
+    // (made uniform, and thereby waited for, where it is read: a wait for it later on would be one for the copies as well)
+    auto lam_of_head = [&](int head) {
+        const float x = lam_of<T>(a, head);
+        return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+    };
+    float lam = lam_of_head(hk * per);
     auto turn = [&](char *__restrict__ ahead, const char *__restrict__ now) __attribute__((always_inline)) {
         tile_there<NW>();
         if (steps > 1) fetch(ahead);
-        const float lam = lam_of<T>(a, hk * per + g);
         const char *gs = now + 2 * Q_BYTES;
         const float *stats = reinterpret_cast<const float *>(gs + G_BYTES) + 32 * qw + 4 * h32;
         // the last key that the first of these queries sees (clamped: only its place among the keys counts)
@@ -660,60 +684,94 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
         const int last = last0 + 4 * h32;
         // some pair is hidden, or some row sees one key only
         const bool masked = key0 + 32 > len || key0 + 31 > last0 || len == 1 || last0 <= 0;
+        // One wave a SIMD has nothing else to do while it waits: reads go out in groups, ahead of what needs them.
+        s16x8 rows[2][DT / 16], grad_rows[KEYS ? DV / 16 : 1];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int d = 0; d < DT / 16; ++d) rows[m][d] = queries.read(now + m * Q_BYTES, qw, d);
+        if constexpr (KEYS)
+#pragma unroll
+            for (int d = 0; d < DV / 16; ++d) grad_rows[d] = grads.read(gs, qw, d);
+        f32x4 ls[2][4], de[2][4];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                ls[m][r] = *reinterpret_cast<const f32x4 *>(stats + m * QT + 8 * r);
+                if constexpr (KEYS) de[m][r] = *reinterpret_cast<const f32x4 *>(stats + (2 + m) * QT + 8 * r);
+            }
+        if constexpr (DT <= 64) __builtin_amdgcn_sched_barrier(0);
         f32x16 dp[1], s[2];
         clear(dp);
         clear(s);
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
-            for (int d = 0; d < DT / 16; ++d) s[m] = mfma32<T>(queries.read(now + m * Q_BYTES, qw, d), kf[m][d], s[m]);
+            for (int d = 0; d < DT / 16; ++d) s[m] = mfma32<T>(rows[m][d], kf[m][d], s[m]);
         if constexpr (KEYS)
 #pragma unroll
-            for (int d = 0; d < DV / 16; ++d) dp[0] = mfma32<T>(grads.read(gs, qw, d), vf[d], dp[0]);
-        f32x16 wt;
+            for (int d = 0; d < DV / 16; ++d) dp[0] = mfma32<T>(grad_rows[d], vf[d], dp[0]);
+        s16x8 query_cols[KEYS ? 2 : 1][2][DT / 32], grad_cols[VALUES ? 2 : 1][DV / 32];
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const f32x4 ls = *reinterpret_cast<const f32x4 *>(stats + m * QT + 2 * r);
-                f32x4 de = {0.f, 0.f, 0.f, 0.f};
-                if constexpr (KEYS) de = *reinterpret_cast<const f32x4 *>(stats + (2 + m) * QT + 2 * r);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][r + e], to_log2, -ls[e]));
-                    float ds = p * (dp[0][r + e] - de[e]);
-                    if (masked) {
-                        // query tile_row(r + e, 0) of the half sees keys up to last + that
-                        if (key >= len || key - last > tile_row(r + e, 0)) p = ds = 0.f;
-                        if (len == 1 || -last == tile_row(r + e, 0)) ds = 0.f;
-                    }
-                    if (m == 0) wt[r + e] = p;
-                    else {
-                        wt[r + e] -= lam * p;
-                        ds *= -lam;
-                    }
-                    s[m][r + e] = ds;
-                }
-            }
+        for (int x = 0; x < 2; ++x) {
             if constexpr (KEYS)
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const s16x8 ds = as_operand<T>(s[m], x);
+                for (int m = 0; m < 2; ++m)
 #pragma unroll
-                    for (int d = 0; d < DT / 32; ++d) dk[m][d] = mfma32<T>(query_columns.read(now + m * Q_BYTES, 32 * qw + 16 * x, d), ds, dk[m][d]);
+                    for (int d = 0; d < DT / 32; ++d) query_cols[m][x][d] = query_columns.read(now + m * Q_BYTES, 32 * qw + 16 * x, d);
+            if constexpr (VALUES)
+#pragma unroll
+                for (int d = 0; d < DV / 32; ++d) grad_cols[x][d] = grad_columns.read(gs, 32 * qw + 16 * x, d);
+        }
+        if constexpr (DT <= 64) __builtin_amdgcn_sched_barrier(0);
+        f32x16 p[2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                p[m][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][r], to_log2, -ls[m][r / 4][r % 4]));
+                if constexpr (KEYS) s[m][r] = p[m][r] * (dp[0][r] - de[m][r / 4][r % 4]);
+            }
+        if (masked) {
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    // query tile_row(r, 0) of the half sees keys up to last + that
+                    if (key >= len || key - last > tile_row(r, 0)) p[m][r] = s[m][r] = 0.f;
+                    if (len == 1 || -last == tile_row(r, 0)) s[m][r] = 0.f;
                 }
         }
-        if constexpr (VALUES)
+        if constexpr (KEYS)
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    if (m && !x)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[1][r] *= -lam;
+                    const s16x8 ds = as_operand<T>(s[m], x);
+#pragma unroll
+                    for (int d = 0; d < DT / 32; ++d) dk[m][d] = mfma32<T>(query_cols[m][x][d], ds, dk[m][d]);
+                }
+        if constexpr (VALUES) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) p[0][r] -= lam * p[1][r];
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                const s16x8 wf = as_operand<T>(wt, x);
+                const s16x8 wf = as_operand<T>(p[0], x);
 #pragma unroll
-                for (int d = 0; d < DV / 32; ++d) dv[d] = mfma32<T>(grad_columns.read(gs, 32 * qw + 16 * x, d), wf, dv[d]);
+                for (int d = 0; d < DV / 32; ++d) dv[d] = mfma32<T>(grad_cols[x][d], wf, dv[d]);
             }
+        }
         i0 += QT;
-        if (i0 >= a.Nq) i0 = i_first, ++g;
-        --steps;
+        if (i0 >= a.Nq && --steps) {
+            i0 = i_first;
+            lam = lam_of_head(hk * per + ++g);
+        } else if (i0 < a.Nq) --steps;
     };
+    __builtin_amdgcn_s_waitcnt(0);                          // (what came before the loop is there, or its turns would wait for as much)
     while (steps > 0) {
         turn(smem + STAGE, smem);
         if (steps > 0) turn(smem, smem + STAGE);
