@@ -464,30 +464,39 @@ struct Choice {
     int64_t split_k;
 };
 
-// What a step of 64 along the summed index takes a workgroup, and how many run on the 256 CUs at once; splitting it costs the parts' way
-// to memory and back and a launch.
+// The least of what the kernels take by this model, in us, fitted to 12 choices at each of 33 sizes from 1 x 4096 x 4096 to
+// 16384 x 4096 x 1024 (rows x sum x columns), of which these are some, measured:
+//                         rows kernel: 16 at a time,   32,    64;  128 x 128 tiles,  in 8 parts;  256 x 256 tiles
+//   128 x 512 x 512                        3.6           4.1    5.0         9.8            10.3           19.1
+//   512 x 512 x 512                        6.3           5.5    5.2         9.9            13.6           19.5
+//   2048 x 512 x 512                      17.3          13.5   11.8        10.4              -            19.4
+//   64 x 4096 x 4096                      31.8          25.9   22.5          -             16.3             -
+//   128 x 4096 x 4096                     59.8          45.4   39.4        36.7            20.0           80.4
+//   2048 x 2048 x 2048                      -           170    143         26.5              -            49.8
+//   16384 x 4096 x 1024                     -             -      -         163               -            121
+// A step of 64 along the sum takes a 128 x 128 tile 0.6 us alone on its CU and 1.15 with another one, a 256 x 256 tile 1.2 on a few
+// CUs and 1.75 on all of them; the kernel for few rows reads 512 of the sum at a time.
 Choice choose(int64_t M, int64_t N, int64_t K, bool rows_ok, bool wide) {
     Choice best = {1, 1, 1, K};
-    if (rows_ok && M <= 64) {
-        best.kind = 0;
-        best.mt = ceil_div64(N, 16) * ceil_div64(M, 16) <= 1024 ? 1 : M <= 16 ? 1 : M <= 32 ? 2 : 4;
-        return best;
-    }
     double least = 1e300;
+    for (int mt = 1; rows_ok && mt <= 4; mt *= 2) {
+        const double blocks = (double)ceil_div64(M, 16 * mt) * (double)ceil_div64(N, 16);
+        const double alone = mt == 1 ? 0.9 : mt == 2 ? 1.4 : 2.4, full = blocks * (mt == 1 ? 0.0036 : mt == 2 ? 0.0053 : 0.0091);
+        const double us = 2.6 + (double)ceil_div64(K, 512) * (full > alone ? full : alone);
+        if (us < least) least = us, best = {0, 1, mt, K};
+    }
+    const int64_t steps = ceil_div64(K, 64);
     for (int kind = 1; kind <= (wide ? 2 : 1); ++kind) {
-        const int64_t t = kind == 2 ? 256 : 128, tn = t;
-        const int64_t tiles = ceil_div64(M, t) * ceil_div64(N, tn), steps = ceil_div64(K, 64);
-        const int at_once = kind == 2 ? 256 : 512;
-        const double step_us = kind == 2 ? 1.2 : 0.9;
-        for (int s = 1; s <= 16; s *= 2) {
-            if (s > 1 && (steps / s < 8 || tiles * s > 2 * at_once)) break;
-            double us = (double)ceil_div64(tiles * s, at_once) * ((double)ceil_div64(steps, s) * step_us + 3.0);
-            if (s > 1) us += 4.0 + (double)M * N * 8.0 * s / 4.0e6;
+        const int64_t t = kind == 2 ? 256 : 128, tiles = ceil_div64(M, t) * ceil_div64(N, t);
+        for (int s = 1; s <= 16 && (s == 1 || (steps / s >= 4 && tiles * s <= 1024)); s *= 2) {
+            const int64_t all = tiles * s, at_once = kind == 2 ? 256 : all <= 256 ? 256 : 512;
+            const double step = kind == 2 ? 1.2 + 0.55 * (all < 256 ? all / 256.0 : 1.0) : all <= 256 ? 0.6 : 1.15;
+            double us = (double)ceil_div64(all, at_once) * ((double)ceil_div64(steps, s) * step + (kind == 2 ? 9.0 : 4.5));
+            if (s > 1) us += 3.0 + (double)M * (double)N * 8.0 * s / 5.0e6;
             if (us < least) least = us, best = {kind, s, 1, ceil_div64(steps, s) * 64};
         }
     }
-    best.splits = (int)ceil_div64(K > 0 ? K : 1, best.split_k > 0 ? best.split_k : 1);
-    if (best.splits < 1) best.splits = 1;
+    best.splits = best.kind == 0 || K == 0 ? 1 : (int)ceil_div64(K, best.split_k);
     return best;
 }
 size_t parts_bytes(const Choice &c, int64_t M, int64_t N) { return c.splits > 1 ? (size_t)c.splits * M * N * 4 : 0; }
