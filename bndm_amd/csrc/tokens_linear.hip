@@ -141,20 +141,18 @@ template <typename T, bool TR, int ROWS, int THREADS> struct Operand {
     static_assert(STEP % 16 == 0 || (TR && STEP == 8), "the swizzle's period is 16 rows, and 8 rows on it differs by 2");
 
     const char *base;              // where the tile of this step begins
-    const void *first;             // the operand itself
     int64_t step_bytes;
     int row, c;                    // of the thread's first chunk
     int ld;
-    int64_t rows_in, inner_in;     // what is there from the first tile on: rows, elements of a row
+    int rows_in, inner_in;         // what is there from the tile of this step on: rows, elements of a row
 
     __device__ __forceinline__ static int place(int row) { return TR ? swizzle<16>(row) : swizzle<4>(row); }
     __device__ __forceinline__ void begin(const void *p, int64_t ld_, int64_t first_, int64_t extent, int64_t k0, int64_t k1, int tid) {
         ld = (int)ld_;
-        first = p;
         base = (const char *)p + (TR ? k0 * ld_ + first_ : first_ * ld_ + k0) * 2;
         step_bytes = TR ? BK * ld_ * 2 : BK * 2;
-        rows_in = TR ? k1 - k0 : extent - first_;
-        inner_in = TR ? extent - first_ : k1 - k0;
+        rows_in = (int)(TR ? k1 - k0 : extent - first_);
+        inner_in = (int)(TR ? extent - first_ : k1 - k0);
         row = tid / C;
         c = (tid % C) ^ place(row);
     }
@@ -176,15 +174,15 @@ template <typename T, bool TR, int ROWS, int THREADS> struct Operand {
         }
     }
     // Any alignment, any size: through registers.  A chunk that the row's end cuts short is read as the row's last 8 elements and shifted
-    // down when it is put away, so that no load waits for another.
+    // down when it is put away.  Past the end along the summed index are zeros; across it whatever is read there does, since its
+    // results go nowhere: the last rows and chunks that are there.  So no load waits for another, and few tiles shift.
     struct Held { s16x8 v[N]; int left[N]; };
     __device__ __forceinline__ void load(Held &h) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int at = chunk(i) * 8, left = left_of(i);
-            const short *p = (const short *)base + (int64_t)(row + i * STEP) * ld + at - (8 - left);
-            h.left[i] = left;                              // (nothing to read here: the operand's first 8 elements, which are there)
-            __builtin_memcpy(&h.v[i], left ? p : (const short *)first, 16);
+            const int r = row + i * STEP, at = chunk(i) * 8, left = inner_in - at;
+            h.left[i] = TR ? (r >= rows_in ? 0 : left > 0 && left < 8 ? left : 8) : max(0, min(8, left));
+            __builtin_memcpy(&h.v[i], (const short *)base + (int64_t)min(r, rows_in - 1) * ld + min(at, inner_in - 8), 16);
         }
     }
     // rows of less than 8 elements
@@ -198,18 +196,18 @@ template <typename T, bool TR, int ROWS, int THREADS> struct Operand {
             for (int e = 0; e < 8; ++e) h.v[i][e] = e < left ? p[e] : (short)0;
         }
     }
-    __device__ __forceinline__ int left_of(int i) const {
-        return row + i * STEP < rows_in ? (int)max((int64_t)0, min((int64_t)8, inner_in - chunk(i) * 8)) : 0;
-    }
+    __device__ __forceinline__ int left_of(int i) const { return row + i * STEP < rows_in ? max(0, min(8, inner_in - chunk(i) * 8)) : 0; }
     __device__ __forceinline__ static void put(char *lds, const Held &h, int tid) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const uint64_t lo = __builtin_bit_cast(u64x2, h.v[i]).x, hi = __builtin_bit_cast(u64x2, h.v[i]).y;
-            const int by = 16 * (8 - h.left[i]);           // 0 .. 128
-            u64x2 v;
-            v.x = by >= 64 ? hi >> (by & 63) : by ? (lo >> by) | (hi << (64 - by)) : lo;
-            v.y = by >= 64 ? 0 : hi >> by;
-            if (by == 128) v.x = 0;
+            u64x2 v = __builtin_bit_cast(u64x2, h.v[i]);
+            if (__any(h.left[i] != 8)) {
+                const uint64_t lo = v.x, hi = v.y;
+                const int by = 16 * (8 - h.left[i]);       // 0 .. 128
+                v.x = by >= 64 ? hi >> (by & 63) : by ? (lo >> by) | (hi << (64 - by)) : lo;
+                v.y = by >= 64 ? 0 : hi >> by;
+                if (by == 128) v.x = 0;
+            }
             *reinterpret_cast<u64x2 *>(lds + (i * THREADS + tid) * 16) = v;
         }
     }
@@ -327,10 +325,12 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void gemm_kernel(Pro
             slot = slot + 1 == STAGES ? 0 : slot + 1;
         }
     } else {
-        // tile s + 1 in registers and tile s + 2 on its way there while tile s is used
-        typename OA::Held va[2];
-        typename OB::Held vb[2];
-        auto fetch = [&](typename OA::Held &a, typename OB::Held &b) {
+        // AHEAD tiles in registers or on their way there while one is used.  (Tiles past the last are zeros and add nothing: no turn depends
+        // on how many there are, or the compiler would wait for all loads wherever the paths meet.  Four ahead take no less time.)
+        constexpr int AHEAD = 2;
+        typename OA::Held va[AHEAD];
+        typename OB::Held vb[AHEAD];
+        auto fetch = [&](typename OA::Held &a, typename OB::Held &b) __attribute__((always_inline)) {
             if constexpr (LOADS == NARROW) {
                 oa.load_narrow(a);
                 ob.load_narrow(b);
@@ -341,20 +341,18 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void gemm_kernel(Pro
             oa.next();
             ob.next();
         };
-        auto turn = [&](int s, typename OA::Held &a, typename OB::Held &b) {
-            char *now = smem + (s & 1) * STAGE;
-            OA::put(now, a, tid);                          // (tile s - 2, which lay here, has been read: every wave is past barrier s - 1)
-            OB::put(now + A_BYTES, b, tid);
-            fetch(a, b);
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            products<T, FM, FN, A_BYTES>(now, ra, rb, acc);
-        };
-        fetch(va[0], vb[0]);
-        fetch(va[1], vb[1]);
-        for (int s = 0; s < steps; s += 2) {
-            turn(s, va[0], vb[0]);
-            if (s + 1 < steps) turn(s + 1, va[1], vb[1]);
-        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) fetch(va[u], vb[u]);
+        for (int s = 0; s < steps; s += AHEAD)
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                char *now = smem + (u & 1) * STAGE;
+                OA::put(now, va[u], tid);                  // (the tile before the last, which lay here, has been read: every wave is past the last barrier)
+                OB::put(now + A_BYTES, vb[u], tid);
+                fetch(va[u], vb[u]);
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                products<T, FM, FN, A_BYTES>(now, ra, rb, acc);
+            }
     }
     wait_lds_dma();                                        // no copy is under way any more
     __syncthreads();
@@ -501,7 +499,7 @@ struct Choice {
 //   2048 x 2048 x 2048                      -           170    143         26.5              -            49.8
 //   16384 x 4096 x 1024                     -             -      -         163               -            121
 // A step of 64 along the sum takes a 128 x 128 tile 0.6 us alone on its CU and 1.15 with another one, a 256 x 256 tile 1.2 on a few
-// CUs and 1.75 on all of them; the kernel for few rows reads 512 of the sum at a time.
+// CUs and 1.75 on all of them, half as much again through registers; the kernel for few rows reads 512 of the sum at a time.
 Choice choose(int64_t M, int64_t N, int64_t K, bool rows_ok, bool wide) {
     Choice best = {1, 1, 1, K};
     double least = 1e300;
@@ -516,7 +514,7 @@ Choice choose(int64_t M, int64_t N, int64_t K, bool rows_ok, bool wide) {
         const int64_t t = kind == 2 ? 256 : 128, tiles = ceil_div64(M, t) * ceil_div64(N, t);
         for (int s = 1; s <= 16 && (s == 1 || (steps / s >= 4 && tiles * s <= 1024)); s *= 2) {
             const int64_t all = tiles * s, at_once = kind == 2 ? 256 : all <= 256 ? 256 : 512;
-            const double step = kind == 2 ? 1.2 + 0.55 * (all < 256 ? all / 256.0 : 1.0) : all <= 256 ? 0.6 : 1.15;
+            const double step = kind == 2 ? 1.2 + 0.55 * (all < 256 ? all / 256.0 : 1.0) : (all <= 256 ? 0.6 : 1.15) * (wide ? 1.0 : 1.5);
             double us = (double)ceil_div64(all, at_once) * ((double)ceil_div64(steps, s) * step + (kind == 2 ? 9.0 : 4.5));
             if (s > 1) us += 3.0 + (double)M * (double)N * 8.0 * s / 5.0e6;
             if (us < least) least = us, best = {kind, s, 1, ceil_div64(steps, s) * 64};
