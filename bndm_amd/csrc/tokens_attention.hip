@@ -592,54 +592,49 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
     const int b = id % a.B, tile = id / a.B;
     if (tile >= tiles) return;
     const int per = a.H / a.Hk;
-    const int64_t start = start_of(a, b);
+    // (no key or query has a number above 2^29)
+    const int start = (int)max(-((int64_t)1 << 29), min((int64_t)1 << 29, start_of(a, b))), nq = (int)a.Nq;
     const int len = (int)length_of(a, b), first_key = tile * 64, key0 = first_key + kw * 32, key = key0 + (l & 31);
     const bool key_in = key < len;
 
-    // queries that see any key of this workgroup
-    int64_t i_first = 0;
-    if (a.causal) i_first = max((int64_t)0, first_key - start) / QT * QT;
-    if (first_key >= len) i_first = a.Nq;
-    const int per_head = i_first < a.Nq ? (int)((a.Nq - i_first + QT - 1) / QT) : 0;
+    // queries that see any key of this workgroup: from i_first on
+    int i_first = 0;
+    if (a.causal) i_first = max(0, first_key - start) / QT * QT;
+    if (first_key >= len) i_first = nq;
+    const int per_head = i_first < nq ? (nq - i_first + QT - 1) / QT : 0;
     int steps = per_head * per;
 
-    // the tile of queries that is copied next
+    // the tile of queries that is copied next, and the ways to the next tile and, from behind the last one, to the next head's first
     Stager<QT, CK, NW> stage_q;
     Stager<QT, CV, NW> stage_g;
     stage_q.begin(a.qn, a.D / 8, w, l);
     stage_g.begin(a.don, a.Dv / 8, w, l);
-    int g_next = 0;
-    int64_t i_next = i_first;
-    const T *q_next = nullptr, *d_next = nullptr;
-    const float *s_next = nullptr;
-    auto first_of_head = [&]() __attribute__((always_inline)) {
-        const int head = hk * per + g_next;
-        q_next = (const T *)a.q + (int64_t)b * a.qb + i_first * a.qn + (int64_t)(2 * head) * a.qh;
-        d_next = (const T *)a.dout + (int64_t)b * a.dob + i_first * a.don + (int64_t)head * a.doh;
-        // one of lse1, lse2, D1, D2 a wave.  (Queries past the end have zeros everywhere: their weight of 1 meets do = 0.)
-        s_next = (w < 2 ? a.lse : a.delta) + ((int64_t)b * 2 * a.H + 2 * head + (w & 1)) * a.Nq + i_first;
-        i_next = i_first;
-    };
+    int i_next = i_first;
+    const T *q_next = (const T *)a.q + (int64_t)b * a.qb + i_first * a.qn + (int64_t)(2 * hk * per) * a.qh;
+    const T *d_next = (const T *)a.dout + (int64_t)b * a.dob + i_first * a.don + (int64_t)(hk * per) * a.doh;
+    // one of lse1, lse2, D1, D2 a wave.  (Queries past the end have zeros everywhere: their weight of 1 meets do = 0.)
+    const float *s_next = (w < 2 ? a.lse : a.delta) + ((int64_t)b * 2 * a.H + 2 * (hk * per) + (w & 1)) * a.Nq + i_first;
+    const int64_t q_step = QT * a.qn, d_step = QT * a.don;
+    const int64_t q_turn = 2 * a.qh - per_head * q_step, d_turn = a.doh - per_head * d_step, s_turn = 2 * a.Nq - per_head * QT;
     auto fetch = [&](char *to) __attribute__((always_inline)) {
-        const int in = (int)min((int64_t)QT, a.Nq - i_next);
+        const int in = min(QT, nq - i_next);
         stage_q.copy(to, q_next, in, w);
         stage_q.copy(to + Q_BYTES, q_next + a.qh, in, w);
         stage_g.copy(to + 2 * Q_BYTES, d_next, in, w);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(uniform_rsrc(s_next, kAnywhere), (lds_ptr_t)(to + 2 * Q_BYTES + G_BYTES + w * QT * 4), 4,
                                                  l < in ? (uint32_t)l * 4u : kNowhere, 0, 0, 0);
-        q_next += QT * a.qn;
-        d_next += QT * a.don;
+        q_next += q_step;
+        d_next += d_step;
         s_next += QT;
         i_next += QT;
-        if (i_next >= a.Nq) {
-            ++g_next;
-            first_of_head();
+        if (i_next >= nq) {
+            q_next += q_turn;
+            d_next += d_turn;
+            s_next += s_turn;
+            i_next = i_first;
         }
     };
-    if (steps) {
-        first_of_head();
-        fetch(smem);
-    }
+    if (steps) fetch(smem);
 
     s16x8 kf[2][DT / 16], vf[KEYS ? DV / 16 : 1];
 #pragma unroll
@@ -674,7 +669,7 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
     const float to_log2 = a.scale * kLog2e;
 
     int g = 0;
-    int64_t i0 = i_first;
+    int i0 = i_first;
     // (made uniform, and thereby waited for, where it is read: a wait for it later on would be one for the copies as well)
     auto lam_of_head = [&](int head) {
         const float x = lam_of<T>(a, head);
@@ -687,7 +682,7 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
         const char *gs = now + 2 * Q_BYTES;
         const float *stats = reinterpret_cast<const float *>(gs + G_BYTES) + 32 * qw + 4 * h32;
         // the last key that the first of these queries sees (clamped: only its place among the keys counts)
-        const int last0 = a.causal ? (int)max((int64_t)-64, min((int64_t)1 << 30, start + i0 + 32 * qw)) : 1 << 30;
+        const int last0 = a.causal ? max(-64, start + i0 + 32 * qw) : 1 << 30;
         const int last = last0 + 4 * h32;
         // some pair is hidden, or some row sees one key only
         const bool masked = key0 + 32 > len || key0 + 31 > last0 || len == 1 || last0 <= 0;
@@ -741,14 +736,16 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
                 if constexpr (KEYS) s[m][r] = p[m][r] * (dp[0][r] - de[m][r / 4][r % 4]);
             }
         if (masked) {
+            const int beyond = key < len ? key - last : 1 << 30;
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
+            for (int r = 0; r < 16; ++r) {                  // query tile_row(r, 0) of the half sees keys up to last + that
+                const bool hidden = beyond > tile_row(r, 0), only = -last == tile_row(r, 0) || len == 1;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    // query tile_row(r, 0) of the half sees keys up to last + that
-                    if (key >= len || key - last > tile_row(r, 0)) p[m][r] = s[m][r] = 0.f;
-                    if (len == 1 || -last == tile_row(r, 0)) s[m][r] = 0.f;
+                for (int m = 0; m < 2; ++m) {
+                    if (hidden) p[m][r] = 0.f;
+                    if (hidden || only) s[m][r] = 0.f;
                 }
+            }
         }
         if constexpr (KEYS)
 #pragma unroll
@@ -773,10 +770,10 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
             }
         }
         i0 += QT;
-        if (i0 >= a.Nq && --steps) {
+        if (--steps && i0 >= nq) {
             i0 = i_first;
             lam = lam_of_head(hk * per + ++g);
-        } else if (i0 < a.Nq) --steps;
+        }
     };
     __builtin_amdgcn_s_waitcnt(0);                          // (what came before the loop is there, or its turns would wait for as much)
     while (steps > 0) {
@@ -917,7 +914,7 @@ template <typename T, int DT> int backward(const Args &a, hipStream_t stream) {
 
 int check(const char *what, const bndm_attention_shape *s) {
     TOKENS_REQUIRE(s, "%s: NULL shape", what);
-    TOKENS_REQUIRE(s->B >= 0 && s->Nq >= 0 && s->Nk >= 0 && s->B <= (1 << 20) && s->Nq <= (1 << 30) && s->Nk <= (1 << 30), "%s: sizes", what);
+    TOKENS_REQUIRE(s->B >= 0 && s->Nq >= 0 && s->Nk >= 0 && s->B <= (1 << 20) && s->Nq <= (1 << 29) && s->Nk <= (1 << 29), "%s: sizes", what);
     TOKENS_REQUIRE(s->H >= 1 && s->Hk >= 1 && s->H % s->Hk == 0 && s->H <= 4096, "%s: %d heads over %d key heads", what, s->H, s->Hk);
     TOKENS_REQUIRE(s->D >= 8 && s->D <= 128 && s->D % 8 == 0, "%s: head size %d: a multiple of 8 up to 128", what, s->D);
     TOKENS_REQUIRE(s->Dv >= 8 && s->Dv <= 256 && s->Dv % 8 == 0, "%s: value size %d: a multiple of 8 up to 256", what, s->Dv);
@@ -968,7 +965,7 @@ extern "C" int bndm_tokens_attention(const bndm_attention_shape *s, const void *
     const size_t need = bndm_tokens_attention_workspace_bytes(s);
     TOKENS_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need),
                    "bndm_tokens_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-    TOKENS_REQUIRE(p.blocks < (1 << 24), "bndm_tokens_attention: more tiles than a launch takes");
+    TOKENS_REQUIRE(p.blocks < (1 << 23), "bndm_tokens_attention: more tiles than a launch takes");
     Args a = args_of(s, q, k, v, lam, q_start, kv_lengths);
     a.o = o, a.o2 = o2, a.lse = lse;
     a.heads_per_row = p.heads_per_row, a.splits = p.splits, a.split_keys = p.split_keys;

@@ -122,32 +122,34 @@ int piece_of(const RotarySide &s, int run, int size) {
 }
 
 template <typename T, int V, bool WIDE, bool I>
-void launch(const RotarySide &q, const RotarySide &k, const void *positions, int type, const int64_t *ps, int64_t B, int64_t N, int D,
+int launch(const RotarySide &q, const RotarySide &k, const void *positions, int type, const int64_t *ps, int64_t B, int64_t N, int D,
             int sign, const RotaryTable &table, hipStream_t stream) {
     // tokens of a workgroup: about 8 pieces a thread, while 1024 workgroups (four for each CU) remain; 8 KB of LDS at most
     const int64_t tokens = B * N;
     const int pieces = (q.heads + k.heads) * (I ? D / V : D / 2 / V);
     int per = (int)min((int64_t)(1024 / (D / 2)), max((int64_t)1, (int64_t)8 * THREADS / max(1, pieces)));
     per = (int)max((int64_t)1, min((int64_t)per, tokens / 1024));
-    hipLaunchKernelGGL((rotary_kernel<T, V, WIDE, I>), dim3((unsigned)ceil_div64(tokens, per)), dim3(THREADS), per * (D / 2) * sizeof(float2), stream,
+    const int64_t blocks = ceil_div64(tokens, per);
+    TOKENS_REQUIRE(blocks < (1 << 24), "bndm_tokens_rotary: more tokens than a launch takes");
+    hipLaunchKernelGGL((rotary_kernel<T, V, WIDE, I>), dim3((unsigned)blocks), dim3(THREADS), per * (D / 2) * sizeof(float2), stream,
                        q, k, positions, type, ps[0], ps[1], ps[2], tokens, N, D, per, sign ? -1.0f : 1.0f, table);
+    return tokens_launch_status("rotary");
 }
 
 template <typename T>
-void dispatch(const RotarySide &q, const RotarySide &k, const void *positions, int type, const int64_t *ps, int64_t B, int64_t N, int D,
+int dispatch(const RotarySide &q, const RotarySide &k, const void *positions, int type, const int64_t *ps, int64_t B, int64_t N, int D,
               int interleaved, int inverse, const RotaryTable &table, hipStream_t stream) {
     const int run = interleaved ? D : D / 2;
     int v = piece_of(q, run, sizeof(T));
     if (k.heads) v = min(v, piece_of(k, run, sizeof(T)));
     if (interleaved) {
-        if (v * sizeof(T) == 16) launch<T, 16 / sizeof(T), true, true>(q, k, positions, type, ps, B, N, D, inverse, table, stream);
-        else if (v * sizeof(T) == 8) launch<T, 8 / sizeof(T), true, true>(q, k, positions, type, ps, B, N, D, inverse, table, stream);
-        else launch<T, 2, false, true>(q, k, positions, type, ps, B, N, D, inverse, table, stream);
-    } else {
-        if (v * sizeof(T) == 16) launch<T, 16 / sizeof(T), true, false>(q, k, positions, type, ps, B, N, D, inverse, table, stream);
-        else if (v * sizeof(T) == 8) launch<T, 8 / sizeof(T), true, false>(q, k, positions, type, ps, B, N, D, inverse, table, stream);
-        else launch<T, 1, false, false>(q, k, positions, type, ps, B, N, D, inverse, table, stream);
+        if (v * sizeof(T) == 16) return launch<T, 16 / sizeof(T), true, true>(q, k, positions, type, ps, B, N, D, inverse, table, stream);
+        if (v * sizeof(T) == 8) return launch<T, 8 / sizeof(T), true, true>(q, k, positions, type, ps, B, N, D, inverse, table, stream);
+        return launch<T, 2, false, true>(q, k, positions, type, ps, B, N, D, inverse, table, stream);
     }
+    if (v * sizeof(T) == 16) return launch<T, 16 / sizeof(T), true, false>(q, k, positions, type, ps, B, N, D, inverse, table, stream);
+    if (v * sizeof(T) == 8) return launch<T, 8 / sizeof(T), true, false>(q, k, positions, type, ps, B, N, D, inverse, table, stream);
+    return launch<T, 1, false, false>(q, k, positions, type, ps, B, N, D, inverse, table, stream);
 }
 
 }  // namespace
@@ -185,8 +187,7 @@ extern "C" int bndm_tokens_rotary(const void *q, const int64_t q_strides[3], voi
     RotarySide sq = {q, q_out, q_heads, 0, 0, 0}, sk = {k, k_out, k_heads, 0, 0, 0};
     if (q_heads) sq.sb = q_strides[0], sq.sn = q_strides[1], sq.sh = q_strides[2];
     if (k_heads) sk.sb = k_strides[0], sk.sn = k_strides[1], sk.sh = k_strides[2];
-    if (dtype == BNDM_DTYPE_F16) dispatch<f16>(sq, sk, positions, position_type, position_strides, B, N, D, interleaved, inverse, table, (hipStream_t)stream);
-    else if (dtype == BNDM_DTYPE_BF16) dispatch<bf16>(sq, sk, positions, position_type, position_strides, B, N, D, interleaved, inverse, table, (hipStream_t)stream);
-    else dispatch<float>(sq, sk, positions, position_type, position_strides, B, N, D, interleaved, inverse, table, (hipStream_t)stream);
-    return tokens_launch_status("rotary");
+    if (dtype == BNDM_DTYPE_F16) return dispatch<f16>(sq, sk, positions, position_type, position_strides, B, N, D, interleaved, inverse, table, (hipStream_t)stream);
+    if (dtype == BNDM_DTYPE_BF16) return dispatch<bf16>(sq, sk, positions, position_type, position_strides, B, N, D, interleaved, inverse, table, (hipStream_t)stream);
+    return dispatch<float>(sq, sk, positions, position_type, position_strides, B, N, D, interleaved, inverse, table, (hipStream_t)stream);
 }

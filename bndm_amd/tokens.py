@@ -232,7 +232,7 @@ def _aligned(t):
     b, n, h, d = t.shape
     sb, sn, sh, sd = t.stride()
     sb, sn, sh = 0 if b == 1 else sb, 0 if n == 1 else sn, 0 if h == 1 else sh
-    if (sd == 1 or d == 1) and not (t.data_ptr() % 16 or sb % 8 or sn % 8 or sh % 8):
+    if (sd == 1 or d == 1) and not (t.data_ptr() % 16 or sb % 8 or sn % 8 or sh % 8 or sn > 1 << 23):
         return t, (sb, sn, sh)
     t = t.contiguous()
     if t.data_ptr() % 16 or d % 8:                          # (a head size that the kernels refuse: any strides will do)
@@ -314,7 +314,7 @@ def differential_attention(q, k, v, lam, causal=False, q_start=None, kv_lengths=
     """
     dtype = _type_of("differential_attention(q)", q, (torch.float16, torch.bfloat16))
     if any(t.dim() != 4 for t in (q, k, v)) or q.shape[2] % 2 or k.shape[2] != 2 * v.shape[2] or k.shape[:2] != v.shape[:2] or \
-            q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3] or v.shape[2] < 1 or q.shape[2] < 2 or (q.shape[2] // 2) % v.shape[2]:
+            q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3] or v.shape[2] < 1 or q.shape[2] < 2 or q.shape[3] < 1 or (q.shape[2] // 2) % v.shape[2]:
         raise ValueError(f"differential_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: "
                          "[B, Nq, 2 H, D], [B, Nk, 2 Hk, D], [B, Nk, Hk, Dv] with H a multiple of Hk")
     if lam.shape != (q.shape[2] // 2,) or lam.device != q.device or lam.dtype not in (q.dtype, torch.float32):

@@ -25,6 +25,8 @@ def normal(seed, *shape, dtype=F16, std=1.0):
 # ---------------------------------------------------------------------------------------------- linear
 SIZES = [(1, 8, 8), (1, 512, 1000), (5, 64, 24), (64, 512, 512), (130, 72, 136), (37, 515, 77), (3, 1, 1), (300, 200, 264), (129, 128, 1), (1000, 40, 130),
          (65, 640, 24), (33, 523, 40), (200, 5, 70), (200, 70, 3), (7, 131, 140), (100, 3, 5), (100, 8192, 72), (100, 4099, 70), (8200, 40, 72),                # long sums, in parts
+         (9000, 5, 200), (5003, 139, 300), (1003, 4099, 300),                                        # many rows, unaligned
+         (300, 600, 520), (1003, 515, 515), (2, 4100, 2056), (40, 1030, 9000),                         # few rows at a time, 16, 32 and 64 of them
          (4104, 136, 2312), (4104, 2312, 136), (136, 2312, 4104)]                                      # large tiles, with edges
 
 
@@ -220,14 +222,15 @@ def test_attention_does_not_read_past_a_sequence(T):
 
 
 def test_attention_takes_tensors_as_they_lie(T):
-    """slices of a packed projection, heads before tokens, odd starts and strides, repeated key heads; gradients that arrive strided"""
+    """slices of a packed projection, tokens 2^23 elements apart, heads before tokens, odd starts and strides, repeated key heads; gradients that arrive strided"""
     b, n, h, hk, d = 2, 70, 4, 2, 32
     packed = normal(1, b, n, 2 * (h + hk) * d + 2 * hk * d + 8).cuda()
     split = lambda off: [t.unflatten(-1, s) for t, s in zip(packed[..., off : off + 2 * (h + 2 * hk) * d].split([2 * h * d, 2 * hk * d, 2 * hk * d], -1),
                                                            ((2 * h, d), (2 * hk, d), (hk, 2 * d)))]
     lam = torch.rand(h, generator=torch.Generator().manual_seed(4)).to(F16).cuda()
     base = split(0)
-    cases = [base, split(3), [t.transpose(1, 2).contiguous().transpose(1, 2) for t in base],
+    far = torch.zeros(2, n, (1 << 23) + 8, dtype=F16, device="cuda")[:, :, : 2 * h * d].unflatten(-1, (2 * h, d)).copy_(base[0])
+    cases = [base, split(3), [far, *base[1:]], [t.transpose(1, 2).contiguous().transpose(1, 2) for t in base],
              [base[0], base[1][:, :, :2].repeat(1, 1, 2, 1), base[2][:, :, :1].expand(b, n, hk, 2 * d)]]
     grad = normal(6, b, h, 2 * d, n).cuda().permute(0, 3, 1, 2)
     seen = R.visible(n, n, None, True, None, b)
@@ -442,7 +445,7 @@ def test_refusals(T):
         (lambda: A(q, k, v, lam, q_start=lengths), ValueError), (lambda: A(q, k, v, lam, kv_lengths=lengths[:1]), ValueError),
         (lambda: A(q, k, v, lam, kv_lengths=lengths.float()), ValueError), (lambda: A(q, k, v, lam, kv_lengths=lengths.cpu()), ValueError),
         (lambda: A(q, k, v, lam, scale=-1.0), NotImplementedError), (lambda: A(q, k, v, lam, scale=0.0), NotImplementedError),
-        (lambda: A(q[..., :12], k[..., :12], v, lam), NotImplementedError), (lambda: A(q, k, v[..., :12], lam), NotImplementedError),
+        (lambda: A(q[..., :12], k[..., :12], v, lam), NotImplementedError), (lambda: A(q, k, v[..., :12], lam), NotImplementedError), (lambda: A(q[..., :0], k[..., :0], v, lam), ValueError),
     ]:
         with pytest.raises(error):
             call()

@@ -2,6 +2,8 @@
 import ctypes as C
 import os
 import re
+import struct
+import subprocess
 
 import pytest
 import torch
@@ -111,3 +113,35 @@ def test_attention_refusals(lib):
                          (dict(ds=S(512, 512, 4)), "stride"), (dict(size=need - 1), "workspace")]:
         refused(lib, lib.bndm_tokens_attention_backward(shape(), *{**good, **change}.values(), None), word)
     refused(lib, lib.bndm_tokens_attention_backward(shape(Nq=0), *good.values(), None), "no queries")
+
+
+READELF = "/opt/rocm/llvm/bin/llvm-readelf"
+
+
+@pytest.mark.skipif(not os.path.exists(READELF), reason="needs the ROCm LLVM tools")
+def test_no_kernel_spills(lib, tmp_path):
+    """Every kernel keeps what it works on in registers: one that does not is many times slower, and nothing else would tell."""
+    from bndm_amd import _lib
+    data, magic = open(_lib.TOKENS_LIB_PATH, "rb").read(), b"__CLANG_OFFLOAD_BUNDLE__"
+    kernels, at = 0, data.find(magic)
+    while at >= 0:
+        pos = at + len(magic)
+        count, = struct.unpack_from("<Q", data, pos)
+        pos += 8
+        for _ in range(count):
+            offset, size, length = struct.unpack_from("<QQQ", data, pos)
+            name = data[pos + 24 : pos + 24 + length].decode()
+            pos += 24 + length
+            if not name.startswith("host"):
+                assert name.endswith("gfx950"), name
+                code = tmp_path / "code.o"
+                code.write_bytes(data[at + offset : at + offset + size])
+                notes = subprocess.run([READELF, "--notes", str(code)], capture_output=True, text=True, check=True).stdout
+                fields = re.findall(r"\.(name|vgpr_spill_count|symbol):\s+(\S+)", notes)
+                spills = [int(v) for k, v in fields if k == "vgpr_spill_count"]
+                symbols = [v for k, v in fields if k == "symbol"]
+                assert len(spills) == len(symbols)
+                assert [s for s, n in zip(symbols, spills) if n] == []
+                kernels += len(symbols)
+        at = data.find(magic, pos)
+    assert kernels > 50
