@@ -12,6 +12,8 @@
 //
 // Statistics, sums and gradients' sums are 32 bits; weights (P, dS) are rounded to the inputs' type for the matrix units, as products
 // of 16-bit operands are what those take.
+#include <type_traits>
+
 #include "tokens_common.hpp"
 #include <cmath>
 
@@ -431,6 +433,7 @@ template <typename T> __global__ __launch_bounds__(512) void attention_join_kern
 
 // ---------------------------------------------------------------------------------------------- gradients of the queries
 // As the forward pass: a lane holds one query, dS^T is at once the right operand of  dq^T += k^T dS^T.  Also D1, D2 for the next kernel.
+constexpr int FEW = 512;
 template <typename T, int DT, int KT>
 __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 128 ? 1 : 2, DT == 128 ? 1 : 2))) void attention_dq_kernel(Args a) {
     constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT, NW = 4;
@@ -462,8 +465,11 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
             qf[m][s] = load8(p + c * 8, row_in && c * 8 < a.D);
         }
     }
-    // D2 = do . o2, D1 = do . (o + lam o2)
+    // D2 = do . o2, D1 = do . (o + lam o2), as near as rounded outputs and weights give them: 2^-9 of theirs, which few keys would show.
+    // Up to FEW keys they are formed anew in a pass of its own below; behind more keys, what they are off is found along the way, as
+    // sum_j dS_ij = 0, and the gradients of keys and lam take them without it.
     const float lam = lam_of<T>(a, head);
+    const bool few = j_end <= FEW;
     float delta[2] = {0.f, 0.f};
     {
         const T *g = (const T *)a.dout + (int64_t)b * a.dob + i * a.don + (int64_t)head * a.doh;
@@ -471,34 +477,30 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
 #pragma unroll
         for (int s = 0; s < DV / 16; ++s) {
             const int c = 2 * s + h32;
-            const bool in = row_in && c * 8 < a.Dv;
-            gf[s] = load8(g + c * 8, in);
-            const s16x8 o = load8((const T *)a.o + at + c * 8, in), o2 = load8((const T *)a.o2 + at + c * 8, in);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const short gs = gf[s][e], os = o[e], ps = o2[e];
-                const float ge = widen<T>(gs);
-                delta[0] += ge * widen<T>(os);
-                delta[1] += ge * widen<T>(ps);
-            }
+            gf[s] = load8(g + c * 8, row_in && c * 8 < a.Dv);
         }
-        delta[0] = both_halves_sum(delta[0]);
-        delta[1] = both_halves_sum(delta[1]);
-        delta[0] += lam * delta[1];
-    }
-    float lse[2];
+        if (!few) {
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        const int64_t at = ((int64_t)b * 2 * a.H + 2 * head + m) * a.Nq + i;
-        lse[m] = row_in ? a.lse[at] : INFINITY;
-        if (row_in && h32 == 0) a.delta[at] = delta[m];
-    }
-    {
-        float sum = delta[1];                               // (0 for rows past the end)
+            for (int s = 0; s < DV / 16; ++s) {
+                const int c = 2 * s + h32;
+                const bool in = row_in && c * 8 < a.Dv;
+                const s16x8 o = load8((const T *)a.o + at + c * 8, in), o2 = load8((const T *)a.o2 + at + c * 8, in);
 #pragma unroll
-        for (int x = 1; x < 32; x *= 2) sum += __shfl_xor(sum, x);
-        if (l == 0) a.d2_sums[(((int64_t)head * a.B + b) * tiles + tile) * NW + w] = sum;
+                for (int e = 0; e < 8; ++e) {
+                    const short gs = gf[s][e], os = o[e], ps = o2[e];
+                    const float ge = widen<T>(gs);
+                    delta[0] += ge * widen<T>(os);
+                    delta[1] += ge * widen<T>(ps);
+                }
+            }
+            delta[0] = both_halves_sum(delta[0]);
+            delta[1] = both_halves_sum(delta[1]);
+            delta[0] += lam * delta[1];
+        }
     }
+    float lse[2], off[2] = {0.f, 0.f};
+#pragma unroll
+    for (int m = 0; m < 2; ++m) lse[m] = row_in ? a.lse[((int64_t)b * 2 * a.H + 2 * head + m) * a.Nq + i] : INFINITY;
 
     f32x16 acc[2][DT / 32];
     clear(acc[0]);
@@ -522,7 +524,9 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
     values.begin(l);
     key_columns.begin(l);
     if (0 < j_end) fetch(smem, 0);
-    auto turn = [&](char *__restrict__ ahead, const char *__restrict__ now, int j) __attribute__((always_inline)) {
+    // FIRST: D1, D2 only
+    auto turn = [&](auto first, char *__restrict__ ahead, const char *__restrict__ now, int j) __attribute__((always_inline)) {
+        constexpr bool FIRST = decltype(first)::value;
         tile_there<NW>();
         if (j + KT < j_end) fetch(ahead, j + KT);
 #pragma unroll
@@ -540,28 +544,56 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
                 for (int d = 0; d < DT / 16; ++d) s[0] = mfma32<T>(keys.read(now + m * K_BYTES, t, d), qf[m][d], s[0]);
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    s[0][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], to_log2, -lse[m])) * (dp[0][r] - delta[m]);
+                    s[0][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], to_log2, -lse[m])) * (FIRST ? dp[0][r] : dp[0][r] - delta[m]);
                 if (masked) {                               // (a row that sees one key has weight 1 there whatever its score)
-                    const int n = sees == 1 ? 0 : sees - j - 32 * t - 4 * h32;
+                    const int n = !FIRST && sees == 1 ? 0 : sees - j - 32 * t - 4 * h32;
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
                         if (tile_row(r, 0) >= n) s[0][r] = 0.f;
                 }
+                float sum = 0.f;
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const s16x8 ds = as_operand<T>(s[0], x);
+                for (int r = 0; r < 16; ++r) sum += s[0][r];
+                off[m] += sum;
+                if constexpr (!FIRST)
 #pragma unroll
-                    for (int d = 0; d < DT / 32; ++d) acc[m][d] = mfma32<T>(key_columns.read(now + m * K_BYTES, 32 * t + 16 * x, d), ds, acc[m][d]);
-                }
+                    for (int x = 0; x < 2; ++x) {
+                        const s16x8 ds = as_operand<T>(s[0], x);
+#pragma unroll
+                        for (int d = 0; d < DT / 32; ++d) acc[m][d] = mfma32<T>(key_columns.read(now + m * K_BYTES, 32 * t + 16 * x, d), ds, acc[m][d]);
+                    }
             }
         }
     };
-    __builtin_amdgcn_s_waitcnt(0);                          // (what came before the loop is there, or its turns would wait for as much)
-    for (int j = 0; j < j_end; j += 2 * KT) {
-        turn(smem + STAGE, smem, j);
-        if (j + KT < j_end) turn(smem, smem + STAGE, j + KT);
+    auto pass = [&](auto first) __attribute__((always_inline)) {
+        __builtin_amdgcn_s_waitcnt(0);                      // (what came before the loop is there, or its turns would wait for as much)
+        for (int j = 0; j < j_end; j += 2 * KT) {
+            turn(first, smem + STAGE, smem, j);
+            if (j + KT < j_end) turn(first, smem, smem + STAGE, j + KT);
+        }
+        tile_there<NW>();
+    };
+    if (few) {
+        pass(std::true_type());
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            delta[m] = both_halves_sum(off[m]);
+            off[m] = 0.f;
+        }
+        if (0 < j_end) fetch(smem, 0);
     }
-    tile_there<NW>();
+    pass(std::false_type());
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        delta[m] += both_halves_sum(off[m]);
+        if (row_in && h32 == 0) a.delta[((int64_t)b * 2 * a.H + 2 * head + m) * a.Nq + i] = delta[m];
+    }
+    {
+        float sum = delta[1];                               // (0 for rows past the end)
+#pragma unroll
+        for (int x = 1; x < 32; x *= 2) sum += __shfl_xor(sum, x);
+        if (l == 0) a.d2_sums[(((int64_t)head * a.B + b) * tiles + tile) * NW + w] = sum;
+    }
     char *own = smem + w * 32 * DT * 2;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {

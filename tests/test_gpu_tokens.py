@@ -256,6 +256,26 @@ def test_attention_scores_far_from_zero(T):
             R.assert_within(o, *R.attention(q2, k2, v, lam, seen, scale=scale)["o"], f"scale {scale}")
 
 
+@pytest.mark.parametrize("b,nq,nk", [(2, 8, 8), (1, 1, 600), (3, 5, 513), (1, 130, 1300), (2, 1, 1)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_gradient_of_lam_in_32_bits(T, b, nq, nk, dtype):
+    """dlam adds up whole rows' do . o2, which cancel: it comes from 32-bit sums, not from the rounded output.  Bound: dP and scores are sums
+    of Dv and D products in 32 bits, a score's error times its weight is the weight's; 64 more roundings for exponentials and sums."""
+    h, d, dv = 2, 16, 16
+    q, k, v = normal(1, b, nq, 2 * h, d, dtype=dtype), normal(2, b, nk, 2 * h, d, dtype=dtype), normal(3, b, nk, h, dv, dtype=dtype)
+    grad, lam = normal(4, b, nq, h, dv, dtype=dtype), torch.tensor([0.3, 0.8])
+    leaf = lam.cuda().requires_grad_()
+    o = T.differential_attention(q.cuda(), k.cuda(), v.cuda(), leaf)
+    got, = torch.autograd.grad(o, leaf, grad.cuda())
+    q2, k2 = (t.double().transpose(1, 2)[:, 1::2] for t in (q, k))
+    v, grad = (t.double().transpose(1, 2) for t in (v, grad))
+    p = (q2 @ k2.transpose(-1, -2) * d ** -0.5).softmax(-1)
+    want = -(p * (grad @ v.transpose(-1, -2))).sum((0, 2, 3))
+    size = (p * (grad.abs() @ v.abs().transpose(-1, -2))).sum((0, 2, 3))
+    score = float((q2.abs() @ k2.abs().transpose(-1, -2)).max()) * d ** -0.5
+    assert ((got.cpu().double() - want).abs() <= (dv + d * score + 64) * 2.0 ** -24 * size).all(), (got.cpu(), want, size)
+
+
 def test_attention_gradients_against_differences(T):
     """a step along each gradient changes the loss by its squared length"""
     q, k, v, lam, dout = attention_inputs(2, 24, 40, 2, 1, 32, 64, BF16)
