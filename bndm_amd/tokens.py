@@ -12,31 +12,33 @@ beside their results is allocated through torch for the one call, so they can be
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
 
-_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_HALVES = {torch.float16: 0, torch.bfloat16: 1}
+_FLOATS = {**_HALVES, torch.float32: 2}
 _ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2}
 _POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 _Strides = C.c_int64 * 3
 
 
-# the handle of a device's current stream: what torch.cuda.current_stream(index).cuda_stream is, without making the Stream (2.6 us, more
-# than some of these kernels take)
+# Small calls are bound by what happens here, so it is kept short.  A device's current stream and the current device are asked for
+# without making a Stream (2.6 us) or checking that there is a device (the tensors are on one).
 _stream_of = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
     lambda index: torch.cuda.current_stream(index).cuda_stream
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 
 
-def _launch(fn, what, device, *args):
-    """fn(*args, stream) on the current stream of ``device``."""
-    index = device.index
-    if index == torch.cuda.current_device():
+def _launch(fn, what, index, *args):
+    """fn(*args, stream) on the current stream of device ``index``."""
+    if index == _current_device():
         rc = fn(*args, _stream_of(index))
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             rc = fn(*args, _stream_of(index))
     if rc:
         _lib.check_tokens(rc, what)
@@ -46,19 +48,21 @@ def _ptr(t):
     return 0 if t is None else t.data_ptr()
 
 
-def _same(what, first, **others):
-    """The tensors have the first one's type and device."""
-    dtype, device = first.dtype, first.device
-    for name, t in others.items():
-        if t is not None and (t.dtype != dtype or t.device != device):
+def _same(what, first, others):
+    """The tensors (pairs of name and tensor or None) have the first one's type and device."""
+    dtype, index = first.dtype, first.get_device()
+    for name, t in others:
+        if t is not None and (t.dtype is not dtype or t.get_device() != index):
             raise ValueError(f"{what}: {name} is {t.dtype} on {t.device}, not {first.dtype} on {first.device}")
 
 
 def _type_of(what, t, types):
-    _lib.require_gpu(t, what)
-    if t.dtype not in types:
+    if not t.is_cuda:
+        _lib.require_gpu(t, what)
+    dtype = types.get(t.dtype)
+    if dtype is None:
         raise TypeError(f"{what}: {t.dtype} is not one of {', '.join(str(x) for x in types)}")
-    return _DTYPES[t.dtype]
+    return dtype
 
 
 def _recording(*tensors):
@@ -71,34 +75,36 @@ def _recording(*tensors):
 
 # ---------------------------------------------------------------------------------------------- linear
 def _rows(t, width):
-    """``t`` as rows of ``width`` next to each other's elements, and the distance of two rows."""
+    """``t`` as rows of ``width`` next to each other's elements, their number, and the distance of two rows."""
     if t.dim() != 2:
         t = t.reshape(-1, width)
-    if width > 1 and t.stride(1) != 1:
+    step, inner = t.stride()
+    if inner != 1 and width > 1:
         t = t.contiguous()
-    return t, t.stride(0) if t.shape[0] > 1 else width
+        step = width
+    m = t.shape[0]
+    return t, m, step if m > 1 else width
 
 
 def _linear_forward(x, weight, bias, residual, act, dtype, keep):
     n, k = weight.shape
-    rows, ldx = _rows(x, k)
-    m = rows.shape[0]
-    y = x.new_empty(x.shape[:-1] + (n,))
+    rows, m, ldx = _rows(x, k)
+    y = x.new_empty((*x.shape[:-1], n) if x.dim() != 2 else (m, n))
     z = x.new_empty((m, n)) if keep and act else None
-    res, ldr = _rows(residual, n) if residual is not None else (None, 0)
+    res, _, ldr = _rows(residual, n) if residual is not None else (None, 0, 0)
     if m:
         lib = _lib.load_tokens()
         need = lib.bndm_tokens_linear_workspace_bytes(m, n, k)
-        work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-        _launch(lib.bndm_tokens_linear, "linear", x.device, rows.data_ptr(), ldx, weight.data_ptr(), _ptr(bias), _ptr(res), ldr, y.data_ptr(),
-                _ptr(z), m, n, k, act, dtype, _ptr(work), need)
+        work = x.new_empty(need, dtype=torch.uint8) if need else None
+        _launch(lib.bndm_tokens_linear, "linear", x.get_device(), rows.data_ptr(), ldx, weight.data_ptr(), _ptr(bias), _ptr(res), ldr,
+                y.data_ptr(), _ptr(z), m, n, k, act, dtype, _ptr(work), need)
     return y, z
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, dtype):
-        y, z = _linear_forward(x, weight, bias, residual, act, dtype, any(ctx.needs_input_grad[:3]))
+        y, z = _linear_forward(x, weight, bias, residual, act, dtype, True in ctx.needs_input_grad[:3])
         ctx.act, ctx.dtype = act, dtype
         ctx.save_for_backward(x, weight, z)
         return y
@@ -109,18 +115,17 @@ class _Linear(torch.autograd.Function):
         x, weight, z = ctx.saved_tensors
         n, k = weight.shape
         want_x, want_w, want_b, want_r = ctx.needs_input_grad[:4]
-        rows, ldx = _rows(x, k)
-        m = rows.shape[0]
-        make = torch.empty if m else torch.zeros
-        dx = make(x.shape, dtype=x.dtype, device=x.device) if want_x else None
-        dw = make(weight.shape, dtype=x.dtype, device=x.device) if want_w else None
-        db = make((n,), dtype=x.dtype, device=x.device) if want_b else None
+        rows, m, ldx = _rows(x, k)
+        make = x.new_empty if m else x.new_zeros
+        dx = make(x.shape) if want_x else None
+        dw = make((n, k)) if want_w else None
+        db = make(n) if want_b else None
         if m and (want_x or want_w or want_b):
-            grad, lddy = _rows(dy, n)
+            grad, _, lddy = _rows(dy, n)
             lib = _lib.load_tokens()
             need = lib.bndm_tokens_linear_backward_workspace_bytes(m, n, k, ctx.act, want_b)
-            work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-            _launch(lib.bndm_tokens_linear_backward, "linear backward", x.device, grad.data_ptr(), lddy, _ptr(z), rows.data_ptr(), ldx,
+            work = x.new_empty(need, dtype=torch.uint8) if need else None
+            _launch(lib.bndm_tokens_linear_backward, "linear backward", x.get_device(), grad.data_ptr(), lddy, _ptr(z), rows.data_ptr(), ldx,
                     weight.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), m, n, k, ctx.act, ctx.dtype, _ptr(work), need)
         return dx, dw, db, dy if want_r else None, None, None
 
@@ -132,50 +137,55 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     ``"gelu"`` (z Phi(z)).  Returns [..., N].  With an activation, a pass that records gradients keeps x weight^T + bias in the
     tensors' type for the backward pass.
     """
-    dtype = _type_of("linear(x)", x, (torch.float16, torch.bfloat16))
-    if activation not in _ACTIVATIONS:
+    dtype = _type_of("linear(x)", x, _HALVES)
+    act = _ACTIVATIONS.get(activation)
+    if act is None:
         raise NotImplementedError(f"linear: activation {activation!r}: None, 'silu' or 'gelu'")
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
-        raise ValueError(f"linear: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not go together")
-    n = weight.shape[0]
-    if bias is not None and bias.shape != (n,):
-        raise ValueError(f"linear: bias {tuple(bias.shape)} is not ({n},)")
-    if residual is not None and residual.shape != x.shape[:-1] + (n,):
-        raise ValueError(f"linear: residual {tuple(residual.shape)} is not {tuple(x.shape[:-1] + (n,))}")
-    _same("linear", x, weight=weight, bias=bias, residual=residual)
+    shape, of = tuple(x.shape), tuple(weight.shape)
+    if len(of) != 2 or not shape or shape[-1] != of[1] or 0 in of:
+        raise ValueError(f"linear: x {shape} and weight {of} do not go together")
+    if bias is not None and bias.shape != of[:1]:
+        raise ValueError(f"linear: bias {tuple(bias.shape)} is not ({of[0]},)")
+    if residual is not None and residual.shape != shape[:-1] + of[:1]:
+        raise ValueError(f"linear: residual {tuple(residual.shape)} is not {shape[:-1] + of[:1]}")
+    _same("linear", x, (("weight", weight), ("bias", bias), ("residual", residual)))
     weight = weight.contiguous()
-    bias = bias.contiguous() if bias is not None else None
-    act = _ACTIVATIONS[activation]
+    if bias is not None:
+        bias = bias.contiguous()
     if _recording(x, weight, bias, residual):
         return _Linear.apply(x, weight, bias, residual, act, dtype)
     return _linear_forward(x, weight, bias, residual, act, dtype, False)[0]
 
 
 # ---------------------------------------------------------------------------------------------- rotary
-def _heads_in(t):
-    """``t`` [B, N, H, D] with the elements of a head next to each other."""
-    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
+@functools.lru_cache(maxsize=64)
+def _sections_of(sections):
+    return (C.c_int * len(sections))(*sections)
 
 
 def _rotary_launch(q, k, positions, sections, base, interleaved, inverse, dtype):
     some = q if q is not None else k
     b, n, _, d = some.shape
-    out = []
-    args = []
+    strides, args, out = [], [], []
     for t in (q, k):
         if t is None:
             out.append(None)
-            args += [0, None, 0, 0]
+            strides += (0, 0, 0)
+            args.append((0, 0, 0))
             continue
-        t = _heads_in(t)
-        y = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        out.append((y, t))
-        args += [t.data_ptr(), _Strides(*t.stride()[:3]), y.data_ptr(), t.shape[2]]
-    shared = positions.dim() == 2
-    ps = _Strides(0 if shared else positions.stride(0), positions.stride(-2), positions.stride(-1))
-    _launch(_lib.load_tokens().bndm_tokens_rotary, "rotary", some.device, *args, positions.data_ptr(), ps, _POSITIONS[positions.dtype], b, n, d,
-            (C.c_int * len(sections))(*sections), len(sections), base, interleaved, inverse, dtype)
-    return tuple(None if o is None else o[0] for o in out)
+        if t.stride(3) != 1 and d != 1:
+            t = t.contiguous()
+        y = t.new_empty(t.shape)
+        out.append(y)
+        strides += t.stride()[:3]
+        args.append((t.data_ptr(), y.data_ptr(), t.shape[2], t))    # (t stays until the launch)
+    at = positions.stride()
+    strides = (C.c_int64 * 9)(*strides, 0 if len(at) == 2 else at[0], at[-2], at[-1])
+    s = C.addressof(strides)
+    _launch(_lib.load_tokens().bndm_tokens_rotary, "rotary", some.get_device(), args[0][0], s, args[0][1], args[0][2], args[1][0], s + 24,
+            args[1][1], args[1][2], positions.data_ptr(), s + 48, _POSITIONS[positions.dtype], b, n, d, _sections_of(sections), len(sections),
+            base, interleaved, inverse, dtype)
+    return out
 
 
 class _Rotary(torch.autograd.Function):
@@ -185,7 +195,7 @@ class _Rotary(torch.autograd.Function):
         ctx.how = (sections, base, interleaved, dtype)
         ctx.save_for_backward(positions)
         out = _rotary_launch(q, k, positions, sections, base, interleaved, 0, dtype)
-        return out[0] if k is None else out
+        return out[0] if k is None else tuple(out)
 
     @staticmethod
     @once_differentiable
@@ -207,23 +217,23 @@ def rotary(q, k, positions, sections, base=10000.0, interleaved=False):
     of an axis with s pairs turns by ``position * base ** (-i / s)``, an angle formed in 64 bits.  Pairs are elements (j, j + D / 2), or
     (2j, 2j + 1) with ``interleaved``.  Returns new tensors: (q', k'), or q' alone where k is None.
     """
-    dtype = _type_of("rotary(q)", q, (torch.float16, torch.bfloat16, torch.float32))
-    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
-        raise ValueError(f"rotary: q {tuple(q.shape)} and k {None if k is None else tuple(k.shape)}: [B, N, heads, D] of one B, N and D")
-    _same("rotary", q, k=k)
+    dtype = _type_of("rotary(q)", q, _FLOATS)
+    shape, other, where = tuple(q.shape), None if k is None else tuple(k.shape), tuple(positions.shape)
+    if len(shape) != 4 or (k is not None and (len(other) != 4 or other[:2] != shape[:2] or other[3] != shape[3])):
+        raise ValueError(f"rotary: q {shape} and k {other}: [B, N, heads, D] of one B, N and D")
+    _same("rotary", q, (("k", k),))
     sections = tuple(int(s) for s in sections)
-    if positions.device != q.device or positions.dtype not in _POSITIONS:
+    if positions.get_device() != q.get_device() or positions.dtype not in _POSITIONS:
         raise ValueError(f"rotary: positions are {positions.dtype} on {positions.device}: int32, int64 or float32 on {q.device}")
-    if positions.dim() not in (2, 3) or positions.shape[-2:] != (q.shape[1], len(sections)) or \
-            (positions.dim() == 3 and positions.shape[0] != q.shape[0]):
-        raise ValueError(f"rotary: positions {tuple(positions.shape)}: [N, axes] or [B, N, axes] for q {tuple(q.shape)} and {len(sections)} axes")
+    if where != (shape[1], len(sections)) and where != (shape[0], shape[1], len(sections)):
+        raise ValueError(f"rotary: positions {where}: [N, axes] or [B, N, axes] for q {shape} and {len(sections)} axes")
     if positions.requires_grad:
         raise NotImplementedError("rotary: positions have no gradient")
     base, interleaved = float(base), int(bool(interleaved))
     if _recording(q, k):
         return _Rotary.apply(q, k, positions, sections, base, interleaved, dtype)
     out = _rotary_launch(q, k, positions, sections, base, interleaved, 0, dtype)
-    return out[0] if k is None else out
+    return out[0] if k is None else tuple(out)
 
 
 # ---------------------------------------------------------------------------------------------- differential attention
@@ -231,7 +241,9 @@ def _aligned(t):
     """``t`` [B, N, H, D] as the kernels read it -- heads' elements next to each other, all else in steps of 16 bytes -- and its strides."""
     b, n, h, d = t.shape
     sb, sn, sh, sd = t.stride()
-    sb, sn, sh = 0 if b == 1 else sb, 0 if n == 1 else sn, 0 if h == 1 else sh
+    if b == 1: sb = 0
+    if n == 1: sn = 0
+    if h == 1: sh = 0
     if (sd == 1 or d == 1) and not (t.data_ptr() % 16 or sb % 8 or sn % 8 or sh % 8 or sn > 1 << 23):
         return t, (sb, sn, sh)
     t = t.contiguous()
@@ -242,15 +254,16 @@ def _aligned(t):
 
 def _attention_forward(q, k, v, lam, q_start, kv_lengths, causal, scale, dtype, keep):
     b, nq, maps, d = q.shape
+    _, nk, hk, dv = v.shape
     (q, qs), (k, ks), (v, vs) = _aligned(q), _aligned(k), _aligned(v)
-    shape = _lib.AttentionShape(b, nq, k.shape[1], maps // 2, v.shape[2], d, v.shape[3], *qs, *ks, *vs, causal, dtype, lam.dtype == torch.float32, scale)
-    o = torch.empty((b, nq, maps // 2, v.shape[3]), dtype=q.dtype, device=q.device)
-    o2 = torch.empty_like(o) if keep else None
-    lse = torch.empty((b, maps, nq), dtype=torch.float32, device=q.device) if keep else None
+    shape = _lib.AttentionShape(b, nq, nk, maps // 2, hk, d, dv, *qs, *ks, *vs, causal, dtype, lam.dtype is torch.float32, scale)
+    o = q.new_empty((b, nq, maps // 2, dv))
+    o2 = q.new_empty((b, nq, maps // 2, dv)) if keep else None
+    lse = q.new_empty((b, maps, nq), dtype=torch.float32) if keep else None
     lib = _lib.load_tokens()
     need = lib.bndm_tokens_attention_workspace_bytes(shape)
-    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _launch(lib.bndm_tokens_attention, "differential_attention", q.device, shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(),
+    work = q.new_empty(need, dtype=torch.uint8) if need else None
+    _launch(lib.bndm_tokens_attention, "differential_attention", q.get_device(), shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(),
             _ptr(q_start), _ptr(kv_lengths), o.data_ptr(), _ptr(o2), _ptr(lse), _ptr(work), need)
     return o, o2, lse
 
@@ -268,8 +281,7 @@ class _DifferentialAttention(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, lam, q_start, kv_lengths, o, o2, lse = ctx.saved_tensors
         causal, scale, dtype = ctx.how
-        new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        dq, dk, dv, dlam = new(q), new(k), new(v), new(lam)
+        dq, dk, dv, dlam = (t.new_empty(t.shape) for t in (q, k, v, lam))
         if q.shape[0] == 0 or q.shape[1] == 0:
             for t in (dq, dk, dv, dlam):
                 t.zero_()
@@ -277,11 +289,11 @@ class _DifferentialAttention(torch.autograd.Function):
             b, nq, maps, d = q.shape
             (q, qs), (k, ks), (v, vs), (dout, ds) = _aligned(q), _aligned(k), _aligned(v), _aligned(dout)
             shape = _lib.AttentionShape(b, nq, k.shape[1], maps // 2, v.shape[2], d, v.shape[3], *qs, *ks, *vs, causal, dtype,
-                                        lam.dtype == torch.float32, scale)
+                                        lam.dtype is torch.float32, scale)
             lib = _lib.load_tokens()
             need = lib.bndm_tokens_attention_backward_workspace_bytes(shape)
-            work = torch.empty(need, dtype=torch.uint8, device=q.device)
-            _launch(lib.bndm_tokens_attention_backward, "differential_attention backward", q.device, shape, q.data_ptr(), k.data_ptr(),
+            work = q.new_empty(need, dtype=torch.uint8)
+            _launch(lib.bndm_tokens_attention_backward, "differential_attention backward", q.get_device(), shape, q.data_ptr(), k.data_ptr(),
                     v.data_ptr(), lam.data_ptr(), _ptr(q_start), _ptr(kv_lengths), o.data_ptr(), o2.data_ptr(), lse.data_ptr(),
                     dout.data_ptr(), _Strides(*ds), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr(), work.data_ptr(),
                     need)
@@ -292,9 +304,9 @@ class _DifferentialAttention(torch.autograd.Function):
 def _per_sequence(what, t, q):
     if t is None:
         return None
-    if t.shape != (q.shape[0],) or t.device != q.device or t.dtype not in (torch.int32, torch.int64):
+    if t.shape != (q.shape[0],) or t.get_device() != q.get_device() or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"differential_attention: {what} is {t.dtype} {tuple(t.shape)} on {t.device}: int32 ({q.shape[0]},) on {q.device}")
-    return t.to(torch.int32).contiguous()
+    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
 
 def differential_attention(q, k, v, lam, causal=False, q_start=None, kv_lengths=None, scale=None):
@@ -312,18 +324,18 @@ def differential_attention(q, k, v, lam, causal=False, q_start=None, kv_lengths=
     With gradients, the weights and their gradients are rounded to the tensors' type between products: f16 gradients below about
     1e-5 of a score's lose digits, so scale a loss as for any f16 training.
     """
-    dtype = _type_of("differential_attention(q)", q, (torch.float16, torch.bfloat16))
-    if any(t.dim() != 4 for t in (q, k, v)) or q.shape[2] % 2 or k.shape[2] != 2 * v.shape[2] or k.shape[:2] != v.shape[:2] or \
-            q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3] or v.shape[2] < 1 or q.shape[2] < 2 or q.shape[3] < 1 or (q.shape[2] // 2) % v.shape[2]:
-        raise ValueError(f"differential_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: "
-                         "[B, Nq, 2 H, D], [B, Nk, 2 Hk, D], [B, Nk, Hk, Dv] with H a multiple of Hk")
-    if lam.shape != (q.shape[2] // 2,) or lam.device != q.device or lam.dtype not in (q.dtype, torch.float32):
-        raise ValueError(f"differential_attention: lam is {lam.dtype} {tuple(lam.shape)} on {lam.device}: {q.dtype} or float32 "
-                         f"({q.shape[2] // 2},) on {q.device}")
-    _same("differential_attention", q, k=k, v=v)
+    dtype = _type_of("differential_attention(q)", q, _HALVES)
+    qs, ks, vs = tuple(q.shape), tuple(k.shape), tuple(v.shape)
+    if len(qs) != 4 or len(ks) != 4 or len(vs) != 4 or qs[0] != ks[0] or ks[:2] != vs[:2] or qs[3] != ks[3] or qs[3] < 1 or vs[2] < 1 or \
+            ks[2] != 2 * vs[2] or qs[2] < 2 or qs[2] % ks[2]:
+        raise ValueError(f"differential_attention: q {qs}, k {ks}, v {vs}: [B, Nq, 2 H, D], [B, Nk, 2 Hk, D], [B, Nk, Hk, Dv] with H a multiple of Hk")
+    heads = qs[2] // 2
+    if lam.shape != (heads,) or lam.get_device() != q.get_device() or lam.dtype not in (q.dtype, torch.float32):
+        raise ValueError(f"differential_attention: lam is {lam.dtype} {tuple(lam.shape)} on {lam.device}: {q.dtype} or float32 ({heads},) on {q.device}")
+    _same("differential_attention", q, (("k", k), ("v", v)))
     if q_start is not None and not causal:
         raise ValueError("differential_attention: q_start says where a causal mask begins: causal is False")
-    scale = float(q.shape[3]) ** -0.5 if scale is None else float(scale)
+    scale = qs[3] ** -0.5 if scale is None else float(scale)
     lam = lam.contiguous()
     q_start, kv_lengths = _per_sequence("q_start", q_start, q), _per_sequence("kv_lengths", kv_lengths, q)
     if _recording(q, k, v, lam):
