@@ -1,9 +1,9 @@
 // Differential attention  o = (P1 - lam P2) v,  P_m = softmax(scale q_m k_m^T), and its gradients, on the matrix units.
 //
-// Forward: one pass over the keys for both maps at once, with a running maximum and sum each; the scores are formed TRANSPOSED
+// Forward: one pass over the keys, with a running maximum and sum for each map, which are a wave's each; the scores are formed TRANSPOSED
 // (keys down, queries across), so a lane holds one query: maxima and sums are over its own registers, its running statistics are
 // scalars to it, and the weights of a step are at once the right operand of  o^T += v^T P^T.  v^T comes out of LDS by transposing
-// reads, each fragment used for both maps.  For few queries the keys are split over workgroups and the parts joined by a second kernel.
+// reads.  For few queries the keys are split over workgroups and the parts joined by a second kernel.
 //
 // Backward, with dP = do v^T (the same for both maps), D_m = rowsum(P_m dP) = do . o_m:
 //   dS1 = P1 (dP - D1),  dS2 = -lam P2 (dP - D2),  dq_m = scale dS_m k_m,  dk_m = scale dS_m^T q_m,  dv = (P1 - lam P2)^T do,
@@ -190,11 +190,12 @@ __device__ __forceinline__ int64_t length_of(const Args &a, int b) {
 
 // ---------------------------------------------------------------------------------------------- forward
 // NQ groups of 32 rows (queries), two waves each: one a map, so that a map's sums are all that a wave holds (with both maps in one wave,
-// heads of 64 spilled at two waves a SIMD: 570 us on 32 heads of 4096 queries and keys where this takes 434).  KT keys a tile, 32 of them at a time.  DT: head size rounded up
-// to 32, 64, 128; values are up to 2 DT wide.  The running maximum is followed loosely: sums are scaled down only when it has grown by a
+// heads of 64 spilled at two waves a SIMD: 570 us on 32 heads of 4096 queries and keys where this takes 434).  KT keys a tile, 32 of them
+// at a time.  DT: head size rounded up to 32, 64, 128; values are up to 2 DT wide.  The running maximum is followed loosely: sums are scaled down only when it has grown by a
 // factor of 2^8 (weights stay below 2^8 until then, and the final division takes care of them).
 // What bounds it is the chip's power as much as its units: 434 us on random numbers (950 Tflop/s with both maps' products) are 365 on zeros,
-// and interleaving products with exponentials, or running scores a step ahead, changed neither by more than 3 %.
+// and interleaving products with exponentials, or running scores a step ahead, changed neither by more than 3 %.  Few queries are bound by
+// their keys and values: 34 us for 178 MB (5.2 TB/s; a large copy moves 5.1) with 8 x 16384 of them.
 template <typename T, int DT, int NQ, int KT>
 __global__ __launch_bounds__(128 * NQ, DT == 32 ? 4 : 2) void attention_kernel(Args a) {
     constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT, NW = 2 * NQ;
@@ -449,6 +450,11 @@ template <typename T> __global__ __launch_bounds__(512) void attention_join_kern
 
 // ---------------------------------------------------------------------------------------------- gradients of the queries
 // As the forward pass: a lane holds one query, dS^T is at once the right operand of  dq^T += k^T dS^T.  Also D1, D2 for the next kernel.
+// 90 us for 4 x 2047 causal tokens and 8 heads of 64 over 128 of ragged lengths (31 Gflop, 340 Tflop/s): half of a wave's time goes to exponentials and the
+// arithmetic between the products.
+
+// Up to so many keys D1, D2 are formed anew.  All gradients with and without: 8 x 512 causal tokens and 16 heads 135 and 121 us, 4 x 2047
+// and 8 heads 252 and 248 (310 if always); dq of 4 keys 1.42 and 1.8 times as far off 64 bits as its rounding, of 635 keys 1.45 and 1.5.
 constexpr int FEW = 512;
 template <typename T, int DT, int KT>
 __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 128 ? 1 : 2, DT == 128 ? 1 : 2))) void attention_dq_kernel(Args a) {
@@ -625,6 +631,8 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
 // head that reads them pass through LDS, 64 at a time, so shared heads' gradients are summed here.  Two waves take the first half of the
 // queries in a tile, two the second; their sums are added at the end, in order.
 // WHAT: 1 dv, 2 dk, 3 both.  Both need 450 registers for heads of 128: there dv and dk are summed by a launch each.
+// 129 us for 4 x 2047 causal tokens, 8 heads of 64 over 128 and 4 key heads, ragged (41 Gflop, 320 Tflop/s), bound like the kernel above; one wave
+// a SIMD, because dk, dv and the operands of 32 keys take 420 registers.
 template <typename T, int DT, int WHAT>
 __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
     constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT, NW = 4, QT = 64;
