@@ -86,6 +86,11 @@ def _rows(t, width):
     return t, m, step if m > 1 else width
 
 
+@functools.lru_cache(maxsize=256)
+def _linear_work(m, n, k):
+    return _lib.load_tokens().bndm_tokens_linear_workspace_bytes(m, n, k)
+
+
 def _linear_forward(x, weight, bias, residual, act, dtype, keep):
     n, k = weight.shape
     rows, m, ldx = _rows(x, k)
@@ -93,10 +98,9 @@ def _linear_forward(x, weight, bias, residual, act, dtype, keep):
     z = x.new_empty((m, n)) if keep and act else None
     res, _, ldr = _rows(residual, n) if residual is not None else (None, 0, 0)
     if m:
-        lib = _lib.load_tokens()
-        need = lib.bndm_tokens_linear_workspace_bytes(m, n, k)
+        need = _linear_work(m, n, k)
         work = x.new_empty(need, dtype=torch.uint8) if need else None
-        _launch(lib.bndm_tokens_linear, "linear", x.get_device(), rows.data_ptr(), ldx, weight.data_ptr(), _ptr(bias), _ptr(res), ldr,
+        _launch(_lib.load_tokens().bndm_tokens_linear, "linear", x.get_device(), rows.data_ptr(), ldx, weight.data_ptr(), _ptr(bias), _ptr(res), ldr,
                 y.data_ptr(), _ptr(z), m, n, k, act, dtype, _ptr(work), need)
     return y, z
 
@@ -222,7 +226,7 @@ def rotary(q, k, positions, sections, base=10000.0, interleaved=False):
     if len(shape) != 4 or (k is not None and (len(other) != 4 or other[:2] != shape[:2] or other[3] != shape[3])):
         raise ValueError(f"rotary: q {shape} and k {other}: [B, N, heads, D] of one B, N and D")
     _same("rotary", q, (("k", k),))
-    sections = tuple(int(s) for s in sections)
+    sections = tuple(map(int, sections))
     if positions.get_device() != q.get_device() or positions.dtype not in _POSITIONS:
         raise ValueError(f"rotary: positions are {positions.dtype} on {positions.device}: int32, int64 or float32 on {q.device}")
     if where != (shape[1], len(sections)) and where != (shape[0], shape[1], len(sections)):
