@@ -415,6 +415,82 @@ def test_captured_and_replayed(T):
                 assert torch.equal(a, b)
 
 
+def test_offsets_past_32_bits(T):
+    """rows, tokens and stored keys whose last elements lie more than 2^32 bytes from the first: what a copy that does not gives"""
+    w, rows = normal(1, 24, 1024).cuda(), (1 << 31) // 1024 + 100
+    x = torch.zeros(rows, 1024, dtype=F16, device="cuda")
+    x[-200:] = normal(2, 200, 1024)
+    # other tiles add up in another order: half a step of f16 on either side, and sums of 1024 (200) products in 32 bits, 2^-24 of their size each
+    assert torch.allclose(T.linear(x, w)[-200:], T.linear(x[-200:].clone(), w), rtol=2 ** -10, atol=2 * 1024 * 1024 * 2.0 ** -24)
+    y = torch.zeros(rows, 24, dtype=F16, device="cuda")
+    y[-200:] = normal(3, 200, 24)
+    leaf, part, weight = x.requires_grad_(), x[-200:].detach().clone().requires_grad_(), w.requires_grad_()
+    dx, dw = torch.autograd.grad(T.linear(leaf, weight), [leaf, weight], y)
+    ex, ew = torch.autograd.grad(T.linear(part, weight), [part, weight], y[-200:].contiguous())
+    assert torch.allclose(dx[-200:], ex, rtol=2 ** -10, atol=2 * 24 * 24 * 2.0 ** -24) and torch.allclose(dw, ew, rtol=2 ** -10, atol=2 * 200 * 200 * 2.0 ** -24)
+    assert not dx[:-200].any()
+    del x, leaf, dx
+
+    positions = torch.arange(300, dtype=torch.int32, device="cuda")[:, None]
+    store = torch.zeros(1, 300, 1 << 23, dtype=F16, device="cuda")            # 5 GB
+    h, hk, d = 4, 2, 64
+    store[..., : 2 * hk * d] = normal(4, 1, 300, 2 * hk * d)
+    store[..., 4096 : 4096 + hk * 2 * d] = normal(5, 1, 300, hk * 2 * d)
+    k, v = store[..., : 2 * hk * d].unflatten(-1, (2 * hk, d)), store[..., 4096 : 4096 + hk * 2 * d].unflatten(-1, (hk, 2 * d))
+    assert torch.equal(T.rotary(k, None, positions, (d // 2,)), T.rotary(k.contiguous(), None, positions, (d // 2,)))
+    lam = torch.tensor([0.2, 0.4, 0.6, 0.8], device="cuda")
+    for nq in (1, 300):
+        q = normal(6, 1, nq, 2 * h, d).cuda()
+        got, want = ([t.detach().requires_grad_() for t in (q, kk, vv)] for kk, vv in ((k, v), (k.contiguous(), v.contiguous())))
+        o, p = T.differential_attention(*got, lam, causal=True), T.differential_attention(*want, lam, causal=True)
+        assert torch.equal(o, p)
+        g = normal(7, *o.shape).cuda()
+        for a, b in zip(torch.autograd.grad(o, got, g), torch.autograd.grad(p, want, g)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_large_kernels_captured_beside_eager_ones(T, d):
+    """the kernels that take more LDS than a launch has by default: replayed while eager calls of the same sizes run on another stream"""
+    sizes = dict(x=(2048, 1024), w=(2048, 1024), q=(2, 700, 8, d), k=(2, 700, 4, d), v=(2, 700, 2, 2 * d))
+
+    def inputs(seed):
+        return {name: normal(seed + i, *size, dtype=BF16, std=0.5).cuda().requires_grad_() for i, (name, size) in enumerate(sizes.items())}
+
+    lam = torch.tensor([0.2, 0.4, 0.6, 0.8], device="cuda", requires_grad=True)
+
+    def work(t):
+        y = T.linear(t["x"], t["w"], activation="gelu")
+        o = T.differential_attention(t["q"], t["k"], t["v"], lam, causal=True)
+        return (y, *torch.autograd.grad(y, [t["x"], t["w"]], torch.ones_like(y)), o,
+                *torch.autograd.grad(o, [t["q"], t["k"], t["v"], lam], torch.ones_like(o)))
+
+    mine, side = inputs(1), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work(mine)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work(mine)
+    others = [inputs(100 * n) for n in range(1, 4)]
+    alone = [[t.clone() for t in work(other)] for other in others]
+    torch.cuda.synchronize()
+    for n, other in enumerate(others):
+        with torch.no_grad():
+            for name, t in mine.items():
+                t.copy_(other[name])
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(side):
+            beside = work(others[n - 1])
+        torch.cuda.synchronize()
+        for a, b in zip(out, alone[n]):
+            assert torch.equal(a, b)
+        for a, b in zip(beside, alone[n - 1]):
+            assert torch.equal(a, b)
+
+
 def test_the_same_bits_every_time(T):
     q, k, v, lam, dout = attention_inputs(2, 150, 150, 4, 2, 64, 128, F16)
     x, w = normal(1, 300, 520), normal(2, 260, 520, std=0.05)
