@@ -80,11 +80,6 @@ template <typename T> __device__ __forceinline__ s16x4 pack4(float a, float b, f
     const typename Vec<T>::x4 v = {(T)a, (T)b, (T)c, (T)d};
     return __builtin_bit_cast(s16x4, v);
 }
-template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
-    typedef T x2 __attribute__((ext_vector_type(2)));
-    const x2 v = {(T)a, (T)b};
-    return __builtin_bit_cast(uint32_t, v);
-}
 template <typename T> __device__ __forceinline__ float widen(short s) { return (float)__builtin_bit_cast(T, s); }
 
 // The 16-byte chunk in which chunk c of row `row` lies, for LDS tiles with rows of C chunks (C = 4, 8, 16, 32) that are read both as

@@ -256,6 +256,14 @@ def _aligned(t):
     return t, (n * h * d, h * d, d)
 
 
+@functools.lru_cache(maxsize=256)
+def _attention_work(backward, b, nq, nk, h, hk, d, dv):
+    """Bytes of scratch (0 for sizes that the call itself refuses)."""
+    lib = _lib.load_tokens()
+    ask = lib.bndm_tokens_attention_backward_workspace_bytes if backward else lib.bndm_tokens_attention_workspace_bytes
+    return ask(_lib.AttentionShape(b, nq, nk, h, hk, d, dv, *(0,) * 9, 0, 0, 0, 1.0))
+
+
 def _attention_forward(q, k, v, lam, q_start, kv_lengths, causal, scale, dtype, keep):
     b, nq, maps, d = q.shape
     _, nk, hk, dv = v.shape
@@ -264,10 +272,9 @@ def _attention_forward(q, k, v, lam, q_start, kv_lengths, causal, scale, dtype, 
     o = q.new_empty((b, nq, maps // 2, dv))
     o2 = q.new_empty((b, nq, maps // 2, dv)) if keep else None
     lse = q.new_empty((b, maps, nq), dtype=torch.float32) if keep else None
-    lib = _lib.load_tokens()
-    need = lib.bndm_tokens_attention_workspace_bytes(shape)
+    need = _attention_work(False, b, nq, nk, maps // 2, hk, d, dv)
     work = q.new_empty(need, dtype=torch.uint8) if need else None
-    _launch(lib.bndm_tokens_attention, "differential_attention", q.get_device(), shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(),
+    _launch(_lib.load_tokens().bndm_tokens_attention, "differential_attention", q.get_device(), shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(),
             _ptr(q_start), _ptr(kv_lengths), o.data_ptr(), _ptr(o2), _ptr(lse), _ptr(work), need)
     return o, o2, lse
 
@@ -294,10 +301,9 @@ class _DifferentialAttention(torch.autograd.Function):
             (q, qs), (k, ks), (v, vs), (dout, ds) = _aligned(q), _aligned(k), _aligned(v), _aligned(dout)
             shape = _lib.AttentionShape(b, nq, k.shape[1], maps // 2, v.shape[2], d, v.shape[3], *qs, *ks, *vs, causal, dtype,
                                         lam.dtype is torch.float32, scale)
-            lib = _lib.load_tokens()
-            need = lib.bndm_tokens_attention_backward_workspace_bytes(shape)
+            need = _attention_work(True, b, nq, k.shape[1], maps // 2, v.shape[2], d, v.shape[3])
             work = q.new_empty(need, dtype=torch.uint8)
-            _launch(lib.bndm_tokens_attention_backward, "differential_attention backward", q.get_device(), shape, q.data_ptr(), k.data_ptr(),
+            _launch(_lib.load_tokens().bndm_tokens_attention_backward, "differential_attention backward", q.get_device(), shape, q.data_ptr(), k.data_ptr(),
                     v.data_ptr(), lam.data_ptr(), _ptr(q_start), _ptr(kv_lengths), o.data_ptr(), o2.data_ptr(), lse.data_ptr(),
                     dout.data_ptr(), _Strides(*ds), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr(), work.data_ptr(),
                     need)
