@@ -795,11 +795,11 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
             const int beyond = key < len ? key - last : 1 << 30;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {                  // query tile_row(r, 0) of the half sees keys up to last + that
-                const bool hidden = beyond > tile_row(r, 0), only = -last == tile_row(r, 0) || len == 1;
+                const bool hidden = beyond > tile_row(r, 0), none = hidden | (-last == tile_row(r, 0)) | (len == 1);
 #pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                    if (hidden) p[m][r] = 0.f;
-                    if (hidden || only) s[m][r] = 0.f;
+                for (int m = 0; m < 2; ++m) {               // (selections: as branches they are 3000 instructions)
+                    p[m][r] = hidden ? 0.f : p[m][r];
+                    s[m][r] = none ? 0.f : s[m][r];
                 }
             }
         }
