@@ -8,7 +8,8 @@
 // Backward, with dP = do v^T (the same for both maps), D_m = rowsum(P_m dP) = do . o_m:
 //   dS1 = P1 (dP - D1),  dS2 = -lam P2 (dP - D2),  dq_m = scale dS_m k_m,  dk_m = scale dS_m^T q_m,  dv = (P1 - lam P2)^T do,
 //   dlam = - sum over rows of D2.
-// Two kernels, each with the sums it owns in registers: no atomics, and the same result every time.
+// Two kernels, one for the queries and one for the keys, each with the sums it owns in registers: no atomics, and the same result every
+// time.
 //
 // Statistics, sums and gradients' sums are 32 bits; weights (P, dS) are rounded to the inputs' type for the matrix units, as products
 // of 16-bit operands are what those take.
@@ -631,7 +632,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
 // head that reads them pass through LDS, 64 at a time, so shared heads' gradients are summed here.  Two waves take the first half of the
 // queries in a tile, two the second; their sums are added at the end, in order.
 // WHAT: 1 dv, 2 dk, 3 both.  Both need 450 registers for heads of 128: there dv and dk are summed by a launch each.
-// 129 us for 4 x 2047 causal tokens, 8 heads of 64 over 128 and 4 key heads, ragged (41 Gflop, 320 Tflop/s), bound like the kernel above; one wave
+// 117 us for 4 x 2047 causal tokens, 8 heads of 64 over 128 and 4 key heads, ragged (41 Gflop, 350 Tflop/s), bound like the kernel above; one wave
 // a SIMD, because dk, dv and the operands of 32 keys take 420 registers.
 template <typename T, int DT, int WHAT>
 __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
