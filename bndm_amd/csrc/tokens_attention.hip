@@ -104,11 +104,14 @@ template <int C, bool COLUMNS = false> struct ColumnReader {       // operand wh
 };
 
 // Workgroups go to the 8 XCDs in turn.  This deals out heads (the units that share keys, `tiles` workgroups each) to the XCDs, so that one's
-// workgroups run behind one L2, and within a head the last tile first: with a causal mask it is the longest.
+// workgroups run behind one L2, and within a head the last tile first: with a causal mask it is the longest.  An XCD's second 32
+// workgroups begin beside its first 32, one on each of its CUs: every other 32 go the other way, so that long ones meet short ones (the
+// forward pass of 4 x 2047 causal tokens of ragged lengths and 8 heads 70 us, 79 without; the queries' gradients 86 and 93).
 __device__ __forceinline__ void place(int id, int units, int tiles, int &unit, int &tile) {
     const int even = units & ~7;
     if (id < even * tiles) {
-        const int seq = id >> 3;
+        int seq = id >> 3;
+        if ((seq & 32) && (seq | 31) < even / 8 * tiles) seq ^= 31;
         unit = (seq / tiles) * 8 + (id & 7);
         tile = tiles - 1 - seq % tiles;
     } else {
@@ -190,15 +193,16 @@ __device__ __forceinline__ int64_t length_of(const Args &a, int b) {
 }
 
 // ---------------------------------------------------------------------------------------------- forward
-// NQ groups of 32 rows (queries), two waves each: one a map, so that a map's sums are all that a wave holds (with both maps in one wave,
-// heads of 64 spilled at two waves a SIMD: 570 us on 32 heads of 4096 queries and keys where this takes 434).  KT keys a tile, 32 of them
-// at a time.  DT: head size rounded up to 32, 64, 128; values are up to 2 DT wide.  The running maximum is followed loosely: sums are scaled down only when it has grown by a
-// factor of 2^8 (weights stay below 2^8 until then, and the final division takes care of them).
-// What bounds it is the chip's power as much as its units: 434 us on random numbers (950 Tflop/s with both maps' products) are 365 on zeros,
-// and interleaving products with exponentials, or running scores a step ahead, changed neither by more than 3 %.  Few queries are bound by
-// their keys and values: 34 us for 178 MB (5.2 TB/s; a large copy moves 5.1) with 8 x 16384 of them.
+// NQ groups of 32 rows (queries), two waves each: one a map, so that a map's sums are all that a wave holds.  KT keys a tile, 32 of them
+// at a time.  DT: head size rounded up to 32, 64, 128; values are up to 2 DT wide.  The running maximum is followed loosely: sums are
+// scaled down only when it has grown by a factor of 2^8 (weights stay below 2^8 until then, and the final division takes care of them).
+// What bounds it is the chip's power as much as its units: with two waves a SIMD, 430 us on random numbers were 365 on zeros for 32 heads
+// of 64, 4096 queries and keys, and interleaving products with exponentials, or running scores a step ahead, changed neither by more than
+// 3 %.  Four waves a SIMD, for which heads of 64 make do with tiles of 32 keys and 128 registers, take 397 (1040 Tflop/s with both maps'
+// products); both maps in one wave took 570.
+// Few queries are bound by their keys and values: 34 us for 178 MB (5.2 TB/s; a large copy moves 5.1) with 8 x 16384 of them.
 template <typename T, int DT, int NQ, int KT>
-__global__ __launch_bounds__(128 * NQ, DT == 32 ? 4 : 2) void attention_kernel(Args a) {
+__global__ __launch_bounds__(128 * NQ, DT == 32 || (DT == 64 && NQ == 4) ? 4 : 2) void attention_kernel(Args a) {
     constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT, NW = 2 * NQ;
     // Weights go to the matrix units in the inputs' type.  bf16's 8 bits are about as far off as the output's own rounding (2.6e-3 in all
     // where that alone is 1.7e-3); a second product with what was rounded off takes that away.  Few queries wait for their keys (8 x 16384 of
@@ -936,7 +940,7 @@ template <typename F> int allow_lds(F kernel, int bytes, const char *what) {
 }
 
 template <typename T, int DT> int forward(const Args &a, const Plan &p, hipStream_t stream) {
-    constexpr int KT = DT == 128 ? 32 : 64;
+    constexpr int KT = DT == 32 ? 64 : 32;
     if (p.waves == 1) hipLaunchKernelGGL((attention_kernel<T, DT, 1, 32>), dim3((unsigned)p.blocks), dim3(128), 0, stream, a);
     else hipLaunchKernelGGL((attention_kernel<T, DT, 4, KT>), dim3((unsigned)p.blocks), dim3(512), 0, stream, a);
     if (int rc = tokens_launch_status("attention")) return rc;
