@@ -455,8 +455,8 @@ template <typename T> __global__ __launch_bounds__(512) void attention_join_kern
 
 // ---------------------------------------------------------------------------------------------- gradients of the queries
 // As the forward pass: a lane holds one query, dS^T is at once the right operand of  dq^T += k^T dS^T.  Also D1, D2 for the next kernel.
-// 90 us for 4 x 2047 causal tokens and 8 heads of 64 over 128 of ragged lengths (31 Gflop, 340 Tflop/s): half of a wave's time goes to exponentials and the
-// arithmetic between the products.
+// 85 us for 4 x 2047 causal tokens and 8 heads of 64 over 128 of ragged lengths (31 Gflop, 360 Tflop/s): half of a wave's time goes to
+// exponentials and the arithmetic between the products.
 
 // Up to so many keys D1, D2 are formed anew.  All gradients with and without: 8 x 512 causal tokens and 16 heads 135 and 121 us, 4 x 2047
 // and 8 heads 252 and 248 (310 if always); dq of 4 keys 1.42 and 1.8 times as far off 64 bits as its rounding, of 635 keys 1.45 and 1.5.
@@ -636,7 +636,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
 // head that reads them pass through LDS, 64 at a time, so shared heads' gradients are summed here.  Two waves take the first half of the
 // queries in a tile, two the second; their sums are added at the end, in order.
 // WHAT: 1 dv, 2 dk, 3 both.  Both need 450 registers for heads of 128: there dv and dk are summed by a launch each.
-// 117 us for 4 x 2047 causal tokens, 8 heads of 64 over 128 and 4 key heads, ragged (41 Gflop, 350 Tflop/s), bound like the kernel above; one wave
+// 120 us for 4 x 2047 causal tokens, 8 heads of 64 over 128 and 4 key heads, ragged (41 Gflop, 340 Tflop/s), bound like the kernel above; one wave
 // a SIMD, because dk, dv and the operands of 32 keys take 420 registers.
 template <typename T, int DT, int WHAT>
 __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
