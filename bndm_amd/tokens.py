@@ -245,9 +245,7 @@ def _aligned(t):
     """``t`` [B, N, H, D] as the kernels read it -- heads' elements next to each other, all else in steps of 16 bytes -- and its strides."""
     b, n, h, d = t.shape
     sb, sn, sh, sd = t.stride()
-    if b == 1: sb = 0
-    if n == 1: sn = 0
-    if h == 1: sh = 0
+    sb, sn, sh = sb * (b > 1), sn * (n > 1), sh * (h > 1)       # (of one there is no distance)
     if (sd == 1 or d == 1) and not (t.data_ptr() % 16 or sb % 8 or sn % 8 or sh % 8 or sn > 1 << 23):
         return t, (sb, sn, sh)
     t = t.contiguous()
