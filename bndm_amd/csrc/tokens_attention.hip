@@ -8,7 +8,7 @@
 // Backward, with dP = do v^T (the same for both maps), D_m = rowsum(P_m dP) = do . o_m:
 //   dS1 = P1 (dP - D1),  dS2 = -lam P2 (dP - D2),  dq_m = scale dS_m k_m,  dk_m = scale dS_m^T q_m,  dv = (P1 - lam P2)^T do,
 //   dlam = - sum over rows of D2.
-// Two kernels, one for the queries and one for the keys, each with the sums it owns in registers: no atomics, and the same result every
+// A kernel for D_m, one for the queries and one for the keys, each with the sums it owns in registers: no atomics, and the same result every
 // time.
 //
 // Statistics, sums and gradients' sums are 32 bits; weights (P, dS) are rounded to the inputs' type for the matrix units, as products
@@ -453,14 +453,137 @@ template <typename T> __global__ __launch_bounds__(512) void attention_join_kern
     }
 }
 
-// ---------------------------------------------------------------------------------------------- gradients of the queries
-// As the forward pass: a lane holds one query, dS^T is at once the right operand of  dq^T += k^T dS^T.  Also D1, D2 for the next kernel.
-// 85 us for 4 x 2047 causal tokens and 8 heads of 64 over 128 of ragged lengths (31 Gflop, 360 Tflop/s): half of a wave's time goes to
-// exponentials and the arithmetic between the products.
+// ---------------------------------------------------------------------------------------------- centres of the gradients
+// D1 and D2, which both kernels of gradients need first.  dP - D cancels in rows whose weight is nearly all on a few keys, and then what D
+// is off by is what dq shows: from outputs rounded to 16 bits, D' = do . o_m, scores of deviation 6 gave a bf16 dq as far off as it is long.
+// So a pass over the keys forms  D_m = D' + sum_j P_mj (dP_j - D')  in 32 bits.  (Of the differences: what log-sum-exp of large scores is
+// off by makes the weights' sum 1 + e, and counts here as e (D - D'), not as e D.)
+// 70 us for 4 x 2047 causal tokens and 8 heads of 64 over 128 of ragged lengths (21 Gflop, 300 Tflop/s): exponentials, the arithmetic around
+// them and the products take about as long as one another, and three waves a SIMD run them beside one another.  Done in the next kernel, with the registers that its
+// sums hold, it took as long with two.
+template <typename T, int DT, int KT>
+__global__ __launch_bounds__(THREADS, DT == 32 ? 4 : DT == 64 ? 3 : 2) void attention_delta_kernel(Args a) {
+    constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT, NW = 4;
+    constexpr int K_BYTES = KT * CK * 16, V_BYTES = KT * CV * 16, STAGE = 2 * K_BYTES + V_BYTES;
+    __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
+    const int tid = threadIdx.x, l = tid & 63, h32 = l >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tiles = (int)((a.Nq + 127) / 128);
+    int unit, tile;
+    place(blockIdx.x, a.B * a.H, tiles, unit, tile);
+    const int head = unit % a.H, b = unit / a.H;
+    const int hk = head / (a.H / a.Hk);
+    const int64_t row = (int64_t)tile * 128 + w * 32 + (l & 31);
+    const bool row_in = row < a.Nq;
+    const int64_t i = row_in ? row : 0;
+    const int64_t start = start_of(a, b);
+    const int len = (int)length_of(a, b);
+    auto upto = [&](int64_t i) { return a.causal ? (int)min((int64_t)len, max((int64_t)0, start + i + 1)) : len; };
+    const int sees = row_in ? upto(i) : 0, j_end = upto(min(a.Nq - 1, (int64_t)tile * 128 + 127)), fewest = upto((int64_t)tile * 128 + w * 32);
+    s16x8 qf[2][DT / 16], gf[DV / 16];
+    float delta[2] = {0.f, 0.f};
+    {
+        const T *g = (const T *)a.dout + (int64_t)b * a.dob + i * a.don + (int64_t)head * a.doh;
+        const int64_t at = (((int64_t)b * a.Nq + i) * a.H + head) * a.Dv;
+#pragma unroll
+        for (int s = 0; s < DV / 16; ++s) {
+            const int c = 2 * s + h32;
+            const bool in = row_in && c * 8 < a.Dv;
+            gf[s] = load8(g + c * 8, in);
+            const s16x8 o = load8((const T *)a.o + at + c * 8, in), o2 = load8((const T *)a.o2 + at + c * 8, in);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const short gs = gf[s][e], os = o[e], ps = o2[e];
+                const float ge = widen<T>(gs);
+                delta[0] += ge * widen<T>(os);
+                delta[1] += ge * widen<T>(ps);
+            }
+        }
+        delta[0] = both_halves_sum(delta[0]);
+        delta[1] = both_halves_sum(delta[1]);
+        delta[0] += lam_of<T>(a, head) * delta[1];          // (o + lam o2 is the first map's output)
+    }
+    __builtin_amdgcn_sched_barrier(0);                      // (queries beside the outputs have no registers in heads of 128)
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        const T *p = (const T *)a.q + (int64_t)b * a.qb + i * a.qn + (int64_t)(2 * head + m) * a.qh;
+#pragma unroll
+        for (int s = 0; s < DT / 16; ++s) {
+            const int c = 2 * s + h32;
+            qf[m][s] = load8(p + c * 8, row_in && c * 8 < a.D);
+        }
+    }
+    float lse[2], off[2] = {0.f, 0.f};
+#pragma unroll
+    for (int m = 0; m < 2; ++m) lse[m] = row_in ? a.lse[((int64_t)b * 2 * a.H + 2 * head + m) * a.Nq + i] : INFINITY;
 
-// Up to so many keys D1, D2 are formed anew.  All gradients with and without: 8 x 512 causal tokens and 16 heads 135 and 121 us, 4 x 2047
-// and 8 heads 252 and 248 (310 if always); dq of 4 keys 1.42 and 1.8 times as far off 64 bits as its rounding, of 635 keys 1.45 and 1.5.
-constexpr int FEW = 512;
+    const float to_log2 = a.scale * kLog2e;
+    const T *kp = (const T *)a.k + (int64_t)b * a.kb + (int64_t)(2 * hk) * a.kh;
+    const T *vp = (const T *)a.v + (int64_t)b * a.vb + (int64_t)hk * a.vh;
+    Stager<KT, CK, NW> stage_k;
+    Stager<KT, CV, NW> stage_v;
+    stage_k.begin(a.kn, a.D / 8, w, l);
+    stage_v.begin(a.vn, a.Dv / 8, w, l);
+    auto fetch = [&](char *to, int j) __attribute__((always_inline)) {
+        stage_k.copy(to, kp + j * a.kn, len - j, w);
+        stage_k.copy(to + K_BYTES, kp + a.kh + j * a.kn, len - j, w);
+        stage_v.copy(to + 2 * K_BYTES, vp + j * a.vn, len - j, w);
+    };
+    RowReader<CK> keys;
+    RowReader<CV> values;
+    keys.begin(l);
+    values.begin(l);
+    if (0 < j_end) fetch(smem, 0);
+    auto turn = [&](char *__restrict__ ahead, const char *__restrict__ now, int j) __attribute__((always_inline)) {
+        tile_there<NW>();
+        if (j + KT < j_end) fetch(ahead, j + KT);
+#pragma unroll
+        for (int t = 0; t < KT / 32; ++t) {
+            f32x16 dp[1];
+            clear(dp);
+#pragma unroll
+            for (int d = 0; d < DV / 16; ++d) dp[0] = mfma32<T>(values.read(now + 2 * K_BYTES, t, d), gf[d], dp[0]);
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                f32x16 s[1];
+                clear(s);
+#pragma unroll
+                for (int d = 0; d < DT / 16; ++d) s[0] = mfma32<T>(keys.read(now + m * K_BYTES, t, d), qf[m][d], s[0]);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[0][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], to_log2, -lse[m]));
+                if (j + 32 * t + 32 > fewest) {
+                    const int n = sees - j - 32 * t - 4 * h32;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (tile_row(r, 0) >= n) s[0][r] = 0.f;
+                }
+                float sum[2] = {0.f, 0.f};                  // (two chains: a sum waits for the one before)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sum[r & 1] = __builtin_fmaf(s[0][r], dp[0][r] - delta[m], sum[r & 1]);
+                off[m] += sum[0] + sum[1];
+            }
+        }
+    };
+    __builtin_amdgcn_s_waitcnt(0);                          // (what came before the loop is there, or its turns would wait for as much)
+    for (int j = 0; j < j_end; j += 2 * KT) {
+        turn(smem + STAGE, smem, j);
+        if (j + KT < j_end) turn(smem, smem + STAGE, j + KT);
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        delta[m] += both_halves_sum(off[m]);
+        if (row_in && h32 == 0) a.delta[((int64_t)b * 2 * a.H + 2 * head + m) * a.Nq + i] = delta[m];
+    }
+    float sum = delta[1];                                   // (0 for rows past the end)
+#pragma unroll
+    for (int x = 1; x < 32; x *= 2) sum += __shfl_xor(sum, x);
+    if (l == 0) a.d2_sums[(((int64_t)head * a.B + b) * tiles + tile) * NW + w] = sum;
+}
+
+// ---------------------------------------------------------------------------------------------- gradients of the queries
+// As the forward pass: a lane holds one query, dS^T is at once the right operand of  dq^T += k^T dS^T.
+// 71 us for 4 x 2047 causal tokens and 8 heads of 64 over 128 of ragged lengths (31 Gflop, 440 Tflop/s): half of a wave's time goes to
+// exponentials and the arithmetic between the products.
 template <typename T, int DT, int KT>
 __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 128 ? 1 : 2, DT == 128 ? 1 : 2))) void attention_dq_kernel(Args a) {
     constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT, NW = 4;
@@ -492,42 +615,22 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
             qf[m][s] = load8(p + c * 8, row_in && c * 8 < a.D);
         }
     }
-    // D2 = do . o2, D1 = do . (o + lam o2), as near as rounded outputs and weights give them: 2^-9 of theirs, which few keys would show.
-    // Up to FEW keys they are formed anew in a pass of its own below; behind more keys, what they are off is found along the way, as
-    // sum_j dS_ij = 0, and the gradients of keys and lam take them without it.
     const float lam = lam_of<T>(a, head);
-    const bool few = j_end <= FEW;
-    float delta[2] = {0.f, 0.f};
     {
         const T *g = (const T *)a.dout + (int64_t)b * a.dob + i * a.don + (int64_t)head * a.doh;
-        const int64_t at = (((int64_t)b * a.Nq + i) * a.H + head) * a.Dv;
 #pragma unroll
         for (int s = 0; s < DV / 16; ++s) {
             const int c = 2 * s + h32;
             gf[s] = load8(g + c * 8, row_in && c * 8 < a.Dv);
         }
-        if (!few) {
-#pragma unroll
-            for (int s = 0; s < DV / 16; ++s) {
-                const int c = 2 * s + h32;
-                const bool in = row_in && c * 8 < a.Dv;
-                const s16x8 o = load8((const T *)a.o + at + c * 8, in), o2 = load8((const T *)a.o2 + at + c * 8, in);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const short gs = gf[s][e], os = o[e], ps = o2[e];
-                    const float ge = widen<T>(gs);
-                    delta[0] += ge * widen<T>(os);
-                    delta[1] += ge * widen<T>(ps);
-                }
-            }
-            delta[0] = both_halves_sum(delta[0]);
-            delta[1] = both_halves_sum(delta[1]);
-            delta[0] += lam * delta[1];
-        }
     }
-    float lse[2], off[2] = {0.f, 0.f};
+    float lse[2], delta[2];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) lse[m] = row_in ? a.lse[((int64_t)b * 2 * a.H + 2 * head + m) * a.Nq + i] : INFINITY;
+    for (int m = 0; m < 2; ++m) {
+        const int64_t at = ((int64_t)b * 2 * a.H + 2 * head + m) * a.Nq + i;
+        lse[m] = row_in ? a.lse[at] : INFINITY;
+        delta[m] = row_in ? a.delta[at] : 0.f;
+    }
 
     f32x16 acc[2][DT / 32];
     clear(acc[0]);
@@ -551,9 +654,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
     values.begin(l);
     key_columns.begin(l);
     if (0 < j_end) fetch(smem, 0);
-    // FIRST: D1, D2 only
-    auto turn = [&](auto first, char *__restrict__ ahead, const char *__restrict__ now, int j) __attribute__((always_inline)) {
-        constexpr bool FIRST = decltype(first)::value;
+    auto turn = [&](char *__restrict__ ahead, const char *__restrict__ now, int j) __attribute__((always_inline)) {
         tile_there<NW>();
         if (j + KT < j_end) fetch(ahead, j + KT);
 #pragma unroll
@@ -570,57 +671,28 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
 #pragma unroll
                 for (int d = 0; d < DT / 16; ++d) s[0] = mfma32<T>(keys.read(now + m * K_BYTES, t, d), qf[m][d], s[0]);
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    s[0][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], to_log2, -lse[m])) * (FIRST ? dp[0][r] : dp[0][r] - delta[m]);
+                for (int r = 0; r < 16; ++r) s[0][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], to_log2, -lse[m])) * (dp[0][r] - delta[m]);
                 if (masked) {                               // (a row that sees one key has weight 1 there whatever its score)
-                    const int n = !FIRST && sees == 1 ? 0 : sees - j - 32 * t - 4 * h32;
+                    const int n = sees == 1 ? 0 : sees - j - 32 * t - 4 * h32;
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
                         if (tile_row(r, 0) >= n) s[0][r] = 0.f;
                 }
-                float sum = 0.f;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) sum += s[0][r];
-                off[m] += sum;
-                if constexpr (!FIRST)
+                for (int x = 0; x < 2; ++x) {
+                    const s16x8 ds = as_operand<T>(s[0], x);
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const s16x8 ds = as_operand<T>(s[0], x);
-#pragma unroll
-                        for (int d = 0; d < DT / 32; ++d) acc[m][d] = mfma32<T>(key_columns.read(now + m * K_BYTES, 32 * t + 16 * x, d), ds, acc[m][d]);
-                    }
+                    for (int d = 0; d < DT / 32; ++d) acc[m][d] = mfma32<T>(key_columns.read(now + m * K_BYTES, 32 * t + 16 * x, d), ds, acc[m][d]);
+                }
             }
         }
     };
-    auto pass = [&](auto first) __attribute__((always_inline)) {
-        __builtin_amdgcn_s_waitcnt(0);                      // (what came before the loop is there, or its turns would wait for as much)
-        for (int j = 0; j < j_end; j += 2 * KT) {
-            turn(first, smem + STAGE, smem, j);
-            if (j + KT < j_end) turn(first, smem, smem + STAGE, j + KT);
-        }
-        tile_there<NW>();
-    };
-    if (few) {
-        pass(std::true_type());
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            delta[m] = both_halves_sum(off[m]);
-            off[m] = 0.f;
-        }
-        if (0 < j_end) fetch(smem, 0);
+    __builtin_amdgcn_s_waitcnt(0);                          // (what came before the loop is there, or its turns would wait for as much)
+    for (int j = 0; j < j_end; j += 2 * KT) {
+        turn(smem + STAGE, smem, j);
+        if (j + KT < j_end) turn(smem, smem + STAGE, j + KT);
     }
-    pass(std::false_type());
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        delta[m] += both_halves_sum(off[m]);
-        if (row_in && h32 == 0) a.delta[((int64_t)b * 2 * a.H + 2 * head + m) * a.Nq + i] = delta[m];
-    }
-    {
-        float sum = delta[1];                               // (0 for rows past the end)
-#pragma unroll
-        for (int x = 1; x < 32; x *= 2) sum += __shfl_xor(sum, x);
-        if (l == 0) a.d2_sums[(((int64_t)head * a.B + b) * tiles + tile) * NW + w] = sum;
-    }
+    tile_there<NW>();
     char *own = smem + w * 32 * DT * 2;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
@@ -880,7 +952,7 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
     if constexpr (VALUES) store_rows<T, DV>(own, (T *)a.dv, (at * a.Hk + hk) * a.Dv, to_write, a.Dv, l, [&](int t, int r) { return dv[t][r]; });
 }
 
-// dlam[h] = - sum over sequences and queries of D2, of which each wave above has left the sum of its 32: one workgroup a head, in a
+// dlam[h] = - sum over sequences and queries of D2, of which each wave of the first kernel has left the sum of its 32: one workgroup a head, in a
 // fixed order.  4 us for 8 heads of 8188 queries, where reading all of D2 here took 11.
 template <typename T> __global__ __launch_bounds__(THREADS) void attention_dlam_kernel(Args a) {
     __shared__ float part[THREADS];
@@ -961,6 +1033,8 @@ template <typename T, int DT, int WHAT> int launch_dkv(const Args &a, hipStream_
 template <typename T, int DT> int backward(const Args &a, hipStream_t stream) {
     constexpr int KT = DT == 128 ? 32 : 64;
     const int64_t nq = ceil_div64(a.Nq, 128) * a.H * a.B;
+    hipLaunchKernelGGL((attention_delta_kernel<T, DT, 32>), dim3((unsigned)nq), dim3(THREADS), 0, stream, a);
+    if (int rc = tokens_launch_status("attention delta")) return rc;
     hipLaunchKernelGGL((attention_dq_kernel<T, DT, KT>), dim3((unsigned)nq), dim3(THREADS), 0, stream, a);
     if (int rc = tokens_launch_status("attention dq")) return rc;
     if (a.Nk > 0) {

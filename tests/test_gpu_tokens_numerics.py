@@ -1,0 +1,115 @@
+"""GPU tests of what bndm_amd.tokens keeps between its 16-bit inputs and outputs: weights, statistics, gradients that cancel, values past
+the types' ranges, memory that no query sees.
+
+Bounds are worst cases to first order.  u = finfo(t).eps / 2 is what storing a value may take off it, relative to it; in 32 bits that is
+E = 2^-24.  A sum of n products in 32 bits is off by n E of the sum of their magnitudes at most, whatever its order."""
+import math
+
+import pytest
+import torch
+
+from tests import tokens_reference as R
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+E = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def T():
+    from bndm_amd import tokens
+    return tokens
+
+
+def normal(seed, *shape, dtype=F16, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * std).to(dtype)
+
+
+def on_gpu(values):
+    return None if values is None else torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def attention_in_64_bits(q, k, v, lam, seen, dout=None, scale=None):
+    """-> {name: (value, bound)} as R.attention, but the weights, the outputs and the sums of weights times their gradients are held in 32
+    bits (weights in two parts of 16): what is rounded to 16 bits is the results, the weights dv is formed of, and scale dS."""
+    dtype, u, tiny = q.dtype, R.unit(q.dtype), R.smallest(q.dtype)
+    b, nq, maps, d = q.shape
+    nk, hk, dv = v.shape[1:]
+    per = maps // 2 // hk
+    scale = d ** -0.5 if scale is None else scale
+    wide = lambda t: t.unflatten(1, (hk, 2)).repeat_interleave(per, 1).flatten(1, 2)
+    q64, k64 = q.double().transpose(1, 2), wide(k.double().transpose(1, 2))
+    v64 = v.double().transpose(1, 2).repeat_interleave(per, 1)
+    l = lam.double()[:, None, None]
+    s = (q64 @ k64.transpose(-1, -2) * scale).masked_fill(~seen, -math.inf)
+    top = s.amax(-1, keepdim=True)
+    top = torch.where(top.isfinite(), top, torch.zeros_like(top))
+    e = torch.exp(s - top)
+    total = e.sum(-1, keepdim=True)
+    p = e / torch.where(total > 0, total, torch.ones_like(total))
+    # a score is a sum of d products; it meets the running maximum and the sum's logarithm, 8 roundings of numbers of that size with the
+    # exponential's own; sums of nk weights, and as many again where a running maximum moves
+    size = q64.abs() @ k64.abs().transpose(-1, -2) * scale
+    off_p = (d * E * size + 8 * E * (1 + size.amax(-1, keepdim=True) + math.log(nk))) + 2 * nk * E
+    p1, p2, e1, e2 = p[:, 0::2], p[:, 1::2], off_p[:, 0::2], off_p[:, 1::2]
+    w = p1 - l * p2
+    o = w @ v64
+    # two parts of 16 bits leave u of u of a weight, and the least number of the type of a sum that is 1 at least
+    part = lambda pm, em: ((pm * (em + (pm * em).sum(-1, keepdim=True) + u * u) + tiny * (pm > 0)) @ v64.abs()) + nk * E * (pm @ v64.abs())
+    off_o = part(p1, e1) + l.abs() * part(p2, e2)
+    out = {"o": (o.transpose(1, 2), (off_o + u * (o.abs() + off_o) + tiny).transpose(1, 2))}
+    if dout is None:
+        return out
+    g = dout.double().transpose(1, 2)
+    gv, mag = g @ v64.transpose(-1, -2), g.abs() @ v64.abs().transpose(-1, -2)
+    ds, off, sums = [], [], []
+    for pm, em, f in ((p1, e1, torch.ones_like(l)), (p2, e2, -l)):
+        big = pm * em
+        centre = (pm * gv).sum(-1, keepdim=True)
+        # dP is a sum of dv products, D = sum P dP in 32 bits
+        raw = dv * E * mag
+        off_d = (pm * raw + big * (gv - centre).abs()).sum(-1, keepdim=True) + 2 * nk * E * (pm * gv.abs()).sum(-1, keepdim=True)
+        sums.append((centre, off_d))
+        x = pm * (gv - centre) * f
+        ds.append(x)
+        off.append(f.abs() * (pm * (raw + off_d + 4 * E * (gv.abs() + centre.abs())) + (em + (pm * em).sum(-1, keepdim=True)) * pm * (gv - centre).abs())
+                   + u * x.abs() + tiny / scale * (pm > 0))
+    ds, off = torch.stack(ds, 2).flatten(1, 2), torch.stack(off, 2).flatten(1, 2)
+
+    def shared(t, two):
+        t = t.unflatten(1, (hk, per, 2)) if two else t.unflatten(1, (hk, per))
+        return t.sum(2).flatten(1, 2) if two else t.sum(2)
+
+    def add(key, grad, err, size, n):
+        out[key] = (grad.transpose(1, 2), (err + n * E * size + u * (grad.abs() + err) + tiny).transpose(1, 2))
+
+    add("q", ds @ k64 * scale, off @ k64.abs() * scale, ds.abs() @ k64.abs() * scale, nk)
+    add("k", shared(ds.transpose(-1, -2) @ q64, True) * scale, shared(off.transpose(-1, -2) @ q64.abs(), True) * scale,
+        shared(ds.abs().transpose(-1, -2) @ q64.abs(), True) * scale, nq * per)
+    off_w = u * w.abs() + p1 * e1 + l.abs() * p2 * e2 + (p1 * (p1 * e1).sum(-1, keepdim=True) + l.abs() * p2 * (p2 * e2).sum(-1, keepdim=True)) + tiny * (p1 > 0)
+    add("v", shared(w.transpose(-1, -2) @ g, False), shared(off_w.transpose(-1, -2) @ g.abs(), False), shared(w.abs().transpose(-1, -2) @ g.abs(), False), nq * per)
+    (_, _), (d2, off_d2) = sums
+    grad, err = -d2.sum((0, 2, 3)), off_d2.sum((0, 2, 3)) + nq * b * E * d2.abs().sum((0, 2, 3))
+    out["lam"] = (grad, err + R.unit(lam.dtype) * (grad.abs() + err) + R.smallest(lam.dtype))
+    return out
+
+
+# ---------------------------------------------------------------------------------------------- gradients of peaked rows
+@pytest.mark.parametrize("b,nq,nk,h,hk,d,dv,causal", [(1, 70, 513, 2, 1, 64, 128, False), (2, 40, 1030, 2, 2, 64, 128, False), (1, 600, 600, 2, 1, 64, 128, True),
+                                                      (1, 33, 2000, 1, 1, 128, 256, False), (2, 130, 700, 2, 1, 32, 64, False), (1, 64, 200, 2, 1, 64, 128, False),
+                                                      (2, 5, 1500, 4, 2, 24, 40, True)])
+@pytest.mark.parametrize("std", [1.0, 4.0, 6.0])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_gradients_of_peaked_rows(T, b, nq, nk, h, hk, d, dv, causal, std, dtype):
+    """Few keys have nearly all of a row's weight: dP - D cancels there, and what D is off by is all that is left.  So D must not come from
+    outputs that were rounded to 16 bits."""
+    q, k = normal(1, b, nq, 2 * h, d, dtype=dtype, std=std ** 0.5), normal(2, b, nk, 2 * hk, d, dtype=dtype, std=std ** 0.5)
+    v, g = normal(3, b, nk, hk, dv, dtype=dtype), normal(4, b, nq, h, dv, dtype=dtype)
+    lam = torch.rand(h, generator=torch.Generator().manual_seed(5)) + 0.1
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v, lam)]
+    o = T.differential_attention(*leaves, causal=causal)
+    want = attention_in_64_bits(q, k, v, lam, R.visible(nq, nk, None, causal, None, b), g)
+    for name, got in zip(("q", "k", "v", "lam"), torch.autograd.grad(o, leaves, g.cuda())):
+        R.assert_within(got, *want[name], "d" + name)
