@@ -11,10 +11,8 @@
 // A kernel for D_m, one for the queries and one for the keys, each with the sums it owns in registers: no atomics, and the same result every
 // time.
 //
-// Statistics, sums and gradients' sums are 32 bits; weights (P, dS) are rounded to the inputs' type for the matrix units, as products
-// of 16-bit operands are what those take.
-#include <type_traits>
-
+// Statistics, sums and gradients' sums are 32 bits.  The matrix units take products of 16-bit operands: the forward pass's weights go there in two
+// parts, P as rounded and what that left off, the gradients' (P1 - lam P2 for dv, dS) rounded once, like a value that is stored.
 #include "tokens_common.hpp"
 #include <cmath>
 
@@ -196,18 +194,17 @@ __device__ __forceinline__ int64_t length_of(const Args &a, int b) {
 // NQ groups of 32 rows (queries), two waves each: one a map, so that a map's sums are all that a wave holds.  KT keys a tile, 32 of them
 // at a time.  DT: head size rounded up to 32, 64, 128; values are up to 2 DT wide.  The running maximum is followed loosely: sums are
 // scaled down only when it has grown by a factor of 2^8 (weights stay below 2^8 until then, and the final division takes care of them).
-// What bounds it is the chip's power as much as its units: with two waves a SIMD, 430 us on random numbers were 365 on zeros for 32 heads
-// of 64, 4096 queries and keys, and interleaving products with exponentials, or running scores a step ahead, changed neither by more than
-// 3 %.  Four waves a SIMD, for which heads of 64 make do with tiles of 32 keys and 128 registers, take 397 (1040 Tflop/s with both maps'
-// products); both maps in one wave took 570.
-// Few queries are bound by their keys and values: 34 us for 178 MB (5.2 TB/s; a large copy moves 5.1) with 8 x 16384 of them.
+// Weights in two parts: both maps' common part goes out of the difference, what their weights were rounded by does not.  Rounded once, outputs
+// of 4096 keys at lam = 0.5 were 1.55 times as far off as their own rounding leaves them, in f16 and in bf16, and the further the nearer the maps
+// are to each other; in two parts they are as exact as that.  4 x 4096 queries and keys, 8 heads of 64, take 590 us with it, 395 without; 8 x 1 query over 16384
+// keys 35 either way.
+// Its products and exponentials take turns more than they overlap, and the chip's power bounds both: 590 us (1160 Tflop/s of products, the second parts'
+// among them) with four waves a SIMD, for which heads of 64 make do with tiles of 32 keys and 128 registers; 640 with two.  Both maps in one wave took half as
+// long again as one map a wave.
+// Few queries are bound by their keys and values: 35 us for 178 MB (5.1 TB/s; a large copy moves 5.1) with 8 x 16384 of them.
 template <typename T, int DT, int NQ, int KT>
 __global__ __launch_bounds__(128 * NQ, DT == 32 || (DT == 64 && NQ == 4) ? 4 : 2) void attention_kernel(Args a) {
     constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT, NW = 2 * NQ;
-    // Weights go to the matrix units in the inputs' type.  bf16's 8 bits are about as far off as the output's own rounding (2.6e-3 in all
-    // where that alone is 1.7e-3); a second product with what was rounded off takes that away.  Few queries wait for their keys (8 x 16384 of
-    // them 33.8 us with it, 32.8 without); many wait for the matrix units (628 us with it, 426 without), and keep to one.
-    constexpr bool TWO = NQ == 1 && std::is_same<T, bf16>::value;
     constexpr int K_BYTES = KT * CK * 16, V_BYTES = KT * CV * 16, STAGE = 2 * K_BYTES + V_BYTES;
     static_assert(NQ * 32 * DV * 2 <= 2 * STAGE && NQ * 8192 <= 2 * STAGE, "results go through the same memory");
     __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
@@ -320,23 +317,19 @@ __global__ __launch_bounds__(128 * NQ, DT == 32 || (DT == 64 && NQ == 4) ? 4 : 2
                 sum += s[0][r];
             }
             total += sum;
-            const s16x8 pf[2] = {as_operand<T>(s[0], 0), as_operand<T>(s[0], 1)};
-            s16x8 rest[2];
-            if constexpr (TWO)
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
+            for (int x = 0; x < 2; ++x) {
+                const s16x8 pf = as_operand<T>(s[0], x);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) { const short p = pf[x][e]; s[0][8 * x + e] -= widen<T>(p); }
-                    rest[x] = as_operand<T>(s[0], x);
-                }
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
+                for (int e = 0; e < 8; ++e) { const short p = pf[e]; s[0][8 * x + e] -= widen<T>(p); }     // (exact)
+                const s16x8 rest = as_operand<T>(s[0], x);
 #pragma unroll
                 for (int v = 0; v < DV / 32; ++v) {
                     const s16x8 column = values.read(now + 2 * K_BYTES, 32 * t + 16 * x, v);
-                    acc[v] = mfma32<T>(column, pf[x], acc[v]);
-                    if constexpr (TWO) acc[v] = mfma32<T>(column, rest[x], acc[v]);
+                    acc[v] = mfma32<T>(column, pf, acc[v]);
+                    acc[v] = mfma32<T>(column, rest, acc[v]);
                 }
+            }
         }
     };
     __builtin_amdgcn_s_waitcnt(0);                          // (what came before the loop is there, or its turns would wait for as much)
@@ -346,8 +339,8 @@ __global__ __launch_bounds__(128 * NQ, DT == 32 || (DT == 64 && NQ == 4) ? 4 : 2
     }
     total = both_halves_sum(total);
 
-    int lane = l;                                           // (told apart from l, so that nothing of the row is kept through the loop)
-    asm volatile("" : "+v"(lane));
+    // (asked for anew, so that nothing of the lane and its row is kept through the loop)
+    const int lane = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)), half = lane >> 5;
     const auto [i, head, row_in] = row_of(lane);
     if (a.part) {                                           // unfinished sums of this part
         if (!row_in) return;
@@ -356,11 +349,11 @@ __global__ __launch_bounds__(128 * NQ, DT == 32 || (DT == 64 && NQ == 4) ? 4 : 2
         for (int t = 0; t < DV / 32; ++t)
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
-                const int d = 32 * t + tile_row(r, h32);
+                const int d = 32 * t + tile_row(r, half);
                 const f32x4 v = {acc[t][r], acc[t][r + 1], acc[t][r + 2], acc[t][r + 3]};
                 if (d < a.Dv) *reinterpret_cast<f32x4 *>(to + m * a.Dv + d) = v;
             }
-        if (h32 == 0) to[2 * a.Dv + m] = top, to[2 * a.Dv + 2 + m] = total;
+        if (half == 0) to[2 * a.Dv + m] = top, to[2 * a.Dv + 2 + m] = total;
         return;
     }
     const float weight = total == 0.f ? 0.f : 1.0f / total;
@@ -374,7 +367,7 @@ __global__ __launch_bounds__(128 * NQ, DT == 32 || (DT == 64 && NQ == 4) ? 4 : 2
 #pragma unroll
     for (int t = 0; t < DV / 32; t += 2) {
         tile_there<NW>();                                   // (every wave is through with what lies there)
-        f32x4 *by = reinterpret_cast<f32x4 *>(smem) + qw * 512 + l;
+        f32x4 *by = reinterpret_cast<f32x4 *>(smem) + qw * 512 + lane;
         if (m)
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
@@ -393,12 +386,12 @@ __global__ __launch_bounds__(128 * NQ, DT == 32 || (DT == 64 && NQ == 4) ? 4 : 2
     }
     char *own = smem + qw * 32 * DV * 2;
     tile_there<NW>();
-    if (!m) store_rows<T, DV>(own, (T *)a.o, at, row_in, a.Dv, l, [&](int t, int r) { return acc[t][r]; });
+    if (!m) store_rows<T, DV>(own, (T *)a.o, at, row_in, a.Dv, lane, [&](int t, int r) { return acc[t][r]; });
     if (a.o2) {
         tile_there<NW>();
-        if (m) store_rows<T, DV>(own, (T *)a.o2, at, row_in, a.Dv, l, [&](int t, int r) { return acc[t][r]; });
+        if (m) store_rows<T, DV>(own, (T *)a.o2, at, row_in, a.Dv, lane, [&](int t, int r) { return acc[t][r]; });
     }
-    if (a.lse && row_in && h32 == 0)
+    if (a.lse && row_in && half == 0)
         a.lse[((int64_t)b * 2 * a.H + 2 * head + m) * a.Nq + i] = total == 0.f ? INFINITY : top + __log2f(total);
 }
 

@@ -113,3 +113,18 @@ def test_gradients_of_peaked_rows(T, b, nq, nk, h, hk, d, dv, causal, std, dtype
     want = attention_in_64_bits(q, k, v, lam, R.visible(nq, nk, None, causal, None, b), g)
     for name, got in zip(("q", "k", "v", "lam"), torch.autograd.grad(o, leaves, g.cuda())):
         R.assert_within(got, *want[name], "d" + name)
+
+
+# ---------------------------------------------------------------------------------------------- outputs of maps that cancel
+@pytest.mark.parametrize("b,nq,nk,h,hk,d,dv", [(1, 200, 2100, 2, 1, 64, 128), (1, 40, 300, 2, 2, 128, 256), (2, 130, 130, 2, 1, 32, 64), (2, 33, 1000, 1, 1, 64, 128),
+                                               (2, 1, 3000, 4, 1, 64, 128), (1, 300, 70, 1, 1, 8, 16)])
+@pytest.mark.parametrize("std", [0.3, 1.0])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_outputs_of_maps_that_cancel(T, b, nq, nk, h, hk, d, dv, std, dtype):
+    """Both maps' common part goes out of the difference, what the weights were rounded by does not: at lam = 0.9 and nearly flat weights the
+    output is a fifth of either map's.  It is as exact as its own rounding for few queries and for many."""
+    q, k = normal(1, b, nq, 2 * h, d, dtype=dtype, std=std ** 0.5), normal(2, b, nk, 2 * hk, d, dtype=dtype, std=std ** 0.5)
+    v = normal(3, b, nk, hk, dv, dtype=dtype)
+    lam = torch.full((h,), 0.9)
+    o = T.differential_attention(*(t.cuda() for t in (q, k, v, lam)))
+    R.assert_within(o, *attention_in_64_bits(q, k, v, lam, R.visible(nq, nk, None, False, None, b))["o"], "o")
