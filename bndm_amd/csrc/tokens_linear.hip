@@ -38,13 +38,18 @@ __device__ __forceinline__ float act_value(int act, float z) {
     if (act == BNDM_ACT_GELU) return z * gauss(z).below;
     return z;
 }
+// Past +-128 both slopes are 1 and 0 to 32 bits.  The kept z may be infinite there (f16 ends at 65504, its result from 32 bits need not be), where
+// the formulas are 0 times infinity.
 __device__ __forceinline__ float act_slope(int act, float z) {
+    float slope;
     if (act == BNDM_ACT_SILU) {
         const float s = logistic(z);
-        return s * (1.0f + z * (1.0f - s));
+        slope = s * (1.0f + z * (1.0f - s));
+    } else {
+        const Gauss g = gauss(z);
+        slope = __builtin_fmaf(z, g.density, g.below);
     }
-    const Gauss g = gauss(z);
-    return __builtin_fmaf(z, g.density, g.below);
+    return fabsf(z) > 128.0f ? (z > 0.f ? 1.0f : 0.0f) : slope;    // (a NaN stays one)
 }
 
 // ---------------------------------------------------------------------------------------------- what is done with a result

@@ -128,3 +128,36 @@ def test_outputs_of_maps_that_cancel(T, b, nq, nk, h, hk, d, dv, std, dtype):
     lam = torch.full((h,), 0.9)
     o = T.differential_attention(*(t.cuda() for t in (q, k, v, lam)))
     R.assert_within(o, *attention_in_64_bits(q, k, v, lam, R.visible(nq, nk, None, False, None, b))["o"], "o")
+
+
+# ---------------------------------------------------------------------------------------------- a kept z past the range of f16
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("m,k,n", [(20, 64, 40), (300, 520, 264), (33, 5, 77)])
+def test_linear_gradients_past_the_range_of_f16(T, act, m, k, n):
+    """x W^T + b of -70000 and +100000, which f16 does not hold: slopes there are 0 and 1"""
+    x, w, dy = normal(1, m, k), normal(2, n, k, std=k ** -0.5), normal(3, m, n)
+    low, high = 3, n - 2                                     # columns
+    w[low], w[high] = 0, 0
+    w[low, 0], w[high, 0] = -35000.0, 50000.0
+    x[:, 0] = 0
+    x[5, 0] = 2.0
+    dy[:, low] *= 0.25                                       # (other rows' slopes there are about a half: their dx stays in range)
+    dy[:, high] *= 0.25
+    b = normal(4, n, std=0.1)
+    leaves = [t.cuda().requires_grad_() for t in (x, w, b)]
+    y = T.linear(*leaves, activation=act)
+    assert float(y[5, low]) == 0 and float(y[5, high]) == math.inf
+    got = torch.autograd.grad(y, leaves, dy.cuda())
+    z = x.double() @ w.double().t() + b.double()
+    _, slope, curve = R.act(act, z)
+    slope[5, low], slope[5, high] = 0, 1
+    dz = dy.double() * slope
+    # the kept z is rounded, then its slope taken, where that is neither 0 nor 1
+    u, sums = R.unit(F16), 2 * max(m, n, k) * E
+    off = dy.double().abs() * (curve * torch.where(z.abs() < 100, z.abs(), torch.zeros_like(z)) * (u + sums) + 2.0 ** -17) + u * dz.abs() + R.smallest(F16)
+    off[5, low] = 0
+    off[5, high] = u * abs(float(dy[5, high]))
+    for name, g, want, size, err in (("x", got[0], dz @ w.double(), dz.abs() @ w.double().abs(), off @ w.double().abs()),
+                                     ("w", got[1], dz.t() @ x.double(), dz.abs().t() @ x.double().abs(), off.t() @ x.double().abs()),
+                                     ("b", got[2], dz.sum(0), dz.abs().sum(0), off.sum(0))):
+        R.assert_within(g, want, err + sums * size + u * (want.abs() + err) + R.smallest(F16), "d" + name)
