@@ -246,14 +246,14 @@ __global__ __launch_bounds__(128 * NQ, DT == 32 || (DT == 64 && NQ == 4) ? 4 : 2
     Stager<KT, CV, NW, true> stage_v;
     stage_k.begin(a.kn, a.D / 8, w, l);
     stage_v.begin(a.vn, a.Dv / 8, w, l);
-    // the tile that is copied next
+    // the tile that is copied next; what lies past the last key that any of its rows sees is not read
     int j_next = j_begin;
     const T *k_next = kp + j_begin * a.kn, *v_next = vp + j_begin * a.vn;
     const int64_t k_step = KT * a.kn, v_step = KT * a.vn;
     auto fetch = [&](char *to) __attribute__((always_inline)) {
-        stage_k.copy(to, k_next, len - j_next, w);
-        stage_k.copy(to + K_BYTES, k_next + a.kh, len - j_next, w);
-        stage_v.copy(to + 2 * K_BYTES, v_next, len - j_next, w);
+        stage_k.copy(to, k_next, most - j_next, w);
+        stage_k.copy(to + K_BYTES, k_next + a.kh, most - j_next, w);
+        stage_v.copy(to + 2 * K_BYTES, v_next, most - j_next, w);
         k_next += k_step;
         v_next += v_step;
         j_next += KT;
@@ -518,9 +518,9 @@ __global__ __launch_bounds__(THREADS, DT == 32 ? 4 : DT == 64 ? 3 : 2) void atte
     stage_k.begin(a.kn, a.D / 8, w, l);
     stage_v.begin(a.vn, a.Dv / 8, w, l);
     auto fetch = [&](char *to, int j) __attribute__((always_inline)) {
-        stage_k.copy(to, kp + j * a.kn, len - j, w);
-        stage_k.copy(to + K_BYTES, kp + a.kh + j * a.kn, len - j, w);
-        stage_v.copy(to + 2 * K_BYTES, vp + j * a.vn, len - j, w);
+        stage_k.copy(to, kp + j * a.kn, j_end - j, w);
+        stage_k.copy(to + K_BYTES, kp + a.kh + j * a.kn, j_end - j, w);
+        stage_v.copy(to + 2 * K_BYTES, vp + j * a.vn, j_end - j, w);
     };
     RowReader<CK> keys;
     RowReader<CV> values;
@@ -636,9 +636,9 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
     stage_k.begin(a.kn, a.D / 8, w, l);
     stage_v.begin(a.vn, a.Dv / 8, w, l);
     auto fetch = [&](char *to, int j) __attribute__((always_inline)) {
-        stage_k.copy(to, kp + j * a.kn, len - j, w);
-        stage_k.copy(to + K_BYTES, kp + a.kh + j * a.kn, len - j, w);
-        stage_v.copy(to + 2 * K_BYTES, vp + j * a.vn, len - j, w);
+        stage_k.copy(to, kp + j * a.kn, j_end - j, w);
+        stage_k.copy(to + K_BYTES, kp + a.kh + j * a.kn, j_end - j, w);
+        stage_v.copy(to + 2 * K_BYTES, vp + j * a.vn, j_end - j, w);
     };
     RowReader<CK> keys;
     RowReader<CV> values;
@@ -720,7 +720,8 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
     const int per = a.H / a.Hk;
     // (no key or query has a number above 2^29)
     const int start = (int)max(-((int64_t)1 << 29), min((int64_t)1 << 29, start_of(a, b))), nq = (int)a.Nq;
-    const int len = (int)length_of(a, b), first_key = tile * 64, key0 = first_key + kw * 32, key = key0 + (l & 31);
+    // keys that some query sees
+    const int length = (int)length_of(a, b), len = a.causal ? max(0, min(length, start + nq)) : length, first_key = tile * 64, key0 = first_key + kw * 32, key = key0 + (l & 31);
     const bool key_in = key < len;
 
     // queries that see any key of this workgroup: from i_first on

@@ -327,7 +327,7 @@ def differential_attention(q, k, v, lam, causal=False, q_start=None, kv_lengths=
     ``kv_lengths`` int32 [B]: the keys of each sequence; what lies past them is not read, and its gradients are zero.  ``causal``:
     query i of a sequence sees keys up to ``q_start + i``; ``q_start`` int32 [B] is where its first query stands among the keys, Nk - Nq
     unless given (0 for whole sequences, the tokens before it for a step that appends to stored keys).  A query that sees no key
-    gives zeros.  Within a sequence's length, values that only later queries see must be finite numbers.
+    gives zeros.  What no query of a sequence sees may hold anything; keys and values that only its later queries see must be finite numbers.
 
     With gradients, the weights and their gradients are rounded to the tensors' type between products: f16 gradients below about
     1e-5 of a score's lose digits, so scale a loss as for any f16 training.

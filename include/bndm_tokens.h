@@ -73,7 +73,8 @@ int bndm_tokens_rotary(const void *q, const int64_t q_strides[3], void *q_out, i
  *   head h reads key head h / (H / Hk).  lam [H] of `dtype` or float.  o [B, Nq, H, Dv] contiguous.  D a multiple of 8 up to 128, Dv a
  *   multiple of 8 up to 256.  Strides {batch, token, head} are multiples of 8, pointers of 16 bytes.
  *   kv_lengths int32 [B] or NULL: keys and values past a sequence's length are not read.
- *   causal != 0: query i of sequence b sees keys j <= start_b + i, start_b = q_start[b] or, where q_start is NULL, Nk - Nq.
+ *   causal != 0: query i of sequence b sees keys j <= start_b + i, start_b = q_start[b] or, where q_start is NULL, Nk - Nq; keys past the
+ *   last query's are not read (those that only later queries than some see must be finite).
  *   A query that sees no key gives zeros, and zero gradients.
  * ------------------------------------------------------------------------------------------ */
 typedef struct bndm_attention_shape {

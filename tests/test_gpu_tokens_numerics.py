@@ -161,3 +161,28 @@ def test_linear_gradients_past_the_range_of_f16(T, act, m, k, n):
                                      ("w", got[1], dz.t() @ x.double(), dz.abs().t() @ x.double().abs(), off.t() @ x.double().abs()),
                                      ("b", got[2], dz.sum(0), dz.abs().sum(0), off.sum(0))):
         R.assert_within(g, want, err + sums * size + u * (want.abs() + err) + R.smallest(F16), "d" + name)
+
+
+# ---------------------------------------------------------------------------------------------- memory that no query sees
+@pytest.mark.parametrize("nq,nk,starts,hk,d", [(1, 700, [30, 600], 1, 64), (3, 3000, [1000, 0], 2, 64), (40, 500, [0, 100], 2, 32), (130, 900, [0, 333], 1, 64),
+                                               (70, 300, [5, 100], 2, 128), (128, 400, [0, 0], 1, 64), (5, 40, [-9, 2], 1, 64)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_keys_that_no_query_sees_are_not_read(T, nq, nk, starts, hk, d, dtype):
+    """a store of keys whose memory past the last query's place was never written, and no kv_lengths"""
+    b, h = 2, 2
+    q, k = normal(1, b, nq, 2 * h, d, dtype=dtype), normal(2, b, nk, 2 * hk, d, dtype=dtype)
+    v, g = normal(3, b, nk, hk, 2 * d, dtype=dtype), normal(4, b, nq, h, 2 * d, dtype=dtype)
+    lam = torch.tensor([0.4, 0.8])
+    seen = R.visible(nq, nk, None, True, starts, b)
+    want = R.attention(q, k, v, lam, seen, dout=g)
+    for bad in (math.nan, math.inf, -math.inf):
+        k2, v2 = k.clone(), v.clone()
+        for i, s in enumerate(starts):
+            k2[i, max(0, s + nq):] = bad
+            v2[i, max(0, s + nq):] = bad
+        leaves = [t.cuda().requires_grad_() for t in (q, k2, v2, lam)]
+        o = T.differential_attention(*leaves, causal=True, q_start=on_gpu(starts))
+        R.assert_within(o, *want["o"], f"o beside {bad}")
+        R.assert_within(T.differential_attention(*(t.detach() for t in leaves), causal=True, q_start=on_gpu(starts)), *want["o"], "o")
+        for name, got in zip(("q", "k", "v", "lam"), torch.autograd.grad(o, leaves, g.cuda())):
+            R.assert_within(got, *want[name], f"d{name} beside {bad}")
