@@ -44,6 +44,8 @@ struct Args {
     void *dq, *dk, *dv, *dlam;
     float *delta;                   // [B, 2H, Nq]: D1, D2
     float *d2_sums;                 // [H, B, runs of 32 queries, up to a multiple of 4]: sums of D2
+    float *peaks;                   // [B, H, the same runs]: the largest max(1, |lam|) |dP|
+    float *steps;                   // [B, Hk]: a power of two that dS is multiplied by on its way to the matrix units
 };
 
 // Copies tiles of R rows of C chunks into LDS, NW waves together.  Rows past rows_in and chunks past the head's size become zeros.  A lane's
@@ -474,6 +476,7 @@ __global__ __launch_bounds__(THREADS, DT == 32 ? 4 : DT == 64 ? 3 : 2) void atte
     auto upto = [&](int64_t i) { return a.causal ? (int)min((int64_t)len, max((int64_t)0, start + i + 1)) : len; };
     const int sees = row_in ? upto(i) : 0, j_end = upto(min(a.Nq - 1, (int64_t)tile * 128 + 127)), fewest = upto((int64_t)tile * 128 + w * 32);
     s16x8 qf[2][DT / 16], gf[DV / 16];
+    const float lam = lam_of<T>(a, head);
     float delta[2] = {0.f, 0.f};
     {
         const T *g = (const T *)a.dout + (int64_t)b * a.dob + i * a.don + (int64_t)head * a.doh;
@@ -494,7 +497,7 @@ __global__ __launch_bounds__(THREADS, DT == 32 ? 4 : DT == 64 ? 3 : 2) void atte
         }
         delta[0] = both_halves_sum(delta[0]);
         delta[1] = both_halves_sum(delta[1]);
-        delta[0] += lam_of<T>(a, head) * delta[1];          // (o + lam o2 is the first map's output)
+        delta[0] += lam * delta[1];                         // (o + lam o2 is the first map's output)
     }
     __builtin_amdgcn_sched_barrier(0);                      // (queries beside the outputs have no registers in heads of 128)
 #pragma unroll
@@ -506,7 +509,7 @@ __global__ __launch_bounds__(THREADS, DT == 32 ? 4 : DT == 64 ? 3 : 2) void atte
             qf[m][s] = load8(p + c * 8, row_in && c * 8 < a.D);
         }
     }
-    float lse[2], off[2] = {0.f, 0.f};
+    float lse[2], off[2] = {0.f, 0.f}, peak = 0.f;
 #pragma unroll
     for (int m = 0; m < 2; ++m) lse[m] = row_in ? a.lse[((int64_t)b * 2 * a.H + 2 * head + m) * a.Nq + i] : INFINITY;
 
@@ -536,6 +539,8 @@ __global__ __launch_bounds__(THREADS, DT == 32 ? 4 : DT == 64 ? 3 : 2) void atte
             clear(dp);
 #pragma unroll
             for (int d = 0; d < DV / 16; ++d) dp[0] = mfma32<T>(values.read(now + 2 * K_BYTES, t, d), gf[d], dp[0]);
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) peak = fmaxf(peak, fmaxf(fabsf(dp[0][r]), fabsf(dp[0][r + 1])));
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 f32x16 s[1];
@@ -570,7 +575,12 @@ __global__ __launch_bounds__(THREADS, DT == 32 ? 4 : DT == 64 ? 3 : 2) void atte
     float sum = delta[1];                                   // (0 for rows past the end)
 #pragma unroll
     for (int x = 1; x < 32; x *= 2) sum += __shfl_xor(sum, x);
-    if (l == 0) a.d2_sums[(((int64_t)head * a.B + b) * tiles + tile) * NW + w] = sum;
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) peak = fmaxf(peak, __shfl_xor(peak, x));
+    if (l == 0) {
+        a.d2_sums[(((int64_t)head * a.B + b) * tiles + tile) * NW + w] = sum;
+        a.peaks[(((int64_t)b * a.H + head) * tiles + tile) * NW + w] = peak * fmaxf(1.0f, fabsf(lam));
+    }
 }
 
 // ---------------------------------------------------------------------------------------------- gradients of the queries
@@ -608,7 +618,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
             qf[m][s] = load8(p + c * 8, row_in && c * 8 < a.D);
         }
     }
-    const float lam = lam_of<T>(a, head);
+    const float lam = lam_of<T>(a, head), step = a.steps[b * a.Hk + hk];
     {
         const T *g = (const T *)a.dout + (int64_t)b * a.dob + i * a.don + (int64_t)head * a.doh;
 #pragma unroll
@@ -622,7 +632,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
     for (int m = 0; m < 2; ++m) {
         const int64_t at = ((int64_t)b * 2 * a.H + 2 * head + m) * a.Nq + i;
         lse[m] = row_in ? a.lse[at] : INFINITY;
-        delta[m] = row_in ? a.delta[at] : 0.f;
+        delta[m] = row_in ? step * a.delta[at] : 0.f;
     }
 
     f32x16 acc[2][DT / 32];
@@ -664,7 +674,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
 #pragma unroll
                 for (int d = 0; d < DT / 16; ++d) s[0] = mfma32<T>(keys.read(now + m * K_BYTES, t, d), qf[m][d], s[0]);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[0][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], to_log2, -lse[m])) * (dp[0][r] - delta[m]);
+                for (int r = 0; r < 16; ++r) s[0][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], to_log2, -lse[m])) * __builtin_fmaf(dp[0][r], step, -delta[m]);
                 if (masked) {                               // (a row that sees one key has weight 1 there whatever its score)
                     const int n = sees == 1 ? 0 : sees - j - 32 * t - 4 * h32;
 #pragma unroll
@@ -689,7 +699,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
     char *own = smem + w * 32 * DT * 2;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-        const float f = m ? -lam * a.scale : a.scale;
+        const float f = (m ? -lam * a.scale : a.scale) / step;
         store_rows<T, DT>(own, (T *)a.dq, (((int64_t)b * a.Nq + i) * 2 * a.H + 2 * head + m) * a.D, row_in, a.D, l,
                           [&](int t, int r) { return acc[m][t][r] * f; });
     }
@@ -803,6 +813,7 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
         return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
     };
     float lam = lam_of_head(hk * per);
+    const float step = a.steps[b * a.Hk + hk];
     auto turn = [&](char *__restrict__ ahead, const char *__restrict__ now) __attribute__((always_inline)) {
         tile_there<NW>();
         if (steps > 1) fetch(ahead);
@@ -879,9 +890,9 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    if (m && !x)
+                    if (!x)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) s[1][r] *= -lam;
+                        for (int r = 0; r < 16; ++r) s[m][r] *= m ? -lam * step : step;
                     const s16x8 ds = as_operand<T>(s[m], x);
 #pragma unroll
                     for (int d = 0; d < DT / 32; ++d) dk[m][d] = mfma32<T>(query_cols[m][x][d], ds, dk[m][d]);
@@ -936,35 +947,46 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
         for (int d = 0; d < DT / 32; ++d) add(dk[0][d], dk[1][d]);
     tile_there<NW>();
     if (qw) return;
+    const float back = a.scale / step;
     char *own = smem + kw * 32 * DV * 2;
     const bool to_write = key < a.Nk;
     const int64_t at = (int64_t)b * a.Nk + (to_write ? key : 0);
     if constexpr (KEYS)
 #pragma unroll
         for (int m = 0; m < 2; ++m)
-            store_rows<T, DT>(own, (T *)a.dk, (at * 2 * a.Hk + 2 * hk + m) * a.D, to_write, a.D, l, [&](int t, int r) { return dk[m][t][r] * a.scale; });
+            store_rows<T, DT>(own, (T *)a.dk, (at * 2 * a.Hk + 2 * hk + m) * a.D, to_write, a.D, l, [&](int t, int r) { return dk[m][t][r] * back; });
     if constexpr (VALUES) store_rows<T, DV>(own, (T *)a.dv, (at * a.Hk + hk) * a.Dv, to_write, a.Dv, l, [&](int t, int r) { return dv[t][r]; });
 }
 
-// dlam[h] = - sum over sequences and queries of D2, of which each wave of the first kernel has left the sum of its 32: one workgroup a head, in a
-// fixed order.  4 us for 8 heads of 8188 queries, where reading all of D2 here took 11.
-template <typename T> __global__ __launch_bounds__(THREADS) void attention_dlam_kernel(Args a) {
+// What the kernel of the centres has left of each 32 queries, joined in a fixed order; a workgroup each.
+// dlam[h] = - sum over sequences and queries of D2.  4 us for 8 heads of 8188 queries, where reading all of D2 here took 11.
+// Behind them, for each sequence and key head: a power of two by which |dP - D| max(1, |lam|), at most twice the largest |dP|, stays within 2^15 in all its
+// queries.  dS goes to the matrix units multiplied by it: f16, which ends at 65504 and has all its digits down to 2^-14, then neither overflows nor loses
+// digits of weights above 2^-29, whatever factor the loss is scaled by.  (bf16 has the same exponents as 32 bits: to it this changes nothing.)
+template <typename T> __global__ __launch_bounds__(THREADS) void attention_totals_kernel(Args a) {
     __shared__ float part[THREADS];
-    const int head = blockIdx.x;
-    const int64_t n = (a.Nq + 127) / 128 * 4 * a.B;
-    const float *of = a.d2_sums + head * n;
-    float sum = 0.f;
-    for (int64_t i = threadIdx.x; i < n; i += THREADS) sum += of[i];
-    part[threadIdx.x] = sum;
+    const bool sums = blockIdx.x < a.H;
+    const int64_t runs = (a.Nq + 127) / 128 * 4, n = runs * (sums ? a.B : a.H / a.Hk);
+    const float *of = sums ? a.d2_sums + blockIdx.x * n : a.peaks + (blockIdx.x - a.H) * n;
+    float x = 0.f;
+    for (int64_t i = threadIdx.x; i < n; i += THREADS) x = sums ? x + of[i] : fmaxf(x, of[i]);
+    part[threadIdx.x] = x;
     __syncthreads();
-    for (int x = THREADS / 2; x > 0; x /= 2) {
-        if (threadIdx.x < x) part[threadIdx.x] += part[threadIdx.x + x];
+    for (int y = THREADS / 2; y > 0; y /= 2) {
+        if (threadIdx.x < y) {
+            const float u = part[threadIdx.x], v = part[threadIdx.x + y];
+            part[threadIdx.x] = sums ? u + v : fmaxf(u, v);
+        }
         __syncthreads();
     }
-    if (threadIdx.x == 0) {
-        if (a.lam_f32) ((float *)a.dlam)[head] = -part[0];
-        else ((T *)a.dlam)[head] = (T)(-part[0]);
-    }
+    if (threadIdx.x) return;
+    x = part[0];
+    if (!sums) {
+        int e = 0;                                          // x < 2^e
+        if (x > 0.f && x <= 3.4e38f) frexpf(x, &e);
+        a.steps[blockIdx.x - a.H] = ldexpf(1.0f, min(100, max(-100, 14 - e)));
+    } else if (a.lam_f32) ((float *)a.dlam)[blockIdx.x] = -x;
+    else ((T *)a.dlam)[blockIdx.x] = (T)-x;
 }
 
 // ---------------------------------------------------------------------------------------------- host side
@@ -1029,16 +1051,15 @@ template <typename T, int DT> int backward(const Args &a, hipStream_t stream) {
     const int64_t nq = ceil_div64(a.Nq, 128) * a.H * a.B;
     hipLaunchKernelGGL((attention_delta_kernel<T, DT, 32>), dim3((unsigned)nq), dim3(THREADS), 0, stream, a);
     if (int rc = tokens_launch_status("attention delta")) return rc;
+    hipLaunchKernelGGL((attention_totals_kernel<T>), dim3((unsigned)(a.H + a.B * a.Hk)), dim3(THREADS), 0, stream, a);
+    if (int rc = tokens_launch_status("attention totals")) return rc;
     hipLaunchKernelGGL((attention_dq_kernel<T, DT, KT>), dim3((unsigned)nq), dim3(THREADS), 0, stream, a);
     if (int rc = tokens_launch_status("attention dq")) return rc;
-    if (a.Nk > 0) {
-        if constexpr (DT == 128) {
-            if (int rc = launch_dkv<T, DT, 1>(a, stream)) return rc;
-            if (int rc = launch_dkv<T, DT, 2>(a, stream)) return rc;
-        } else if (int rc = launch_dkv<T, DT, 3>(a, stream)) return rc;
-    }
-    hipLaunchKernelGGL((attention_dlam_kernel<T>), dim3(a.H), dim3(THREADS), 0, stream, a);
-    return tokens_launch_status("attention dlam");
+    if (a.Nk == 0) return 0;
+    if constexpr (DT == 128) {
+        if (int rc = launch_dkv<T, DT, 1>(a, stream)) return rc;
+        return launch_dkv<T, DT, 2>(a, stream);
+    } else return launch_dkv<T, DT, 3>(a, stream);
 }
 
 int check(const char *what, const bndm_attention_shape *s) {
@@ -1107,7 +1128,7 @@ extern "C" int bndm_tokens_attention(const bndm_attention_shape *s, const void *
 
 extern "C" size_t bndm_tokens_attention_backward_workspace_bytes(const bndm_attention_shape *s) {
     if (check("bndm_tokens_attention_backward_workspace_bytes", s)) return 0;
-    return (size_t)s->B * s->H * (2 * s->Nq + ceil_div64(s->Nq, 128) * 4) * 4;
+    return ((size_t)s->B * s->H * (2 * s->Nq + ceil_div64(s->Nq, 128) * 8) + s->B * s->Hk) * 4;
 }
 
 extern "C" int bndm_tokens_attention_backward(const bndm_attention_shape *s, const void *q, const void *k, const void *v, const void *lam,
@@ -1128,7 +1149,9 @@ extern "C" int bndm_tokens_attention_backward(const bndm_attention_shape *s, con
     Args a = args_of(s, q, k, v, lam, q_start, kv_lengths);
     a.o = (void *)o, a.o2 = (void *)o2, a.lse = (float *)lse;
     a.dout = dout, a.dob = dout_strides[0], a.don = dout_strides[1], a.doh = dout_strides[2];
-    a.dq = dq, a.dk = dk, a.dv = dv, a.dlam = dlam, a.delta = (float *)workspace, a.d2_sums = a.delta + 2 * s->B * s->H * s->Nq;
+    const int64_t runs = s->B * s->H * ceil_div64(s->Nq, 128) * 4;
+    a.dq = dq, a.dk = dk, a.dv = dv, a.dlam = dlam;
+    a.delta = (float *)workspace, a.d2_sums = a.delta + 2 * s->B * s->H * s->Nq, a.peaks = a.d2_sums + runs, a.steps = a.peaks + runs;
     const int d = padded(s->D, s->Dv);
     const hipStream_t st = (hipStream_t)stream;
     if (s->dtype == BNDM_DTYPE_F16) return d == 32 ? backward<f16, 32>(a, st) : d == 64 ? backward<f16, 64>(a, st) : backward<f16, 128>(a, st);

@@ -329,8 +329,8 @@ def differential_attention(q, k, v, lam, causal=False, q_start=None, kv_lengths=
     unless given (0 for whole sequences, the tokens before it for a step that appends to stored keys).  A query that sees no key
     gives zeros.  What no query of a sequence sees may hold anything; keys and values that only its later queries see must be finite numbers.
 
-    With gradients, the weights and their gradients are rounded to the tensors' type between products: f16 gradients below about
-    1e-5 of a score's lose digits, so scale a loss as for any f16 training.
+    In the backward pass weights and their gradients are rounded to the tensors' type between products, the gradients as parts of the
+    largest of their sequence and key head, so that f16 gradients lose nothing to a loss's factor but what q, k, v's own gradients do.
     """
     dtype = _type_of("differential_attention(q)", q, _HALVES)
     qs, ks, vs = tuple(q.shape), tuple(k.shape), tuple(v.shape)

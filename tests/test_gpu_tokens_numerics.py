@@ -163,6 +163,39 @@ def test_linear_gradients_past_the_range_of_f16(T, act, m, k, n):
         R.assert_within(g, want, err + sums * size + u * (want.abs() + err) + R.smallest(F16), "d" + name)
 
 
+# ---------------------------------------------------------------------------------------------- gradients of weights past the range of f16
+def test_weight_gradients_past_the_range_of_f16(T):
+    """dS reaches past 65504, scale dS does not"""
+    b, nq, nk, h, d, dv = 1, 6, 3, 2, 64, 128
+    q, k = normal(1, b, nq, 2 * h, d, std=0.25), normal(2, b, nk, 2 * h, d, std=0.25)
+    v, g = normal(3, b, nk, h, dv, std=250.0), normal(4, b, nq, h, dv, std=200.0)
+    lam = torch.tensor([0.4, 0.8])
+    want = attention_in_64_bits(q, k, v, lam, R.visible(nq, nk, None, False, None, b), g)
+    assert all(float(want[name][0].abs().max()) < 65504 for name in "qkv")
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v, lam)]
+    o = T.differential_attention(*leaves)
+    for name, got in zip(("q", "k", "v", "lam"), torch.autograd.grad(o, leaves, g.cuda())):
+        R.assert_within(got, *want[name], "d" + name)
+
+
+@pytest.mark.parametrize("nq,nk,hk,d,causal", [(40, 300, 1, 64, False), (200, 200, 2, 32, True), (33, 70, 2, 128, False)])
+def test_gradients_follow_the_factor_of_the_loss(T, nq, nk, hk, d, causal):
+    """A loss times a power of two: every gradient times that, bit for bit, but for what f16 cannot hold of the gradients themselves.  dS, a
+    thousandth of them, is not what runs out of digits first."""
+    b, h = 2, 2
+    q, k, v = normal(1, b, nq, 2 * h, d), normal(2, b, nk, 2 * hk, d), normal(3, b, nk, hk, 2 * d)
+    g = normal(4, b, nq, h, 2 * d)
+    g = torch.where(g.abs() < 0.01, torch.full_like(g, 0.01), g)       # (none leaves f16's normal range below)
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v, torch.tensor([0.4, 1.8]))]
+    grads = lambda factor: torch.autograd.grad(T.differential_attention(*leaves, causal=causal), leaves, (g * factor).cuda())
+    one = grads(1.0)
+    for factor in (2.0 ** -6, 2.0 ** 8):
+        for name, a, c in zip(("q", "k", "v", "lam"), grads(factor), one):
+            want = c.double() * factor
+            least = R.smallest(F16) * max(1.0, factor) if a.dtype == F16 else 0.0
+            assert ((a.double() - want).abs() <= least).all(), name
+
+
 # ---------------------------------------------------------------------------------------------- memory that no query sees
 @pytest.mark.parametrize("nq,nk,starts,hk,d", [(1, 700, [30, 600], 1, 64), (3, 3000, [1000, 0], 2, 64), (40, 500, [0, 100], 2, 32), (130, 900, [0, 333], 1, 64),
                                                (70, 300, [5, 100], 2, 128), (128, 400, [0, 0], 1, 64), (5, 40, [-9, 2], 1, 64)])
