@@ -7,14 +7,17 @@
 Tensors are laid out token by token, ``[batch, tokens, heads, size]``, as a projection leaves them; slices of a packed projection are
 taken as they are.  All three have gradients (once, not twice) and run on the current stream of their tensors' device; what they need
 beside their results is allocated through torch for the one call, so they can be captured into graphs.  Storage is f16 or bf16
-(``rotary`` also f32), sums and statistics are 32 bits.  There is no CPU fallback.
+(``rotary`` also f32), sums and statistics are 32 bits.  There is no CPU fallback.  Forward-mode derivatives, tracers (``torch.jit.trace``,
+``make_fx``) are refused.
 """
 from __future__ import annotations
 
 import ctypes as C
 import functools
+import sys
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -46,6 +49,21 @@ def _launch(fn, what, index, *args):
 
 def _ptr(t):
     return 0 if t is None else t.data_ptr()
+
+
+def _refuse_onlookers(what, *tensors):
+    """The kernels take addresses, so what follows torch's operators by watching them would miss these: a tangent would end here and count
+    as zero, a recorded graph would hold the allocation of the result and nothing that fills it."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what}: no forward-mode derivatives")
+    tracing = torch._C._is_tracing()
+    if torch._C._len_torch_dispatch_stack() or torch._C._len_torch_function_stack():    # (or no tracer of torch.fx is at work: 2 us saved)
+        proxies = sys.modules.get("torch.fx.experimental.proxy_tensor")                 # (loaded by whoever traces)
+        tracing = tracing or (proxies is not None and proxies.get_proxy_mode() is not None)
+    if tracing:
+        raise NotImplementedError(f"{what}: a tracer would record its allocations only")
 
 
 def _same(what, first, others):
@@ -116,6 +134,7 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _refuse_onlookers("linear backward", dy)
         x, weight, z = ctx.saved_tensors
         n, k = weight.shape
         want_x, want_w, want_b, want_r = ctx.needs_input_grad[:4]
@@ -141,6 +160,7 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     ``"gelu"`` (z Phi(z)).  Returns [..., N].  With an activation, a pass that records gradients keeps x weight^T + bias in the
     tensors' type for the backward pass.
     """
+    _refuse_onlookers("linear", x, weight, bias, residual)
     dtype = _type_of("linear(x)", x, _HALVES)
     act = _ACTIVATIONS.get(activation)
     if act is None:
@@ -204,6 +224,7 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dq, dk=None):
+        _refuse_onlookers("rotary backward", dq, dk)
         sections, base, interleaved, dtype = ctx.how
         dq = dq if ctx.needs_input_grad[0] else None
         dk = dk if ctx.needs_input_grad[1] else None
@@ -221,6 +242,7 @@ def rotary(q, k, positions, sections, base=10000.0, interleaved=False):
     of an axis with s pairs turns by ``position * base ** (-i / s)``, an angle formed in 64 bits.  Pairs are elements (j, j + D / 2), or
     (2j, 2j + 1) with ``interleaved``.  Returns new tensors: (q', k'), or q' alone where k is None.
     """
+    _refuse_onlookers("rotary", q, k, positions)
     dtype = _type_of("rotary(q)", q, _FLOATS)
     shape, other, where = tuple(q.shape), None if k is None else tuple(k.shape), tuple(positions.shape)
     if len(shape) != 4 or (k is not None and (len(other) != 4 or other[:2] != shape[:2] or other[3] != shape[3])):
@@ -288,6 +310,7 @@ class _DifferentialAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
+        _refuse_onlookers("differential_attention backward", dout)
         q, k, v, lam, q_start, kv_lengths, o, o2, lse = ctx.saved_tensors
         causal, scale, dtype = ctx.how
         dq, dk, dv, dlam = (t.new_empty(t.shape) for t in (q, k, v, lam))
@@ -332,6 +355,7 @@ def differential_attention(q, k, v, lam, causal=False, q_start=None, kv_lengths=
     In the backward pass weights and their gradients are rounded to the tensors' type between products, the gradients as parts of the
     largest of their sequence and key head, so that f16 gradients lose nothing to a loss's factor but what q, k, v's own gradients do.
     """
+    _refuse_onlookers("differential_attention", q, k, v, lam)
     dtype = _type_of("differential_attention(q)", q, _HALVES)
     qs, ks, vs = tuple(q.shape), tuple(k.shape), tuple(v.shape)
     if len(qs) != 4 or len(ks) != 4 or len(vs) != 4 or qs[0] != ks[0] or ks[:2] != vs[:2] or qs[3] != ks[3] or qs[3] < 1 or vs[2] < 1 or \

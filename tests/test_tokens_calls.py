@@ -1,0 +1,77 @@
+"""CPU checks of bndm_amd.tokens' Python side: calls whose results would be wrong in silence are refused before anything is launched.  Where a call
+has to get past the device check, the launch is replaced by one that only counts."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+F16 = torch.float16
+
+
+@pytest.fixture
+def T(monkeypatch):
+    """bndm_amd.tokens with CPU tensors let through and nothing launched; T.launches names the calls"""
+    from bndm_amd import tokens
+    monkeypatch.setattr(tokens, "_type_of", lambda what, t, types: types[t.dtype])
+    monkeypatch.setattr(tokens, "launches", [], raising=False)
+    monkeypatch.setattr(tokens, "_launch", lambda fn, what, index, *args: tokens.launches.append((what, *args)))
+    return tokens
+
+
+def calls(T):
+    """name -> (call of one tensor, that tensor)"""
+    zeros = lambda *shape: torch.zeros(*shape, dtype=F16)
+    w, pos = zeros(24, 16), torch.zeros(5, 2, dtype=torch.int32)
+    k, v, lam = zeros(2, 5, 2, 16), zeros(2, 5, 1, 32), zeros(2)
+    return {"linear": (lambda t: T.linear(t, w, activation="silu"), zeros(3, 16)), "rotary": (lambda t: T.rotary(t, None, pos, (4, 4)), zeros(2, 5, 4, 16)),
+            "differential_attention": (lambda t: T.differential_attention(t, k, v, lam), zeros(2, 5, 4, 16))}
+
+
+OPERATORS = ["linear", "rotary", "differential_attention"]
+
+
+# ---------------------------------------------------------------------------------------------- who follows torch's operators misses these
+@pytest.mark.parametrize("name", OPERATORS)
+@pytest.mark.parametrize("leaf", [False, True])
+def test_forward_mode_is_refused(T, name, leaf):
+    call, x = calls(T)[name]
+    with forward_ad.dual_level():
+        call(x)                                              # (a tensor without a tangent is one like any other)
+        before = len(T.launches)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(forward_ad.make_dual(x.clone().requires_grad_(leaf), torch.ones_like(x)))
+        assert len(T.launches) == before
+        other = x.clone().requires_grad_()
+        y = call(other)
+        before = len(T.launches)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(y, other, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
+        assert len(T.launches) == before
+    call(x)
+
+
+def test_forward_mode_of_any_input_is_refused(T):
+    x, w, b, r = (torch.zeros(*s, dtype=F16) for s in ((3, 16), (24, 16), (24,), (3, 24)))
+    q, k, v, lam = (torch.zeros(*s, dtype=F16) for s in ((2, 5, 4, 16), (2, 5, 2, 16), (2, 5, 1, 32), (2,)))
+    pos = torch.zeros(5, 2, dtype=torch.int32)
+    for call, tensors in ((lambda x, w, b, r: T.linear(x, w, b, residual=r), [x, w, b, r]), (lambda q, k: T.rotary(q, k, pos, (4, 4)), [q, k]),
+                          (T.differential_attention, [q, k, v, lam])):
+        for at, t in enumerate(tensors):
+            with forward_ad.dual_level():
+                some = list(tensors)
+                some[at] = forward_ad.make_dual(t, torch.ones_like(t))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(*some)
+    assert T.launches == []
+
+
+@pytest.mark.parametrize("name", OPERATORS)
+def test_tracers_are_refused(T, name):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call, x = calls(T)[name]
+    for trace in (lambda: torch.jit.trace(call, (x,), check_trace=False), lambda: make_fx(call)(x), lambda: make_fx(call, pre_dispatch=True)(x),
+                  lambda: make_fx(call, tracing_mode="fake")(x)):
+        with pytest.raises(NotImplementedError, match="tracer"):
+            trace()
+    assert T.launches == []
+    call(x)
+    assert len(T.launches) == 1
