@@ -8,7 +8,7 @@ Tensors are laid out token by token, ``[batch, tokens, heads, size]``, as a proj
 taken as they are.  All three have gradients (once, not twice) and run on the current stream of their tensors' device; what they need
 beside their results is allocated through torch for the one call, so they can be captured into graphs.  Storage is f16 or bf16
 (``rotary`` also f32), sums and statistics are 32 bits.  There is no CPU fallback.  Forward-mode derivatives, tracers (``torch.jit.trace``,
-``make_fx``) are refused.
+``make_fx``) and tensors without memory of their own are refused.
 """
 from __future__ import annotations
 
@@ -48,7 +48,13 @@ def _launch(fn, what, index, *args):
 
 
 def _ptr(t):
-    return 0 if t is None else t.data_ptr()
+    """An optional tensor's address: 0 stands for none, which a tensor without memory (a wrapper) must not pass for."""
+    if t is None:
+        return 0
+    at = t.data_ptr()
+    if not at and t.numel():
+        raise NotImplementedError(f"{type(t).__name__} has no memory of its own for a kernel to read")
+    return at
 
 
 def _refuse_onlookers(what, *tensors):

@@ -75,3 +75,26 @@ def test_tracers_are_refused(T, name):
     assert T.launches == []
     call(x)
     assert len(T.launches) == 1
+
+
+def test_optional_tensors_without_memory_are_refused(T):
+    """an address of 0 stands for none"""
+    class Wrapper(torch.Tensor):
+        @staticmethod
+        def __new__(cls, shape, dtype):
+            return torch.Tensor._make_wrapper_subclass(cls, shape, dtype=dtype)
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            if func is torch.ops.aten.detach.default:
+                return args[0]
+            raise AssertionError(func)
+
+    x, w = torch.zeros(3, 16, dtype=F16), torch.zeros(24, 16, dtype=F16)
+    with pytest.raises(NotImplementedError, match="no memory"):
+        T.linear(x, w, Wrapper((24,), F16))
+    q, k, v, lam = (torch.zeros(*s, dtype=F16) for s in ((2, 5, 4, 16), (2, 5, 2, 16), (2, 5, 1, 32), (2,)))
+    for name in ("q_start", "kv_lengths"):
+        with pytest.raises(NotImplementedError, match="no memory"):
+            T.differential_attention(q, k, v, lam, causal=True, **{name: Wrapper((2,), torch.int32)})
+    assert T.launches == []
