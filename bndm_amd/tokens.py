@@ -99,14 +99,14 @@ def _recording(*tensors):
 
 # ---------------------------------------------------------------------------------------------- linear
 def _rows(t, width):
-    """``t`` as rows of ``width`` next to each other's elements, their number, and the distance of two rows."""
+    """``t`` as rows of ``width`` next to each other's elements, their number, and the distance of two rows, which the kernels take up to 2^22."""
     if t.dim() != 2:
         t = t.reshape(-1, width)
     step, inner = t.stride()
-    if inner != 1 and width > 1:
+    m = t.shape[0]
+    if (inner != 1 and width > 1) or (step > 1 << 22 and m > 1):
         t = t.contiguous()
         step = width
-    m = t.shape[0]
     return t, m, step if m > 1 else width
 
 

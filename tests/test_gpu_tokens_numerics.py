@@ -219,3 +219,27 @@ def test_keys_that_no_query_sees_are_not_read(T, nq, nk, starts, hk, d, dtype):
         R.assert_within(T.differential_attention(*(t.detach() for t in leaves), causal=True, q_start=on_gpu(starts)), *want["o"], "o")
         for name, got in zip(("q", "k", "v", "lam"), torch.autograd.grad(o, leaves, g.cuda())):
             R.assert_within(got, *want[name], f"d{name} beside {bad}")
+
+
+# ---------------------------------------------------------------------------------------------- rows that lie far apart
+def test_linear_rows_far_apart(T):
+    """the last token of each long sequence: rows 2^23 elements apart; gradients that arrive so"""
+    h = torch.zeros(6, (1 << 23) + 24, dtype=F16, device="cuda")
+    for m, k, n in ((6, 512, 72), (6, 517, 72), (5, 24, 300)):
+        for start in (0, 3):
+            x, w, b = normal(1, m, k), normal(2, n, k, std=k ** -0.5), normal(3, n)
+            h[:m, start : start + k] = x.cuda()
+            rows = h[:m, start : start + k]
+            y = T.linear(rows, w.cuda(), b.cuda())
+            R.assert_within(y, *R.linear(x, w, b, None, None, F16), "y")
+            leaves = [rows.detach().requires_grad_(), w.cuda().requires_grad_(), b.cuda().requires_grad_()]
+            y = T.linear(*leaves, activation="silu")
+            dy = normal(4, m, n)
+            far = torch.zeros(m, (1 << 22) + 8, dtype=F16, device="cuda")[:, 1 : 1 + n].copy_(dy)
+            got = torch.autograd.grad(y, leaves, far)
+            for name, g in zip("xwb", got):
+                R.assert_within(g, *R.linear_gradients(x, w, b, "silu", dy, F16)[name], "d" + name)
+    tiles = torch.zeros(150, 1 << 23, dtype=F16, device="cuda")[:, 8:2056]          # as many rows as the large tiles take
+    x, w = normal(5, 150, 2048), normal(6, 264, 2048, std=0.02)
+    tiles.copy_(x)
+    R.assert_within(T.linear(tiles, w.cuda()), *R.linear(x, w, None, None, None, F16), "y")

@@ -98,3 +98,22 @@ def test_optional_tensors_without_memory_are_refused(T):
         with pytest.raises(NotImplementedError, match="no memory"):
             T.differential_attention(q, k, v, lam, causal=True, **{name: Wrapper((2,), torch.int32)})
     assert T.launches == []
+
+
+# ---------------------------------------------------------------------------------------------- rows and numbers that the kernels do not take as they are
+def test_linear_rows_further_apart_than_the_kernels_take(T):
+    """the last token of each of some long sequences; a gradient that arrives so"""
+    far = (1 << 22) + 1
+    h = torch.empty(3, far, dtype=F16)
+    h[:, -16:] = torch.arange(48, dtype=F16).reshape(3, 16)
+    w = torch.zeros(24, 16, dtype=F16).requires_grad_()
+    y = T.linear(h[:, -16:], w)
+    grad = h[:, -24:]
+    torch.autograd.grad(y, w, grad)
+    T.linear(h[:, -16:].detach(), w.detach(), residual=h[:, -24:])
+    (_, x, ldx, *_), (_, dy, lddy, _, x2, ldx2, *_), (_, *last) = T.launches
+    assert (ldx, lddy, ldx2, last[1], last[5]) == (16, 24, 16, 16, 24)
+    assert T._rows(h[:, -16:], 16)[0].equal(h[:, -16:]) and T._rows(h[:1, -16:], 16)[0].data_ptr() == h[:1, -16:].data_ptr()
+    near = torch.empty(2, 1 << 22, dtype=F16)
+    rows, m, step = T._rows(near[:, 8:24], 16)
+    assert rows.data_ptr() == near[:, 8:24].data_ptr() and (m, step) == (2, 1 << 22)
