@@ -343,7 +343,9 @@ def _per_sequence(what, t, q):
         return None
     if t.shape != (q.shape[0],) or t.get_device() != q.get_device() or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"differential_attention: {what} is {t.dtype} {tuple(t.shape)} on {t.device}: int32 ({q.shape[0]},) on {q.device}")
-    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+    if t.dtype is torch.int64:
+        t = t.clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32)      # (further out than any key either way: wrapped, it would be among them)
+    return t.contiguous()
 
 
 def differential_attention(q, k, v, lam, causal=False, q_start=None, kv_lengths=None, scale=None):
@@ -353,8 +355,8 @@ def differential_attention(q, k, v, lam, causal=False, q_start=None, kv_lengths=
     multiple of Hk, head h reads key head h // (H // Hk).  f16 or bf16; D a multiple of 8 up to 128, Dv up to 256.  lam [H], of the same
     type or float32.  ``scale``: 1 / sqrt(D) unless given, positive.  Returns [B, Nq, H, Dv].
 
-    ``kv_lengths`` int32 [B]: the keys of each sequence; what lies past them is not read, and its gradients are zero.  ``causal``:
-    query i of a sequence sees keys up to ``q_start + i``; ``q_start`` int32 [B] is where its first query stands among the keys, Nk - Nq
+    ``kv_lengths`` int32 (or int64) [B]: the keys of each sequence; what lies past them is not read, and its gradients are zero.  ``causal``:
+    query i of a sequence sees keys up to ``q_start + i``; ``q_start``, likewise, is where its first query stands among the keys, Nk - Nq
     unless given (0 for whole sequences, the tokens before it for a step that appends to stored keys).  A query that sees no key
     gives zeros.  What no query of a sequence sees may hold anything; keys and values that only its later queries see must be finite numbers.
 

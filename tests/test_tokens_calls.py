@@ -117,3 +117,14 @@ def test_linear_rows_further_apart_than_the_kernels_take(T):
     near = torch.empty(2, 1 << 22, dtype=F16)
     rows, m, step = T._rows(near[:, 8:24], 16)
     assert rows.data_ptr() == near[:, 8:24].data_ptr() and (m, step) == (2, 1 << 22)
+
+
+def test_places_past_32_bits(T):
+    """int64 lengths and starts beyond 32 bits ("all of them") stay on their side of every key"""
+    q = torch.zeros(4, 1, 2, 16, dtype=F16)
+    big = torch.tensor([2 ** 63 - 1, 2 ** 32 + 5, -2 ** 40, 7])
+    assert T._per_sequence("kv_lengths", big, q).tolist() == [2 ** 31 - 1, 2 ** 31 - 1, -2 ** 31, 7]
+    same = torch.tensor([1, 2, 3, 4], dtype=torch.int32)
+    assert T._per_sequence("q_start", same, q) is same
+    wide = torch.tensor([[1, 2, 3, 4], [5, 6, 7, 8]], dtype=torch.int32).t()[:, 0]
+    assert T._per_sequence("q_start", wide, q).tolist() == [1, 2, 3, 4] and T._per_sequence("q_start", wide, q).is_contiguous()
