@@ -532,7 +532,7 @@ BUILDERS["s_cbranch_execnz"] = _cbr(lambda w: (w.s[EXEC] | w.s[EXEC + 1]) != 0)
 
 
 @op("s_nop", "s_setprio", "s_sleep", "s_sethalt", "s_setkill", "s_inst_prefetch", "s_clause", "s_code_end", "s_icache_inv",
-    "s_dcache_wb", "s_dcache_inv", "buffer_wbl2", "buffer_inv", "s_ttracedata", "s_incperflevel", "s_decperflevel")
+    "s_dcache_inv", "buffer_wbl2", "buffer_inv", "s_ttracedata", "s_incperflevel", "s_decperflevel")
 def _(ins):
     return lambda w: None
 
