@@ -243,3 +243,20 @@ def test_linear_rows_far_apart(T):
     x, w = normal(5, 150, 2048), normal(6, 264, 2048, std=0.02)
     tiles.copy_(x)
     R.assert_within(T.linear(tiles, w.cuda()), *R.linear(x, w, None, None, None, F16), "y")
+
+
+# ---------------------------------------------------------------------------------------------- sums in 32 bits
+@pytest.mark.parametrize("m,k,n", [(5, 8192, 40), (40, 4100, 72), (130, 8192, 264), (2056, 2048, 264), (257, 515, 300), (100, 7, 70), (4104, 264, 2312)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_linear_sums_of_whole_numbers(T, m, k, n, dtype):
+    """Whole numbers up to 3: every sum is one below 2^24, which 32 bits hold exactly and fewer do not, so that the result is the rounded sum,
+    bit for bit; gradients likewise."""
+    g = torch.Generator().manual_seed(m)
+    whole = lambda *shape: torch.randint(-3, 4, shape, generator=g).to(dtype).cuda()
+    x, w, b, r, dy = whole(m, k).requires_grad_(), whole(n, k).requires_grad_(), whole(n).requires_grad_(), whole(m, n), whole(m, n)
+    y = T.linear(x, w, b, residual=r)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    wide = lambda t: t.detach().double().cpu()
+    X, W, D = wide(x), wide(w), wide(dy)
+    for got, want in ((y, X @ W.t() + wide(b) + wide(r)), (dx, D @ W), (dw, D.t() @ X), (db, D.sum(0))):
+        assert torch.equal(got.cpu(), want.to(dtype))
