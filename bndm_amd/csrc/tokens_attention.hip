@@ -1144,6 +1144,7 @@ extern "C" int bndm_tokens_attention_backward(const bndm_attention_shape *s, con
     for (int i = 0; i < 3; ++i)
         TOKENS_REQUIRE(dout_strides[i] >= 0 && dout_strides[i] % 8 == 0 && (i != 1 || dout_strides[i] <= (1 << 23)),
                        "bndm_tokens_attention_backward: stride %lld: a multiple of 8, between tokens up to 2^23", (long long)dout_strides[i]);
+    TOKENS_REQUIRE(s->H + s->B * s->Hk < (1 << 24), "bndm_tokens_attention_backward: more heads than a launch takes");
     const size_t need = bndm_tokens_attention_backward_workspace_bytes(s);
     TOKENS_REQUIRE(workspace && workspace_bytes >= need, "bndm_tokens_attention_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     Args a = args_of(s, q, k, v, lam, q_start, kv_lengths);

@@ -128,3 +128,20 @@ def test_places_past_32_bits(T):
     assert T._per_sequence("q_start", same, q) is same
     wide = torch.tensor([[1, 2, 3, 4], [5, 6, 7, 8]], dtype=torch.int32).t()[:, 0]
     assert T._per_sequence("q_start", wide, q).tolist() == [1, 2, 3, 4] and T._per_sequence("q_start", wide, q).is_contiguous()
+
+
+def test_more_heads_than_a_launch_takes():
+    """the backward pass has a workgroup for each head and for each sequence's key heads in one launch"""
+    from bndm_amd import _lib
+    lib, P = _lib.load_tokens(), 4096                        # (4096 stands for a tensor: refused before any is read)
+    b = (1 << 20) - 1
+    strides = (16 * 32, 16 * 32, 16)
+    shape = _lib.AttentionShape(b, 1, 1, 16, 16, 16, 16, *strides, *strides, *strides, 0, 0, 0, 0.25)
+    need = lib.bndm_tokens_attention_backward_workspace_bytes(shape)
+    rc = lib.bndm_tokens_attention_backward(shape, P, P, P, P, 0, 0, P, P, P, P, strides_of(strides), P, P, P, P, P, need, None)
+    assert rc == -1 and b"more heads" in lib.bndm_tokens_last_error()
+
+
+def strides_of(values):
+    import ctypes
+    return (ctypes.c_int64 * 3)(*values)
