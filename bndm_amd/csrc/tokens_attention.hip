@@ -106,7 +106,7 @@ template <int C, bool COLUMNS = false> struct ColumnReader {       // operand wh
 // Workgroups go to the 8 XCDs in turn.  This deals out heads (the units that share keys, `tiles` workgroups each) to the XCDs, so that one's
 // workgroups run behind one L2, and within a head the last tile first: with a causal mask it is the longest.  An XCD's second 32
 // workgroups begin beside its first 32, one on each of its CUs: every other 32 go the other way, so that long ones meet short ones (the
-// forward pass of 4 x 2047 causal tokens of ragged lengths and 8 heads 70 us, 79 without; the queries' gradients 86 and 93).
+// forward pass of 4 x 2047 causal tokens of ragged lengths and 8 heads 97 us, 114 without; the queries' gradients 73 and 81).
 __device__ __forceinline__ void place(int id, int units, int tiles, int &unit, int &tile) {
     const int even = units & ~7;
     if (id < even * tiles) {
@@ -201,7 +201,8 @@ __device__ __forceinline__ int64_t length_of(const Args &a, int b) {
 // are to each other; in two parts they are as exact as that.  4 x 4096 queries and keys, 8 heads of 64, take 590 us with it, 395 without; 8 x 1 query over 16384
 // keys 35 either way.
 // Its products and exponentials take turns more than they overlap, and the chip's power bounds both: 590 us (1160 Tflop/s of products, the second parts'
-// among them) with four waves a SIMD, for which heads of 64 make do with tiles of 32 keys and 128 registers; 640 with two.  Both maps in one wave took half as
+// among them) with four waves a SIMD, for which heads of 64 make do with tiles of 32 keys and 128 registers; 640 with two.  (8192 causal tokens of one
+// sequence, 8 heads: 347 and 372.)  Both maps in one wave took half as
 // long again as one map a wave.
 // Few queries are bound by their keys and values: 35 us for 178 MB (5.1 TB/s; a large copy moves 5.1) with 8 x 16384 of them.
 template <typename T, int DT, int NQ, int KT>
@@ -453,7 +454,7 @@ template <typename T> __global__ __launch_bounds__(512) void attention_join_kern
 // is off by is what dq shows: from outputs rounded to 16 bits, D' = do . o_m, scores of deviation 6 gave a bf16 dq as far off as it is long.
 // So a pass over the keys forms  D_m = D' + sum_j P_mj (dP_j - D')  in 32 bits.  (Of the differences: what log-sum-exp of large scores is
 // off by makes the weights' sum 1 + e, and counts here as e (D - D'), not as e D.)
-// 70 us for 4 x 2047 causal tokens and 8 heads of 64 over 128 of ragged lengths (21 Gflop, 300 Tflop/s): exponentials, the arithmetic around
+// 68 us for 4 x 2047 causal tokens and 8 heads of 64 over 128 of ragged lengths (21 Gflop, 300 Tflop/s): exponentials, the arithmetic around
 // them and the products take about as long as one another, and three waves a SIMD run them beside one another.  Done in the next kernel, with the registers that its
 // sums hold, it took as long with two.
 template <typename T, int DT, int KT>
@@ -585,7 +586,7 @@ __global__ __launch_bounds__(THREADS, DT == 32 ? 4 : DT == 64 ? 3 : 2) void atte
 
 // ---------------------------------------------------------------------------------------------- gradients of the queries
 // As the forward pass: a lane holds one query, dS^T is at once the right operand of  dq^T += k^T dS^T.
-// 71 us for 4 x 2047 causal tokens and 8 heads of 64 over 128 of ragged lengths (31 Gflop, 440 Tflop/s): half of a wave's time goes to
+// 68 us for 4 x 2047 causal tokens and 8 heads of 64 over 128 of ragged lengths (31 Gflop, 460 Tflop/s): half of a wave's time goes to
 // exponentials and the arithmetic between the products.
 template <typename T, int DT, int KT>
 __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 128 ? 1 : 2, DT == 128 ? 1 : 2))) void attention_dq_kernel(Args a) {
@@ -710,9 +711,9 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
 // of  dv^T += do^T W  and  dk_m^T += q_m^T dS_m.  A workgroup owns 64 keys, whose operands stay in registers while the queries of every
 // head that reads them pass through LDS, 64 at a time, so shared heads' gradients are summed here.  Two waves take the first half of the
 // queries in a tile, two the second; their sums are added at the end, in order.
-// WHAT: 1 dv, 2 dk, 3 both.  Both need 450 registers for heads of 128: there dv and dk are summed by a launch each.
-// 120 us for 4 x 2047 causal tokens, 8 heads of 64 over 128 and 4 key heads, ragged (41 Gflop, 340 Tflop/s), bound like the kernel above; one wave
-// a SIMD, because dk, dv and the operands of 32 keys take 420 registers.
+// WHAT: 1 dv, 2 dk, 3 both.  Of heads of 128 dk alone takes a wave's 512 registers: there dv and dk are summed by a launch each.
+// 118 us for 4 x 2047 causal tokens, 8 heads of 64 over 128 and 4 key heads, ragged (41 Gflop, 350 Tflop/s), bound like the kernel above; one wave
+// a SIMD, because dk, dv and the operands of 32 keys take 410 registers.
 template <typename T, int DT, int WHAT>
 __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
     constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT, NW = 4, QT = 64;
@@ -959,7 +960,7 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {
 }
 
 // What the kernel of the centres has left of each 32 queries, joined in a fixed order; a workgroup each.
-// dlam[h] = - sum over sequences and queries of D2.  4 us for 8 heads of 8188 queries, where reading all of D2 here took 11.
+// dlam[h] = - sum over sequences and queries of D2.  4.5 us for 8 heads of 8188 queries, where reading all of D2 here took 11.
 // Behind them, for each sequence and key head: a power of two by which |dP - D| max(1, |lam|), at most twice the largest |dP|, stays within 2^15 in all its
 // queries.  dS goes to the matrix units multiplied by it: f16, which ends at 65504 and has all its digits down to 2^-14, then neither overflows nor loses
 // digits of weights above 2^-29, whatever factor the loss is scaled by.  (bf16 has the same exponents as 32 bits: to it this changes nothing.)
@@ -1005,7 +1006,7 @@ Plan plan_of(const bndm_attention_shape &s) {
     const int64_t rows = s.Nq * p.heads_per_row;
     p.waves = rows <= 32 ? 1 : 4;
     const int64_t tiles = ceil_div64(rows, 32 * p.waves) * (s.H / p.heads_per_row) * s.B;
-    // parts of the keys: as many as fill 256 CUs with four one-wave workgroups or one of four waves, of 256 keys at least
+    // parts of the keys: as many as give 256 CUs four workgroups of two waves or one of eight, of 256 keys at least
     const int64_t want = p.waves == 1 ? 1024 : 256;
     int64_t splits = tiles >= want ? 1 : ceil_div64(want, tiles);
     const int64_t most = s.Nk / 256 < 1 ? 1 : s.Nk / 256;

@@ -7,14 +7,18 @@
 // One kernel takes all three: an operand whose rows run along the summed index is read from LDS as rows, one whose rows run across it
 // by transposing LDS reads, so no operand is copied into another layout first.  Few rows go to a kernel of their own, which reads the
 // weights straight into registers.
+//
+// Sums are 32 bits.  16 bits are, beside inputs and results: the kept z = x W^T + b, whose slope is taken (of 32 bits it would be twice the memory that a step
+// keeps), and dz, because the matrix units multiply 16-bit operands.  Gradients are 1.4 times as far off as their own rounding leaves them.
 #include "tokens_common.hpp"
 
 namespace bndm {
 namespace {
 
 // ---------------------------------------------------------------------------------------------- activation
-// Phi(-|z|) = exp(-z^2 / 2) t P(t) / 2 with t = 1 / (1 + 0.3 |z| / sqrt 2): P was fitted to exp(x^2) erfc(x) over x >= 0, least largest
-// relative error 2.0e-8 in exact arithmetic, 4.9e-7 in 32 bits, in the far tail too, where 1 + erf(z) has nothing left.
+// Phi(-|z|) = exp(-z^2 / 2) t P(t) / 2 with t = 1 / (1 + 0.3 |z| / sqrt 2): P was fitted to exp(x^2) erfc(x).  With these coefficients it is off by
+// 4.5e-8 of itself at most up to |z| = 14 (past which Phi(-|z|) is no normal number of 32 bits).  In 32 bits the whole is off by 5e-7 below
+// |z| = 2, 1e-6 below 4 and 8e-6 near 13, where the rounding of the exponent is what counts; 1 + erf(z) has nothing left there.
 struct Gauss { float below, density; };          // Phi(z), exp(-z^2 / 2) / sqrt(2 pi)
 __device__ __forceinline__ Gauss gauss(float z) {
     const float t = __builtin_amdgcn_rcpf(1.0f + 0.21213203435596426f * fabsf(z));
@@ -124,8 +128,8 @@ __device__ __forceinline__ void finish8(const Epilogue &e, T *c, int64_t m, int6
 // The tiles of a step of 32 of the summed index are copied into LDS three steps ahead of the products: with one step of 64 ahead, in the
 // same 128 KB, 137 Gflop took 165 us, this way 131.
 // 256 x 256 tiles are bound by the chip's power and the matrix units, and by a tile's end, which nothing overlaps: 16384 x 4096 x 1024 takes
-// 126 us with W across (1090 Tflop/s; the library's product takes 120), dW in four parts 127 and 13 to join them (980), 16384 x 1024 x 4096 with
-// gelu and z kept 205 (670).  32768 x 512 x 512 with a residual takes 28 us, for 101 MB (3.6 TB/s).
+// 132 us with W across (1040 Tflop/s; 128 at its least, the library's product 120), dW in four parts 132 and 14 to join them (940), 16384 x 1024 x 4096 with
+// gelu and z kept 216 (640).  32768 x 512 x 512 with a residual takes 29 us, for 101 MB (3.5 TB/s).
 constexpr int BK = 32;
 
 // how operands come in: pieces of 16 bytes straight into LDS; through registers; element by element (rows of less than 8)
@@ -588,7 +592,7 @@ size_t gemm_bytes(int64_t M, int64_t N, int64_t K, bool rows_ok) {
 }
 
 // ---------------------------------------------------------------------------------------------- dz = dy act'(z), column sums
-// Bound by memory: 402 MB in 83 us (4.8 TB/s).
+// Bound by memory: 402 MB in 91 us (4.4 TB/s).
 // A workgroup takes 256 columns x a run of rows, 8 columns a thread and 8 rows at a time.  Column sums are of the unrounded dz, one row
 // of partial sums for each run, added up in a fixed order by the second kernel.
 constexpr int DZ_COLS = 256;

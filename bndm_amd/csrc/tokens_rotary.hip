@@ -1,8 +1,8 @@
 // Rotary positions on several axes.  Pair (a, b) of a head turns by the angle t = position[axis] * base^(-i / s):
 //   a' = a cos t - b sin t,   b' = a sin t + b cos t;   the backward pass is the same with -t.
 //
-// Bound by memory: every element is read and written once, 3 operations each.  8 x 4096 tokens of 64 heads of 64 in f16 take 104 us
-// (5.2 TB/s; a large copy moves 5.1), 2 x 20250 tokens of 32 heads of 96 in f32 176 us (5.7 TB/s).  A workgroup takes a run of tokens and forms their
+// Bound by memory: every element is read and written once, 3 operations each.  8 x 4096 tokens of 64 heads of 64 in f16 take 110 us
+// (4.9 TB/s; a large copy moves 5.1), 2 x 20250 tokens of 32 heads of 96 in f32 178 us (5.6 TB/s).  A workgroup takes a run of tokens and forms their
 // cosines and sines once, in LDS, for all heads of q and k; then its threads stream the heads in 16-byte pieces.  Angles are formed
 // in 64 bits, as revolutions whose whole part is dropped before rounding to 32: position * frequency loses 2^-24 of a far position
 // (0.06 radians at 10^6), which no later step can give back.
