@@ -11,8 +11,9 @@
 // A kernel for D_m, one for the queries and one for the keys, each with the sums it owns in registers: no atomics, and the same result every
 // time.
 //
-// Statistics, sums and gradients' sums are 32 bits.  The matrix units take products of 16-bit operands: the forward pass's weights go there in two
-// parts, P as rounded and what that left off, the gradients' (P1 - lam P2 for dv, dS) rounded once, like a value that is stored.
+// Statistics, sums and gradients' sums are 32 bits.  The matrix units take products of 16-bit operands.  Where a sum cancels, its weights go there
+// in two parts, as rounded and what that left off: P in the forward pass (the maps' common part), dS in dq (a row's dS adds up to 0: the keys'
+// common part).  P1 - lam P2 for dv and dS for dk are rounded once, like a value that is stored.
 #include "tokens_common.hpp"
 #include <cmath>
 
@@ -124,6 +125,13 @@ __device__ __forceinline__ void place(int id, int units, int tiles, int &unit, i
 // registers 8 s .. 8 s + 7 of a result tile as an operand whose k are rows 16 s .. 16 s + 15 in that order
 template <typename T> __device__ __forceinline__ s16x8 as_operand(const f32x16 &p, int s) {
     return pack8<T>(p[8 * s], p[8 * s + 1], p[8 * s + 2], p[8 * s + 3], p[8 * s + 4], p[8 * s + 5], p[8 * s + 6], p[8 * s + 7]);
+}
+
+// what rounding to `p` left off them, as an operand likewise
+template <typename T> __device__ __forceinline__ s16x8 rest_of(f32x16 x, const s16x8 &p, int s) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { const short i = p[e]; x[8 * s + e] -= widen<T>(i); }        // (exact)
+    return as_operand<T>(x, s);
 }
 
 __device__ __forceinline__ int tile_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
@@ -322,10 +330,7 @@ __global__ __launch_bounds__(128 * NQ, DT == 32 || (DT == 64 && NQ == 4) ? 4 : 2
             total += sum;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                const s16x8 pf = as_operand<T>(s[0], x);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) { const short p = pf[e]; s[0][8 * x + e] -= widen<T>(p); }     // (exact)
-                const s16x8 rest = as_operand<T>(s[0], x);
+                const s16x8 pf = as_operand<T>(s[0], x), rest = rest_of<T>(s[0], pf, x);
 #pragma unroll
                 for (int v = 0; v < DV / 32; ++v) {
                     const s16x8 column = values.read(now + 2 * K_BYTES, 32 * t + 16 * x, v);
@@ -454,7 +459,7 @@ template <typename T> __global__ __launch_bounds__(512) void attention_join_kern
 // is off by is what dq shows: from outputs rounded to 16 bits, D' = do . o_m, scores of deviation 6 gave a bf16 dq as far off as it is long.
 // So a pass over the keys forms  D_m = D' + sum_j P_mj (dP_j - D')  in 32 bits.  (Of the differences: what log-sum-exp of large scores is
 // off by makes the weights' sum 1 + e, and counts here as e (D - D'), not as e D.)
-// 68 us for 4 x 2047 causal tokens and 8 heads of 64 over 128 of ragged lengths (21 Gflop, 300 Tflop/s): exponentials, the arithmetic around
+// 72 us for 4 x 2047 causal tokens and 8 heads of 64 over 128 of ragged lengths (21 Gflop, 290 Tflop/s): exponentials, the arithmetic around
 // them and the products take about as long as one another, and three waves a SIMD run them beside one another.  Done in the next kernel, with the registers that its
 // sums hold, it took as long with two.
 template <typename T, int DT, int KT>
@@ -586,8 +591,9 @@ __global__ __launch_bounds__(THREADS, DT == 32 ? 4 : DT == 64 ? 3 : 2) void atte
 
 // ---------------------------------------------------------------------------------------------- gradients of the queries
 // As the forward pass: a lane holds one query, dS^T is at once the right operand of  dq^T += k^T dS^T.
-// 68 us for 4 x 2047 causal tokens and 8 heads of 64 over 128 of ragged lengths (31 Gflop, 460 Tflop/s): half of a wave's time goes to
-// exponentials and the arithmetic between the products.
+// dS in two parts: rounded once, dq of bf16 keys that have six times their deviation in common was off by 1.2e-2 of its length (storing it: 1.6e-3).  88 us for 4 x 2047
+// causal tokens and 8 heads of 64 over 128 of ragged lengths (42 Gflop, 470 Tflop/s), 73 with dS in one part: half of a wave's time goes to exponentials and the
+// arithmetic between the products.
 template <typename T, int DT, int KT>
 __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 128 ? 1 : 2, DT == 128 ? 1 : 2))) void attention_dq_kernel(Args a) {
     constexpr int CK = DT / 8, CV = DT / 4, DV = 2 * DT, NW = 4;
@@ -684,9 +690,13 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
                 }
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    const s16x8 ds = as_operand<T>(s[0], x);
+                    const s16x8 ds = as_operand<T>(s[0], x), rest = rest_of<T>(s[0], ds, x);
 #pragma unroll
-                    for (int d = 0; d < DT / 32; ++d) acc[m][d] = mfma32<T>(key_columns.read(now + m * K_BYTES, 32 * t + 16 * x, d), ds, acc[m][d]);
+                    for (int d = 0; d < DT / 32; ++d) {
+                        const s16x8 column = key_columns.read(now + m * K_BYTES, 32 * t + 16 * x, d);
+                        acc[m][d] = mfma32<T>(column, ds, acc[m][d]);
+                        acc[m][d] = mfma32<T>(column, rest, acc[m][d]);
+                    }
                 }
             }
         }
@@ -712,7 +722,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(DT == 1
 // head that reads them pass through LDS, 64 at a time, so shared heads' gradients are summed here.  Two waves take the first half of the
 // queries in a tile, two the second; their sums are added at the end, in order.
 // WHAT: 1 dv, 2 dk, 3 both.  Of heads of 128 dk alone takes a wave's 512 registers: there dv and dk are summed by a launch each.
-// 118 us for 4 x 2047 causal tokens, 8 heads of 64 over 128 and 4 key heads, ragged (41 Gflop, 350 Tflop/s), bound like the kernel above; one wave
+// 127 us for 4 x 2047 causal tokens, 8 heads of 64 over 128 and 4 key heads, ragged (41 Gflop, 330 Tflop/s), bound like the kernel above; one wave
 // a SIMD, because dk, dv and the operands of 32 keys take 410 registers.
 template <typename T, int DT, int WHAT>
 __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(Args a) {

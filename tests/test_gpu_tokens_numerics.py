@@ -33,7 +33,8 @@ def on_gpu(values):
 
 def attention_in_64_bits(q, k, v, lam, seen, dout=None, scale=None):
     """-> {name: (value, bound)} as R.attention, but the weights, the outputs and the sums of weights times their gradients are held in 32
-    bits (weights in two parts of 16): what is rounded to 16 bits is the results, the weights dv is formed of, and scale dS."""
+    bits (weights, and dS on its way to dq, in two parts of 16): what is rounded to 16 bits is the results, the weights dv is formed of, and
+    the dS that dk is."""
     dtype, u, tiny = q.dtype, R.unit(q.dtype), R.smallest(q.dtype)
     b, nq, maps, d = q.shape
     nk, hk, dv = v.shape[1:]
@@ -64,7 +65,7 @@ def attention_in_64_bits(q, k, v, lam, seen, dout=None, scale=None):
         return out
     g = dout.double().transpose(1, 2)
     gv, mag = g @ v64.transpose(-1, -2), g.abs() @ v64.abs().transpose(-1, -2)
-    ds, off, sums = [], [], []
+    ds, off, part_off, sums = [], [], [], []
     for pm, em, f in ((p1, e1, torch.ones_like(l)), (p2, e2, -l)):
         big = pm * em
         centre = (pm * gv).sum(-1, keepdim=True)
@@ -74,9 +75,10 @@ def attention_in_64_bits(q, k, v, lam, seen, dout=None, scale=None):
         sums.append((centre, off_d))
         x = pm * (gv - centre) * f
         ds.append(x)
-        off.append(f.abs() * (pm * (raw + off_d + 4 * E * (gv.abs() + centre.abs())) + (em + (pm * em).sum(-1, keepdim=True)) * pm * (gv - centre).abs())
-                   + u * x.abs() + tiny / scale * (pm > 0))
-    ds, off = torch.stack(ds, 2).flatten(1, 2), torch.stack(off, 2).flatten(1, 2)
+        err = f.abs() * (pm * (raw + off_d + 4 * E * (gv.abs() + centre.abs())) + (em + (pm * em).sum(-1, keepdim=True)) * pm * (gv - centre).abs())
+        off.append(err + u * x.abs() + tiny / scale * (pm > 0))
+        part_off.append(err + u * u * x.abs() + tiny / scale * (pm > 0))
+    ds, off, part_off = (torch.stack(t, 2).flatten(1, 2) for t in (ds, off, part_off))
 
     def shared(t, two):
         t = t.unflatten(1, (hk, per, 2)) if two else t.unflatten(1, (hk, per))
@@ -85,7 +87,7 @@ def attention_in_64_bits(q, k, v, lam, seen, dout=None, scale=None):
     def add(key, grad, err, size, n):
         out[key] = (grad.transpose(1, 2), (err + n * E * size + u * (grad.abs() + err) + tiny).transpose(1, 2))
 
-    add("q", ds @ k64 * scale, off @ k64.abs() * scale, ds.abs() @ k64.abs() * scale, nk)
+    add("q", ds @ k64 * scale, part_off @ k64.abs() * scale, ds.abs() @ k64.abs() * scale, nk)
     add("k", shared(ds.transpose(-1, -2) @ q64, True) * scale, shared(off.transpose(-1, -2) @ q64.abs(), True) * scale,
         shared(ds.abs().transpose(-1, -2) @ q64.abs(), True) * scale, nq * per)
     off_w = u * w.abs() + p1 * e1 + l.abs() * p2 * e2 + (p1 * (p1 * e1).sum(-1, keepdim=True) + l.abs() * p2 * (p2 * e2).sum(-1, keepdim=True)) + tiny * (p1 > 0)
@@ -111,6 +113,20 @@ def test_gradients_of_peaked_rows(T, b, nq, nk, h, hk, d, dv, causal, std, dtype
     leaves = [t.cuda().requires_grad_() for t in (q, k, v, lam)]
     o = T.differential_attention(*leaves, causal=causal)
     want = attention_in_64_bits(q, k, v, lam, R.visible(nq, nk, None, causal, None, b), g)
+    for name, got in zip(("q", "k", "v", "lam"), torch.autograd.grad(o, leaves, g.cuda())):
+        R.assert_within(got, *want[name], "d" + name)
+
+
+@pytest.mark.parametrize("b,nq,nk,h,hk,d,causal", [(1, 70, 60, 2, 1, 64, False), (2, 40, 530, 2, 2, 8, False), (1, 200, 200, 2, 1, 32, True), (2, 33, 20, 1, 1, 128, False)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_gradients_of_keys_with_a_common_part(T, b, nq, nk, h, hk, d, causal, dtype):
+    """A row's dS adds up to 0: what all keys have in common (a projection's bias) goes out of dq, and what dS was rounded by, times that, does not."""
+    q, v, g = normal(1, b, nq, 2 * h, d, dtype=dtype), normal(3, b, nk, hk, 2 * d, dtype=dtype), normal(4, b, nq, h, 2 * d, dtype=dtype)
+    k = (normal(2, b, nk, 2 * hk, d, dtype=F32) + 6 * normal(5, d, dtype=F32)).to(dtype)
+    lam = torch.full((h,), 0.5)
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v, lam)]
+    o = T.differential_attention(*leaves, causal=causal, scale=0.25 * d ** -0.5)
+    want = attention_in_64_bits(q, k, v, lam, R.visible(nq, nk, None, causal, None, b), g, scale=0.25 * d ** -0.5)
     for name, got in zip(("q", "k", "v", "lam"), torch.autograd.grad(o, leaves, g.cuda())):
         R.assert_within(got, *want[name], "d" + name)
 
