@@ -16,8 +16,8 @@ def sources():
 
 
 def test_no_source_writes_through_the_scalar_data_cache():
-    """Its stores, atomics, write-back and discard are not to be used on the machines this runs on, and a tree whose files so much as name them is not
-    taken there: neither kernels nor the simulator's table of instructions may."""
+    """Kernels write through vector stores alone: the scalar cache's stores, atomics, write-back and discard have no place in them, nor a name in the
+    simulator's table of instructions."""
     names = re.compile(r"\bs_(?:dcache_(?:wb|discard)|(?:buffer_|scratch_)?(?:store_dword|atomic_))")
     paths = list(sources())
     assert len(paths) > 80
